@@ -610,6 +610,104 @@ lbh_status lbh_moe_create_cached(lbh_ctx *ctx, lbh_expert_cache *cache, const lb
 lbh_status lbh_moe_forward_leased(lbh_ctx *ctx, lbh_moe *moe, const lbh_expert_lease *leases, const float *coefs,
                                   size_t n_routed, const float *x_dev, float *y_dev);
 
+/* ---- dense blocks in 8-bit integers ---------------------------------------------
+ * What stands before and around the matrices of a dense layer: the RMS norm of
+ * the residual stream with 8-bit outputs, and products of int8 rows (one scale a
+ * token) with int8 channels (one scale a channel).  The reference's dense block
+ * is residual_add_in_place and rms_norm_into (crates/bridge-kernels-reference/
+ * src/norm.rs) around gemv_into on Q8_K rows; the Q8_K form below feeds this
+ * header's Q8_K products bit for bit, the int8 forms have no counterpart there.
+ *
+ * Row operands are float32, binary16 or bfloat16 (LBH_F32, LBH_F16, LBH_BF16);
+ * strides count elements, are at least the row's length, and bytes between the
+ * rows are neither read for their value nor written.  Pointers need the alignment
+ * of their element; rows whose address and stride are multiples of 16 bytes are
+ * the fast ones.  Outputs may share no byte with each other or with an input,
+ * except where "in place" is said.  rows / n_tokens == 0 does nothing.  At most
+ * 2^20 rows a call. */
+#define LBH_F16 1
+#define LBH_BF16 30
+
+/* [async] RMS norm of `rows` rows of n elements:
+ *   h = hidden + delta           (delta NULL: hidden), rounded to float32 and to `type`
+ *   v = h * weight / sqrt(mean(h^2) + eps)
+ * hidden_out (optional) receives h; it may be hidden or delta themselves, in
+ * place.  y receives v in y_type.  Sums and products are in 64 bits, and v is
+ * rounded to float32 and from there to y_type: results do not depend on the
+ * launch shape.  eps > 0.  n up to 2^23. */
+lbh_status lbh_rms_norm_rows(lbh_ctx *ctx, int32_t type, const void *hidden_dev, size_t hidden_stride,
+                             const void *delta_dev, size_t delta_stride, const float *weight_dev, double eps,
+                             size_t rows, size_t n, void *hidden_out_dev, size_t hidden_out_stride, int32_t y_type,
+                             void *y_dev, size_t y_stride, lbh_error *err);
+/* [async] The same with the Q8_K rows of v in float32 (lbh_quantize_q8_k_rows: rows
+ * * (n / 256) * 292 bytes, 4-byte aligned; n % 256 == 0, n <= 16384).  y optional. */
+lbh_status lbh_rms_norm_q8_k_rows(lbh_ctx *ctx, int32_t type, const void *hidden_dev, size_t hidden_stride,
+                                  const void *delta_dev, size_t delta_stride, const float *weight_dev, double eps,
+                                  size_t rows, size_t n, void *hidden_out_dev, size_t hidden_out_stride, int32_t y_type,
+                                  void *y_dev, size_t y_stride, uint8_t *encoded_dev, lbh_error *err);
+/* [async] The same with int8 rows of v: scales_dev[t] = max |v| / 127 rounded to
+ * float32, q = v / scale to the nearest integer, ties to even.  A row whose scale
+ * is below 2^-126 (the least normal float32) gets scale 0 and zeros; a row with a
+ * value that is not finite, or whose scale would not be, gets scale NaN and zeros.
+ * y optional. */
+lbh_status lbh_rms_norm_i8_rows(lbh_ctx *ctx, int32_t type, const void *hidden_dev, size_t hidden_stride,
+                                const void *delta_dev, size_t delta_stride, const float *weight_dev, double eps,
+                                size_t rows, size_t n, void *hidden_out_dev, size_t hidden_out_stride, int32_t y_type,
+                                void *y_dev, size_t y_stride, int8_t *q_dev, size_t q_stride, float *scales_dev,
+                                lbh_error *err);
+/* [async] int8 rows of x itself (v = x in the rules above). */
+lbh_status lbh_quantize_i8_rows(lbh_ctx *ctx, int32_t type, const void *x_dev, size_t x_stride, size_t rows, size_t n,
+                                int8_t *q_dev, size_t q_stride, float *scales_dev, lbh_error *err);
+
+/* An int8 matrix resident in HBM in the product's tile layout: `rows` channels of
+ * k weights with a scale each, or a gated pair (gate and up of one shape).
+ * k <= 131071, so that k * 128 * 128 sums are exact in 32 bits; rows <= 2^26. */
+typedef struct lbh_i8_matrix lbh_i8_matrix;
+
+/* [sync] weights [rows][k] row-major, scales [rows]; host memory when on_device ==
+ * 0, device memory otherwise.  A scale that is not finite is refused
+ * (LBH_NON_FINITE_SCALE: row, bits, field 0 = the matrix or the gate, 1 = the up). */
+lbh_status lbh_i8_matrix_create(lbh_ctx *ctx, size_t rows, size_t k, const int8_t *weights, const float *scales,
+                                int32_t on_device, lbh_i8_matrix **out, lbh_error *err);
+lbh_status lbh_i8_matrix_create_gated(lbh_ctx *ctx, size_t rows, size_t k, const int8_t *gate, const float *gate_scales,
+                                      const int8_t *up, const float *up_scales, int32_t on_device, lbh_i8_matrix **out,
+                                      lbh_error *err);
+/* [sync] The int8 form of an uploaded matrix (Q4_K, Q5_K, IQ2_S, IQ3_S or F32), each
+ * row's decoded values quantized as by lbh_quantize_i8_rows; with `up`, the gated
+ * pair of m (the gate) and up, of one shape.  An F32 row with a value that is not
+ * finite is refused as above.  The packed matrices stay as they are. */
+lbh_status lbh_i8_matrix_from_packed(lbh_ctx *ctx, const lbh_matrix *m, const lbh_matrix *up, lbh_i8_matrix **out,
+                                     lbh_error *err);
+lbh_status lbh_i8_matrix_destroy(lbh_i8_matrix *m);
+/* [sync] The weights [rows][k] and scales [rows] back on the host: which = 0 the
+ * matrix or the pair's gate, 1 the pair's up. */
+lbh_status lbh_i8_matrix_read(lbh_ctx *ctx, const lbh_i8_matrix *m, int32_t which, int8_t *weights_host,
+                              size_t weights_len, float *scales_host, size_t scales_len, lbh_error *err);
+size_t lbh_i8_matrix_rows(const lbh_i8_matrix *m);
+size_t lbh_i8_matrix_k(const lbh_i8_matrix *m);
+int32_t lbh_i8_matrix_gated(const lbh_i8_matrix *m);
+size_t lbh_i8_matrix_device_bytes(const lbh_i8_matrix *m);
+
+/* Workspace bytes that serve every call of the matrix with up to n_tokens tokens.
+ * x rows at multiples of 16 bytes with k % 16 == 0 need none (NULL).  Calls that
+ * may run at once (two streams, two captured graphs) need a workspace each. */
+size_t lbh_gemm_i8_workspace_bytes(const lbh_i8_matrix *m, size_t n_tokens);
+
+/* [async] y[t][c] = residual[t][c] + sum_i x[t][i] w[c][i] * x_scales[t] * scale[c]:
+ * the sum exact in int32, converted and scaled in float32 (the token's scale, then
+ * the channel's), the residual (optional, of y_type; it may be y itself, in place)
+ * added in float32, rounded to y_type once.  x_stride <= 2^23.  A token whose scale
+ * is NaN gives NaN.  The same bits for any number of tokens in the call. */
+lbh_status lbh_gemm_i8(lbh_ctx *ctx, const lbh_i8_matrix *m, const int8_t *x_dev, size_t x_stride,
+                       const float *x_scales_dev, size_t n_tokens, int32_t y_type, void *y_dev, size_t y_stride,
+                       const void *residual_dev, size_t residual_stride, void *workspace_dev, size_t workspace_len,
+                       lbh_error *err);
+/* [async] The gated pair's SwiGLU: h[t][c] = g / (1 + exp(-g)) * u with g and u the
+ * products above of the gate and the up, in float32, rounded to h_type once. */
+lbh_status lbh_gemm_i8_swiglu(lbh_ctx *ctx, const lbh_i8_matrix *m, const int8_t *x_dev, size_t x_stride,
+                              const float *x_scales_dev, size_t n_tokens, int32_t h_type, void *h_dev, size_t h_stride,
+                              void *workspace_dev, size_t workspace_len, lbh_error *err);
+
 /* ---- diagnostics ------------------------------------------------------------- */
 
 /* Polls of the router chains' bounded LDS-ring waits before they give up (0: the

@@ -359,7 +359,41 @@ __global__ void __launch_bounds__(256, THREE ? 3 : 2) k_gemv_dequant(DequantArgs
     }
 }
 
+// The decoded values of rows r0 .. r0 + n - 1, one group of 32 a thread (what
+// the DequantF32 matvec multiplies by, times one).
+template <int TY>
+__global__ void __launch_bounds__(256) k_dequant_rows(MatView m, long long r0, long long n, float *out) {
+    const Planes P = make_planes(m.planes, m.units, m.bytes);
+    const void *grid = TY == T_IQ2_S ? (const void *)c_iq2s_grid : (const void *)c_iq3s_grid;
+    float one[32], v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) one[i] = 1.0f;
+    const long long total = n * m.nb * 8;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const int sub = (int)(i & 7);
+        const long long u = r0 * m.nb + (i >> 3);
+        dequant_group<TY>(dequant_load<TY>(P, (uint32_t)u, sub), sub, grid, one, v);
+        float4 *dst = reinterpret_cast<float4 *>(out + i * 32);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dst[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    }
+}
+
 // ---------------------------------------------------------------- launchers
+
+hipError_t launch_dequant_rows(const MatView &m, long long r0, long long n, float *out, hipStream_t s) {
+    if (n <= 0) return hipSuccess;
+    long long grid = (n * m.nb * 8 + 255) / 256;
+    grid = grid > 16384 ? 16384 : grid;
+    switch (m.type) {
+    case T_IQ2_S: hipLaunchKernelGGL(k_dequant_rows<T_IQ2_S>, dim3((int)grid), dim3(256), 0, s, m, r0, n, out); break;
+    case T_IQ3_S: hipLaunchKernelGGL(k_dequant_rows<T_IQ3_S>, dim3((int)grid), dim3(256), 0, s, m, r0, n, out); break;
+    case T_Q4_K: hipLaunchKernelGGL(k_dequant_rows<T_Q4_K>, dim3((int)grid), dim3(256), 0, s, m, r0, n, out); break;
+    case T_Q5_K: hipLaunchKernelGGL(k_dequant_rows<T_Q5_K>, dim3((int)grid), dim3(256), 0, s, m, r0, n, out); break;
+    default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
 
 hipError_t launch_dot_ggml(int ty, const uint8_t *w, long long rows, int nb, const uint8_t *q8, float *y,
                            const DevStatus *st, hipStream_t s) {

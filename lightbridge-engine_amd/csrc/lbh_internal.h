@@ -222,6 +222,41 @@ struct BatchArgs {
     float *xd_mx, *hd_mx_r, *hd_mx_s;
 };
 
+// ------------------------------------------- norm and 8-bit integer products
+
+// Rows through the norm (norm != 0) or as they are, and the outputs asked for
+// (each may be NULL).  Strides are in elements.
+struct NormArgs {
+    const void *hidden, *delta;   // [rows][n] of `type`; delta optional
+    void *hidden_out;             // hidden + delta, of `type`
+    const float *weight;          // [n]; NULL: ones
+    void *y;                      // [rows][n] of y_type
+    uint8_t *q8k;                 // [rows][n / 256] Q8_K blocks, rows adjacent (n % 256 == 0, n <= 16384)
+    int8_t *q;                    // [rows][n]
+    float *scale;                 // [rows]
+    long long hidden_stride, delta_stride, hidden_out_stride, y_stride, q_stride;
+    long long rows;
+    int32_t n, type, y_type, norm;
+    double eps;
+};
+constexpr int NORM_MAX_Q8K = 16384;   // a row of Q8_K input waits in LDS
+
+// 8-bit integer product (lbh_i8.hip).  Strides are in elements; x rows start
+// at multiples of 16 bytes.
+struct I8Args {
+    const uint8_t *w;        // tiles: [channel groups][kt][1024]
+    const float *ws;         // [channel groups * 16]
+    const int8_t *x;         // [n_tokens][k]
+    const float *xs;         // [n_tokens]
+    void *y;                 // [n_tokens][rows] of out_type
+    const void *residual;    // optional (plain product)
+    long long x_stride, y_stride, residual_stride;
+    int32_t n_tokens, rows, k, kt;
+    int32_t out_type, gated;
+    int32_t vec_out;         // y and residual: four elements at any multiple of four are one aligned word
+    int32_t cu_count;
+};
+
 // Batch selection: top-k of each token's finished logits (select_route).
 struct RouteBatchArgs {
     RouterArgs r;               // n_experts, top_k, mode, weight_scale, bias
@@ -232,6 +267,17 @@ struct RouteBatchArgs {
     int32_t n_tokens;
     int32_t pad;
 };
+
+hipError_t launch_norm_rows(const NormArgs &a, hipStream_t s);
+// Weight rows [rows][k] and scales [rows] into or out of the product's tiles:
+// channel group g of this matrix is group g * step + part of the tiles.
+hipError_t launch_i8_layout(const int8_t *rowmajor, uint8_t *tiles, const float *scales, float *tile_scales,
+                            long long rows, long long k, long long kt, int step, int part, int to_tiles, hipStream_t s);
+hipError_t launch_i8_align_rows(const int8_t *x, long long stride, int k, int pitch, long long n, uint8_t *out,
+                                hipStream_t s);
+hipError_t launch_i8_product(const I8Args &a, hipStream_t s);
+// out[i][c] = the exact f32 decode of element c of row r0 + i (quantized types).
+hipError_t launch_dequant_rows(const MatView &m, long long r0, long long n, float *out, hipStream_t s);
 
 size_t gemm_a_bytes(int rows, int nb);
 size_t gemm_b_bytes(int n_tokens, int nb);

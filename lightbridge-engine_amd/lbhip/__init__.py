@@ -20,6 +20,7 @@ PKG_DIR = Path(__file__).resolve().parent.parent
 LIB_PATH = PKG_DIR / "liblightbridge_hip.so"
 
 F32, Q4_K, Q5_K, Q8_K, IQ3_S, IQ2_S = 0, 12, 13, 15, 21, 22
+F16, BF16 = 1, 30   # row operands of the norm and the int8 products
 Q8_K_BLOCK_ELEMENTS, Q8_K_BLOCK_BYTES = 256, 292
 BLOCK_BYTES = {Q4_K: 144, Q5_K: 176, IQ2_S: 82, IQ3_S: 110}
 
@@ -150,6 +151,22 @@ def lib() -> C.CDLL:
             "lbh_expert_cache_read_record": ([p, p, p, sz, E], i32),
             "lbh_moe_create_cached": ([p, p, p, p, p, C.POINTER(p), E], i32),
             "lbh_moe_forward_leased": ([p, p, p, p, sz, p, p], i32),
+            "lbh_rms_norm_rows": ([p, i32, p, sz, p, sz, p, C.c_double, sz, sz, p, sz, i32, p, sz, E], i32),
+            "lbh_rms_norm_q8_k_rows": ([p, i32, p, sz, p, sz, p, C.c_double, sz, sz, p, sz, i32, p, sz, p, E], i32),
+            "lbh_rms_norm_i8_rows": ([p, i32, p, sz, p, sz, p, C.c_double, sz, sz, p, sz, i32, p, sz, p, sz, p, E], i32),
+            "lbh_quantize_i8_rows": ([p, i32, p, sz, sz, sz, p, sz, p, E], i32),
+            "lbh_i8_matrix_create": ([p, sz, sz, p, p, i32, C.POINTER(p), E], i32),
+            "lbh_i8_matrix_create_gated": ([p, sz, sz, p, p, p, p, i32, C.POINTER(p), E], i32),
+            "lbh_i8_matrix_from_packed": ([p, p, p, C.POINTER(p), E], i32),
+            "lbh_i8_matrix_destroy": ([p], i32),
+            "lbh_i8_matrix_read": ([p, p, i32, p, sz, p, sz, E], i32),
+            "lbh_i8_matrix_rows": ([p], sz),
+            "lbh_i8_matrix_k": ([p], sz),
+            "lbh_i8_matrix_gated": ([p], i32),
+            "lbh_i8_matrix_device_bytes": ([p], sz),
+            "lbh_gemm_i8_workspace_bytes": ([p, sz], sz),
+            "lbh_gemm_i8": ([p, p, p, sz, p, sz, i32, p, sz, p, sz, p, sz, E], i32),
+            "lbh_gemm_i8_swiglu": ([p, p, p, sz, p, sz, i32, p, sz, p, sz, E], i32),
             "lbh_matrix_create_streamed": ([p, i32, sz, sz, p, p, C.POINTER(p), E], i32),
         }
         for name, (args, res) in sig.items():
@@ -163,6 +180,29 @@ def _dev_ptr(t) -> int:
     import torch
     assert isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous(), "expected a contiguous CUDA tensor"
     return t.data_ptr()
+
+
+def _rows(t, dtype=None):
+    """(address, row stride) of a two-dimensional CUDA tensor with adjacent row elements; (None, 0) for None."""
+    import torch
+    if t is None:
+        return None, 0
+    assert isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2, "expected a two-dimensional CUDA tensor"
+    assert t.shape[1] <= 1 or t.stride(1) == 1, "expected rows of adjacent elements"
+    assert dtype is None or t.dtype == dtype, f"expected {dtype}, got {t.dtype}"
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _row_type(t) -> int:
+    import torch
+    ty = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype)
+    assert ty is not None, f"expected float32, float16 or bfloat16 rows, got {t.dtype}"
+    return ty
+
+
+def _like(t, shape, what: str):
+    assert t is None or tuple(t.shape) == tuple(shape), f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}"
+    return t
 
 
 def _call(fn, *args) -> None:
@@ -351,6 +391,86 @@ class HipBackend:
         st = lib().lbh_debug_read_matrix(self.ctx, m.handle, _dev_ptr(sink), grid, unroll, int(slab))
         if st:
             raise KernelError(LbhError(status=st))
+
+    # -- dense blocks in 8-bit integers ----------------------------------------------------
+    def _norm_args(self, hidden, weight, eps, delta, hidden_out, y):
+        """The arguments every norm call begins with, checked against hidden's shape."""
+        import torch
+        n_rows, n = hidden.shape
+        ty = _row_type(hidden)
+        hp, hs = _rows(hidden)
+        dp, ds = _rows(_like(delta, hidden.shape, "delta"), hidden.dtype)
+        op, os_ = _rows(_like(hidden_out, hidden.shape, "hidden_out"), hidden.dtype)
+        yp, ys = _rows(_like(y, hidden.shape, "y"))
+        assert weight.dtype == torch.float32 and weight.numel() == n, "weight: n float32 values"
+        return (self.ctx, ty, hp, hs, dp, ds, _dev_ptr(weight), eps, n_rows, n, op, os_,
+                _row_type(y) if y is not None else ty, yp, ys)
+
+    def rms_norm_rows(self, hidden, weight, eps: float, y, delta=None, hidden_out=None) -> None:
+        """y = RMS norm of hidden (+ delta, stored in hidden_out when given) [rows, n]; row strides are
+        taken from the tensors (asynchronous).  hidden_out may be hidden: the residual stream in place."""
+        _call(lib().lbh_rms_norm_rows, *self._norm_args(hidden, weight, eps, delta, hidden_out, y))
+
+    def rms_norm_q8_k_rows(self, hidden, weight, eps: float, encoded, y=None, delta=None, hidden_out=None) -> None:
+        """rms_norm_rows into Q8_K blocks (rows * n / 256 * 292 bytes), and into y when given."""
+        n_rows, n = hidden.shape
+        assert n % 256 or encoded.numel() * encoded.element_size() == n_rows * (n // 256) * Q8_K_BLOCK_BYTES, "encoded"
+        _call(lib().lbh_rms_norm_q8_k_rows, *self._norm_args(hidden, weight, eps, delta, hidden_out, y),
+              _dev_ptr(encoded))
+
+    def rms_norm_i8_rows(self, hidden, weight, eps: float, q, scales, y=None, delta=None, hidden_out=None) -> None:
+        """rms_norm_rows into int8 rows q [rows, n] with float32 scales [rows], and into y when given."""
+        import torch
+        qp, qs = _rows(_like(q, hidden.shape, "q"), torch.int8)
+        assert scales.dtype == torch.float32 and scales.numel() == hidden.shape[0], "scales: a float32 value a row"
+        _call(lib().lbh_rms_norm_i8_rows, *self._norm_args(hidden, weight, eps, delta, hidden_out, y), qp, qs,
+              _dev_ptr(scales))
+
+    def quantize_i8_rows(self, x, q, scales) -> None:
+        """int8 rows of x [rows, n] with one float32 scale each (max |x| / 127; asynchronous)."""
+        import torch
+        xp, xs = _rows(x)
+        qp, qs = _rows(_like(q, x.shape, "q"), torch.int8)
+        assert scales.dtype == torch.float32 and scales.numel() == x.shape[0], "scales: a float32 value a row"
+        _call(lib().lbh_quantize_i8_rows, self.ctx, _row_type(x), xp, xs, x.shape[0], x.shape[1], qp, qs,
+              _dev_ptr(scales))
+
+    def upload_i8(self, weights, scales) -> "DeviceI8Matrix":
+        """int8 weights [rows, k] with a float32 scale a row, numpy arrays or CUDA tensors."""
+        return DeviceI8Matrix(self, weights, scales)
+
+    def upload_i8_gated(self, gate, gate_scales, up, up_scales) -> "DeviceI8Matrix":
+        """The gate and up projections of one shape, for gemm_i8_swiglu."""
+        return DeviceI8Matrix(self, gate, gate_scales, up, up_scales)
+
+    def i8_from_packed(self, m: "DeviceMatrix", up: "DeviceMatrix | None" = None) -> "DeviceI8Matrix":
+        """The int8 form of an uploaded matrix, or the gated pair of two."""
+        return DeviceI8Matrix.from_packed(self, m, up)
+
+    @staticmethod
+    def gemm_i8_workspace_bytes(m: "DeviceI8Matrix", n_tokens: int) -> int:
+        return lib().lbh_gemm_i8_workspace_bytes(m.handle, n_tokens)
+
+    def _product_args(self, m, q, scales, y, workspace, residual=None):
+        import torch
+        n = q.shape[0]
+        qp, qs = _rows(_like(q, (n, m.k), "q"), torch.int8)
+        yp, ys = _rows(_like(y, (n, m.rows), "y"))
+        rp, rs = _rows(_like(residual, y.shape, "residual"), y.dtype)
+        assert scales.dtype == torch.float32 and scales.numel() == n, "scales: a float32 value a token"
+        wp, wl = (None, 0) if workspace is None else (_dev_ptr(workspace), workspace.numel() * workspace.element_size())
+        return ((self.ctx, m.handle, qp, qs, _dev_ptr(scales), n, _row_type(y), yp, ys), (rp, rs), (wp, wl))
+
+    def gemm_i8(self, m: "DeviceI8Matrix", q, scales, y, workspace=None, residual=None) -> None:
+        """y [tokens, rows] = (residual +) int8 rows q [tokens, k] times the matrix, scaled by token and
+        channel (asynchronous).  workspace: for rows off 16 bytes (gemm_i8_workspace_bytes)."""
+        head, res, ws = self._product_args(m, q, scales, y, workspace, residual)
+        _call(lib().lbh_gemm_i8, *head, *res, *ws)
+
+    def gemm_i8_swiglu(self, m: "DeviceI8Matrix", q, scales, h, workspace=None) -> None:
+        """h [tokens, rows] = silu(gate) * up of int8 rows q times a gated pair (asynchronous)."""
+        head, _, ws = self._product_args(m, q, scales, h, workspace)
+        _call(lib().lbh_gemm_i8_swiglu, *head, *ws)
 
     def f16_to_f32(self, src, dst) -> None:
         _call(lib().lbh_debug_f16_to_f32, self.ctx, _dev_ptr(src), _dev_ptr(dst), src.numel())
@@ -624,6 +744,68 @@ class DeviceMatrix:
     def close(self) -> None:
         if self.handle:
             lib().lbh_matrix_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class DeviceI8Matrix:
+    """int8 channels with a scale each, or a gated pair of them, resident in HBM."""
+
+    def __init__(self, be: HipBackend, weights, scales, up=None, up_scales=None):
+        import torch
+        on_device = isinstance(weights, torch.Tensor)
+        keep, args = [], []
+        for w, s in ((weights, scales), (up, up_scales)):
+            if w is None:
+                continue
+            if on_device:
+                assert w.dtype == torch.int8 and s.dtype == torch.float32, "int8 weights with float32 scales"
+                w, s = w.contiguous(), s.contiguous()
+                args += [_dev_ptr(w), _dev_ptr(s)]
+            else:
+                w, s = np.ascontiguousarray(w), np.ascontiguousarray(s)
+                assert w.dtype == np.int8 and s.dtype == np.float32, "int8 weights with float32 scales"
+                args += [C.c_void_p(w.ctypes.data), C.c_void_p(s.ctypes.data)]
+            assert w.ndim == 2 and tuple(s.shape) == (w.shape[0],), "weights [rows, k], scales [rows]"
+            keep.append((w, s))
+        assert all(k[0].shape == keep[0][0].shape for k in keep), "gate and up of one shape"
+        rows, k = keep[0][0].shape
+        h = C.c_void_p()
+        self.handle = None
+        fn = lib().lbh_i8_matrix_create if len(keep) == 1 else lib().lbh_i8_matrix_create_gated
+        _call(fn, be.ctx, rows, k, *args, 1 if on_device else 0, C.byref(h))
+        self._take(be, h)
+
+    def _take(self, be, h) -> None:
+        self.be, self.handle = be, h
+        self.rows, self.k = lib().lbh_i8_matrix_rows(h), lib().lbh_i8_matrix_k(h)
+        self.gated = bool(lib().lbh_i8_matrix_gated(h))
+        self.device_bytes = lib().lbh_i8_matrix_device_bytes(h)
+
+    @classmethod
+    def from_packed(cls, be: HipBackend, m: "DeviceMatrix", up: "DeviceMatrix | None" = None) -> "DeviceI8Matrix":
+        self = cls.__new__(cls)
+        self.handle = None
+        h = C.c_void_p()
+        _call(lib().lbh_i8_matrix_from_packed, be.ctx, m.handle, up.handle if up is not None else None, C.byref(h))
+        self._take(be, h)
+        return self
+
+    def read(self, which: int = 0):
+        """(weights [rows, k], scales [rows]) on the host; which = 1: the pair's up."""
+        w, s = np.empty((self.rows, self.k), np.int8), np.empty(self.rows, np.float32)
+        _call(lib().lbh_i8_matrix_read, self.be.ctx, self.handle, which, C.c_void_p(w.ctypes.data), w.size,
+              C.c_void_p(s.ctypes.data), s.size)
+        return w, s
+
+    def close(self) -> None:
+        if self.handle:
+            lib().lbh_i8_matrix_destroy(self.handle)
             self.handle = None
 
     def __del__(self):

@@ -1,0 +1,245 @@
+"""int8 products (plain, with the residual, gated) against a plain 64-bit implementation.
+
+The integer sums are exact; what is left are roundings of u = 2^-24: the sum's conversion and the two scales give
+(1 + u)^3, the residual's addition one more of the result, and the output's type half a step of its own."""
+import numpy as np
+import pytest
+
+from lbhip import synth
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def be():
+    import lbhip
+    if not torch.cuda.is_available():
+        pytest.fail("no GPU visible")
+    b = lbhip.HipBackend(0)
+    yield b
+    b.close()
+
+
+def make(tokens, rows, k, seed):
+    r = np.random.default_rng(seed)
+    q = np.clip(np.rint(r.standard_normal((tokens, k)) * 40), -128, 127).astype(np.int8)
+    w = np.clip(np.rint(r.standard_normal((rows, k)) * 40), -128, 127).astype(np.int8)
+    return q, (r.random(tokens) + 0.5).astype(np.float32) / 40, w, ((r.random(rows) + 0.5) / (40 * k ** 0.5)).astype(np.float32)
+
+
+def on_gpu(q, pad=0, offset=0):
+    """Rows `pad` bytes apart, `offset` bytes into a buffer."""
+    t, k = q.shape
+    buf = torch.full((t * (k + pad) + offset + 16,), 111, dtype=torch.int8, device="cuda")
+    view = buf[offset:offset + t * (k + pad)].view(t, k + pad)[:, :k]
+    view.copy_(torch.from_numpy(q))
+    return view
+
+
+def value(q, s, w, ws):
+    return (q.astype(np.float64) @ w.astype(np.float64).T) * s.astype(np.float64)[:, None] * ws.astype(np.float64)
+
+
+def out_step(ty):
+    """Half a step of the output's type relative to the value, and of its least subnormal."""
+    f = torch.finfo(ty)
+    return (0.0 if ty == torch.float32 else f.eps / 2), f.smallest_normal * f.eps / 2
+
+
+def check(got, want, ty, off):
+    """off: the bound on the error of the 32-bit value."""
+    half, least = out_step(ty)
+    g = got.double().cpu().numpy()
+    limit = off * (1 + half) + (np.abs(want) * half + least) * 1.0001
+    bad = ~(np.abs(g - want) <= limit)
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4].tolist(), float(np.nanmax(np.abs(g - want) / limit)))
+
+
+def plain_off(want):
+    return np.abs(want) * 3.001 * U + 2.0 ** -149
+
+
+# tokens: one, the borders of 16-, 32-, 64-, 128- and 256-token tiles; rows and k of every remainder that matters
+PRODUCTS = [(1, 1, 1), (1, 16, 64), (1, 17, 63), (1, 1000, 4096), (2, 5, 15), (3, 255, 129), (7, 33, 1000), (15, 64, 65),
+            (16, 100, 128), (17, 31, 16), (31, 257, 130), (32, 512, 192), (33, 48, 640), (63, 129, 256), (64, 1, 8191),
+            (65, 130, 127), (100, 511, 512), (127, 256, 1024), (128, 260, 384), (129, 16, 2048), (200, 777, 320),
+            (255, 128, 64), (256, 513, 1040), (257, 300, 272), (300, 1025, 768), (513, 260, 96), (1000, 520, 257)]
+
+
+@pytest.mark.parametrize("tokens,rows,k", PRODUCTS)
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+def test_product(be, tokens, rows, k, ty):
+    t = TYPES[ty]
+    q, s, w, ws = make(tokens, rows, k, seed=tokens * 7 + rows * 3 + k)
+    want = value(q, s, w, ws)
+    m = be.upload_i8(w, ws)
+    assert (m.rows, m.k, m.gated) == (rows, k, False)
+    space = torch.zeros(be.gemm_i8_workspace_bytes(m, tokens), dtype=torch.uint8, device="cuda")
+    sd = torch.from_numpy(s).cuda()
+    first = None
+    for pad, offset, ypad in ((0, 0, 0), (-k % 16, 0, 4), (5, 3, 1)):
+        buf = torch.full((tokens, rows + ypad), 7.0, dtype=t, device="cuda")
+        y = buf[:, :rows]
+        be.gemm_i8(m, on_gpu(q, pad, offset), sd, y, space)
+        check(y, want, t, plain_off(want))
+        assert bool((buf[:, rows:] == 7).all())
+        first = y.clone() if first is None else first
+        assert torch.equal(first, y)         # the same bits by every path
+    res = torch.randn(tokens, rows, generator=torch.Generator().manual_seed(k)).to(t).cuda()
+    total = want + res.double().cpu().numpy()
+    off = plain_off(want) + (np.abs(total) + plain_off(want)) * U
+    y = torch.zeros(tokens, rows, dtype=t, device="cuda")
+    be.gemm_i8(m, on_gpu(q), sd, y, space, residual=res)
+    check(y, total, t, off)
+    be.gemm_i8(m, on_gpu(q), sd, res, space, residual=res)    # in place
+    assert torch.equal(res, y)
+    m.close()
+
+
+def test_product_f16_and_columns_of_one_buffer(be):
+    q, s, w, ws = make(70, 96, 224, 5)
+    want = value(q, s, w, ws)
+    m = be.upload_i8(torch.from_numpy(w).cuda(), torch.from_numpy(ws).cuda())
+    buf = torch.zeros(70, 192, dtype=torch.float16, device="cuda")
+    be.gemm_i8(m, on_gpu(q), torch.from_numpy(s).cuda(), buf[:, 96:], residual=buf[:, :96])
+    check(buf[:, 96:], want, torch.float16, plain_off(want) * 1.5)
+    assert not bool(buf[:, :96].any())
+
+
+def gated_off(g, u, h):
+    """The bound on the 32-bit value's error: g and u to 3 u; g / (1 + exp(-g)) moves by 1 + |g| of g's error; exp is
+    good to two half steps, and the addition, the division and the product round once each.  Where exp(-g) overflows
+    (g < -88) the result is -0 and what it should be is below 2^-118 |u|."""
+    return np.abs(h) * (3 * (1 + np.abs(g)) + 2 + 3 + 3) * 1.01 * U + 2.0 ** -118 * np.abs(u) + 2.0 ** -148
+
+
+@pytest.mark.parametrize("tokens,rows,k", PRODUCTS)
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+def test_gated(be, tokens, rows, k, ty):
+    t = TYPES[ty]
+    q, s, w, ws = make(tokens, rows, k, seed=tokens + rows + k)
+    _, _, v, vs = make(1, rows, k, seed=k)
+    g, u = value(q, s, w, ws), value(q, s, v, vs)
+    with np.errstate(over="ignore"):
+        want = g / (1 + np.exp(-g)) * u
+    m = be.upload_i8_gated(w, ws, v, vs)
+    assert (m.rows, m.k, m.gated) == (rows, k, True)
+    space = torch.zeros(be.gemm_i8_workspace_bytes(m, tokens), dtype=torch.uint8, device="cuda")
+    first = None
+    for pad, offset, ypad in ((0, 0, 0), (-k % 16, 0, 4), (7, 1, 3)):
+        buf = torch.full((tokens, rows + ypad), 7.0, dtype=t, device="cuda")
+        h = buf[:, :rows]
+        be.gemm_i8_swiglu(m, on_gpu(q, pad, offset), torch.from_numpy(s).cuda(), h, space)
+        check(h, want, t, gated_off(g, u, want))
+        assert bool((buf[:, rows:] == 7).all())
+        first = h.clone() if first is None else first
+        assert torch.equal(first, h)
+    for which, (a, b) in enumerate(((w, ws), (v, vs))):
+        got = m.read(which)
+        assert np.array_equal(got[0], a) and np.array_equal(got[1], b)
+    m.close()
+
+
+@pytest.mark.parametrize("tokens", [1, 20, 70, 300])
+def test_gated_far_arguments(be, tokens):
+    """Gates from -200 to 200, where exp(-g) overflows and vanishes."""
+    rows, k = 64, 32
+    q = np.zeros((tokens, k), np.int8)
+    q[:, 0], q[:, 1] = 100, np.arange(tokens) % 100 + 1
+    w, v = np.zeros((rows, k), np.int8), np.zeros((rows, k), np.int8)
+    w[:, 0], v[:, 1] = np.linspace(-127, 127, rows).astype(np.int8), 3
+    s, ws, vs = np.full(tokens, 0.5, np.float32), np.full(rows, 4 / 127, np.float32), np.full(rows, 0.25, np.float32)
+    g, u = value(q, s, w, ws), value(q, s, v, vs)
+    assert g.min() < -199.9 and g.max() > 199.9
+    want = g / (1 + np.exp(-g)) * u
+    m = be.upload_i8_gated(w, ws, v, vs)
+    h = torch.zeros(tokens, rows, device="cuda")
+    be.gemm_i8_swiglu(m, on_gpu(q), torch.from_numpy(s).cuda(), h)
+    check(h, want, torch.float32, gated_off(g, u, want))
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 130])
+def test_largest_sums(be, tokens):
+    """k = 131071 of -128 times -128: 2147467264, the largest sum that int32 has to hold; and its negative."""
+    k, rows = 131071, 18
+    q, w = np.full((tokens, k), -128, np.int8), np.full((rows, k), -128, np.int8)
+    w[1::2] = 127
+    s, ws = np.ones(tokens, np.float32), np.ones(rows, np.float32)
+    m = be.upload_i8(w, ws)
+    y = torch.zeros(tokens, rows, device="cuda")
+    space = torch.zeros(be.gemm_i8_workspace_bytes(m, tokens), dtype=torch.uint8, device="cuda")
+    be.gemm_i8(m, on_gpu(q, pad=1), torch.from_numpy(s).cuda(), y, space)
+    want = np.where(np.arange(rows) % 2 == 0, np.float32(128 * 128 * k), np.float32(-128 * 127 * k))
+    assert np.array_equal(y.cpu().numpy(), np.broadcast_to(want, (tokens, rows)))
+
+
+def test_scales_that_are_not_finite(be):
+    import lbhip
+    q, s, w, ws = make(40, 50, 100, 1)
+    s[3], s[39] = np.nan, 0.0
+    m = be.upload_i8(w, ws)
+    y = torch.zeros(40, 50, device="cuda")
+    be.gemm_i8(m, on_gpu(q, 12), torch.from_numpy(s).cuda(), y,
+               torch.zeros(be.gemm_i8_workspace_bytes(m, 40), dtype=torch.uint8, device="cuda"))
+    nan = torch.isnan(y).cpu().numpy()
+    assert nan[3].all() and nan.sum() == 50 and not bool(y[39].any())
+    ws[7] = np.inf
+    with pytest.raises(lbhip.QuantError) as e:
+        be.upload_i8(w, ws)
+    assert (e.value.variant, e.value.row, e.value.field, e.value.bits) == ("NonFiniteScale", 7, 0, 0x7f800000)
+    with pytest.raises(lbhip.QuantError) as e:
+        be.upload_i8_gated(w, np.ones(50, np.float32), w, ws)
+    assert (e.value.row, e.value.field) == (7, 1)
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 16, 40, 64, 100, 300])
+def test_tokens_do_not_depend_on_their_batch(be, tokens):
+    q, s, w, ws = make(300, 200, 512, 2)
+    m = be.upload_i8(w, ws)
+    full, part = torch.zeros(300, 200, device="cuda"), torch.zeros(tokens, 200, device="cuda")
+    sd = torch.from_numpy(s).cuda()
+    be.gemm_i8(m, on_gpu(q), sd, full)
+    be.gemm_i8(m, on_gpu(q)[300 - tokens:], sd[300 - tokens:], part)
+    assert torch.equal(full[300 - tokens:], part)
+
+
+@pytest.mark.parametrize("ty", [synth.Q4_K, synth.Q5_K, synth.IQ2_S, synth.IQ3_S])
+def test_from_packed(be, oracle, ty):
+    """The int8 form of an uploaded matrix: each decoded row by the row quantizer's rule."""
+    rows, k = 37, 768
+    a, b = synth.random_matrix(ty, rows, k, 3), synth.random_matrix(ty, rows, k, 4)
+    ex = oracle.make_exec(oracle.MODE_DEQUANT_F32)
+    da, db = be.upload(ty, rows, k, a), be.upload(ty, rows, k, b)
+    got = be.i8_from_packed(da, db)
+    for which, raw in enumerate((a, b)):
+        om = oracle.make_matrix(ty, rows, k, raw)
+        eye = np.eye(k, dtype=np.float32)
+        f = np.stack([oracle.gemv(ex, om, eye[i]) for i in range(k)], axis=1).astype(np.float64)
+        s = (np.abs(f).max(axis=1) / 127).astype(np.float32)
+        want = np.rint(f / np.where(s > 0, s, 1).astype(np.float64)[:, None])
+        q, scales = got.read(which)
+        assert np.array_equal(scales, s) and np.array_equal(q, np.where((s > 0)[:, None], want, 0).astype(np.int8))
+    one = be.i8_from_packed(da)
+    assert not one.gated and all(np.array_equal(x, y) for x, y in zip(one.read(), got.read(0)))
+
+
+def test_from_packed_f32_and_refusals(be):
+    import lbhip
+    r = np.random.default_rng(2)
+    w = r.standard_normal((300, 512)).astype(np.float32)
+    w[5] = 0
+    q, s = be.i8_from_packed(be.upload(lbhip.F32, 300, 512, w)).read()
+    want = (np.abs(w.astype(np.float64)).max(axis=1) / 127).astype(np.float32)
+    assert np.array_equal(s, want)
+    assert np.array_equal(q, np.rint(w / np.where(want > 0, want, 1).astype(np.float64)[:, None]).astype(np.int8))
+    other = be.upload(lbhip.F32, 300, 256, w[:, :256])
+    with pytest.raises(lbhip.KernelError) as e:
+        be.i8_from_packed(be.upload(lbhip.F32, 300, 512, w), other)
+    assert e.value.variant == "DimensionMismatch"
+    w[17, 100] = np.nan
+    with pytest.raises(lbhip.QuantError) as e:
+        be.i8_from_packed(be.upload(lbhip.F32, 300, 512, w))
+    assert (e.value.variant, e.value.row) == ("NonFiniteScale", 17)
