@@ -276,7 +276,7 @@ def _own(s):
         return y
     if kind == "block":
         after, q, scale = _own_norm_i8(s)
-        y = torch.empty(tokens, case["rows"], dtype=ty, device=DEVICE)
+        y = torch.empty(tokens, case["rows"], device=DEVICE)   # 32 bits until its own quantization
         be.gemm_i8_swiglu(s["pair"], q, scale, y, s["workspace"])
         q, scale = torch.empty(y.shape, dtype=torch.int8, device=DEVICE), torch.empty_like(scale)
         be.quantize_i8_rows(y, q, scale)
