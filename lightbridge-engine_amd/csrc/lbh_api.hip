@@ -181,6 +181,10 @@ lbh_status lbh_ctx_set_tuning(lbh_ctx *ctx, int32_t key, int32_t value) {
         if (value < 0 || value > 3) return LBH_INVALID_PARAMETER;
         ctx->gemm_shape = value;
         return LBH_OK;
+    case LBH_TUNE_I8_FORM:
+        if (value < 0 || value > I8_FORMS) return LBH_INVALID_PARAMETER;
+        ctx->i8_form = value;
+        return LBH_OK;
     default: return LBH_INVALID_PARAMETER;
     }
 }

@@ -148,7 +148,7 @@ lbh_status alloc_i8(lbh_ctx *ctx, size_t rows, size_t k, int gated, lbh_i8_matri
     m->device = ctx->device;
     m->rows = rows;
     m->k = k;
-    m->kt = (k + 127) / 128 * 2;
+    m->kt = (k + 255) / 256 * 4;
     m->groups = (rows + 15) / 16;
     m->gated = gated;
     const size_t all = m->groups * (gated ? 2 : 1), tb = all * m->kt * 1024, sb = all * 16 * sizeof(float);
@@ -266,8 +266,9 @@ lbh_status product(lbh_ctx *ctx, const lbh_i8_matrix *m, int gated, const int8_t
     a.out_type = y_type;
     a.gated = gated;
     a.cu_count = ctx->cu_count;
-    a.vec_out = aligned_to(y, 4 * e) && y_stride % 4 == 0 &&
-                (!residual || (aligned_to(residual, 4 * e) && residual_stride % 4 == 0));
+    a.form = ctx->i8_form;
+    a.vec_out = aligned_to(y, 16) && y_stride * e % 16 == 0 &&
+                (!residual || (aligned_to(residual, 16) && residual_stride * e % 16 == 0));
     if (!aligned_to(x, 16) || x_stride % 16 || m->k % 16) {
         // The kernels read rows as 16-byte words: such rows go to the workspace first.
         const size_t pitch = m->kt * 64, need = n_tokens * pitch;

@@ -18,6 +18,7 @@ struct lbh_ctx {
     lbh::DevStatus *status_host;   // pinned mirror
     lbh::GemvTuning tuning;
     int gemm_shape;           // K-quant GEMM schedule (LBH_TUNE_GEMM_SHAPE; 0: by rows and tokens)
+    int i8_form;              // int8 product form (LBH_TUNE_I8_FORM; 0: by sizes)
     uint8_t *scratch;         // this device's copy of the library's static scratch array (lbh_api.hip)
 };
 

@@ -13,8 +13,12 @@
 // + 15): a wave's 16 bytes a lane are one contiguous KiB.  Tiles of one
 // channel group follow each other along k; a gated pair's gate and up groups
 // alternate, so both products of a channel end in the same lane.  Channels and
-// k are padded with zeros (k to 128), so what the rows hold behind k never
+// k are padded with zeros (k to 256), so what the rows hold behind k never
 // counts.
+#include <math.h>
+
+#include <type_traits>
+
 #include "lbh_dev.h"
 #include "lbh_internal.h"
 #include "lbh_rowtypes.h"
@@ -24,6 +28,12 @@ namespace lbh {
 namespace {
 
 typedef int i8_v4i __attribute__((ext_vector_type(4)));
+typedef int i8_v16i __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void i8_lds;
+
+// Token rows in LDS: 64 bytes of a token are four pieces, piece c stored at c ^
+// token_swizzle, so that 16 lanes reading one piece of 16 tokens touch every bank.
+__device__ __forceinline__ int token_swizzle(int t) { return (t >> 2) & 3; }
 
 // ------------------------------------------------------------- weight layout
 
@@ -68,7 +78,7 @@ __global__ void k_i8_from_tiles(I8LayoutArgs p) {
     }
 }
 
-// Rows of any alignment and length into rows of `pitch` (a multiple of 128)
+// Rows of any alignment and length into rows of `pitch` (a multiple of 256)
 // aligned bytes, zeros behind k.
 __global__ void k_i8_align_rows(const int8_t *x, long long stride, int k, int pitch, long long n, uint8_t *out) {
     const int words = pitch / 16;
@@ -87,58 +97,106 @@ __global__ void k_i8_align_rows(const int8_t *x, long long stride, int k, int pi
 
 // ------------------------------------------------------------- the epilogue
 
-template <int OUT>
-__device__ __forceinline__ void load4(const row_t<OUT> *p, float (&v)[4]) {
-    const rvec<row_t<OUT>, 4> a = *reinterpret_cast<const rvec<row_t<OUT>, 4> *>(p);
+// V consecutive elements as words of at most 16 bytes.
+template <int OUT, int V>
+__device__ __forceinline__ void load_row(const row_t<OUT> *p, float (&v)[V]) {
+    constexpr int N = V * (int)sizeof(row_t<OUT>) > 16 ? 16 / (int)sizeof(row_t<OUT>) : V;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = (float)a[j];
+    for (int i = 0; i < V; i += N) {
+        const rvec<row_t<OUT>, N> a = *reinterpret_cast<const rvec<row_t<OUT>, N> *>(p + i);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[i + j] = (float)a[j];
+    }
 }
-template <int OUT>
-__device__ __forceinline__ void store4(row_t<OUT> *p, const float (&v)[4]) {
-    rvec<row_t<OUT>, 4> a;
+template <int OUT, int V>
+__device__ __forceinline__ void store_row(row_t<OUT> *p, const float (&v)[V]) {
+    constexpr int N = V * (int)sizeof(row_t<OUT>) > 16 ? 16 / (int)sizeof(row_t<OUT>) : V;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) a[j] = (row_t<OUT>)v[j];
-    *reinterpret_cast<rvec<row_t<OUT>, 4> *>(p) = a;
+    for (int i = 0; i < V; i += N) {
+        rvec<row_t<OUT>, N> a;
+#pragma unroll
+        for (int j = 0; j < N; ++j) a[j] = (row_t<OUT>)v[i + j];
+        *reinterpret_cast<rvec<row_t<OUT>, N> *>(p + i) = a;
+    }
 }
 
-// Four channels c .. c + 3 (c % 4 == 0) of token t from their integer sums
-// (`up`: of the second matrix of a gated pair).  g: channel group of the tiles.
-template <int OUT, bool GATED>
-__device__ __forceinline__ void finish4(const I8Args &p, int t, int c, const i8_v4i &sum, const i8_v4i &up) {
-    const float xs = p.xs[t];
-    float v[4];
-    const int gr = c >> 4;
-    if constexpr (GATED) {
-        const float4 sg = *reinterpret_cast<const float4 *>(p.ws + 32 * gr + (c & 15));
-        const float4 su = *reinterpret_cast<const float4 *>(p.ws + 32 * gr + 16 + (c & 15));
-        const float a[4] = {sg.x, sg.y, sg.z, sg.w}, b[4] = {su.x, su.y, su.z, su.w};
+// The scales of channels c .. c + V - 1 (c % V == 0, V <= 16; channels past the last
+// one have the zeros that fill its group, or those of the last group).
+template <bool GATED, int V>
+struct ChannelScales {
+    float g[V], u[GATED ? V : 1];
+    __device__ __forceinline__ ChannelScales(const I8Args &p, int c) {
+        const int grp = min(c >> 4, (p.rows - 1) >> 4);
+        const float *s = p.ws + (GATED ? 32 : 16) * grp + (c & 15);
+        load_row<T_F32, V>(s, g);
+        if constexpr (GATED) load_row<T_F32, V>(s + 16, u);
+    }
+};
+
+// The value as a 32-bit float: without this the compiler folds a product and its
+// conversion to 16 bits into one rounding, in some of the forms and not in others.
+__device__ __forceinline__ float rounded(float v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
+// g / (1 + exp(-g)) * u.  exp(-g) = 2^z with z = -g log2(e) to some 40 bits (hi +
+// lo), so the argument's rounding does not grow with |g|; below g = -88 the
+// exponent stays there (what is right is below 2^-118 |u|), and 1 / d is the
+// reciprocal with one Newton step.  The library's exp and division cost twice
+// as many instructions, which is what bounds the epilogue.
+__device__ __forceinline__ float swiglu(float g, float u) {
+    constexpr float LOG2E = 0x1.715476p+0f, LOG2E_LO = 0x1.4ae0cp-26f, LN2 = 0x1.62e43p-1f;
+    const float x = fminf(-g, 88.0f);
+    const float hi = x * LOG2E;
+    const float lo = __builtin_fmaf(x, LOG2E_LO, __builtin_fmaf(x, LOG2E, -hi));
+    float e = __builtin_amdgcn_exp2f(hi);
+    e = __builtin_fmaf(e, lo * LN2, e);
+    const float d = 1.0f + e;
+    float r = __builtin_amdgcn_rcpf(d);
+    r = __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+    return g * r * u;
+}
+
+// Channels c .. c + V - 1 of token t from their sums times the token's scale
+// (`up`: of the second matrix of a gated pair).  INSIDE: all of them exist, rows
+// are aligned to 16 bytes, and the residual's values (if any) are at hand.
+template <int OUT, bool GATED, bool INSIDE, int V>
+__device__ __forceinline__ void finish(const I8Args &p, int t, int c, const float (&sum)[V], const float (&up)[V],
+                                       const ChannelScales<GATED, V> &ws,
+                                       const rvec<row_t<OUT>, V> *residual = nullptr) {
+    if (!INSIDE && c >= p.rows) return;
+    float v[V];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float g = (float)sum[j] * xs * a[j], u = (float)up[j] * xs * b[j];
-            v[j] = g / (1.0f + expf(-g)) * u;
-        }
-    } else {
-        const float4 s4 = *reinterpret_cast<const float4 *>(p.ws + 16 * gr + (c & 15));
-        const float a[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = (float)sum[j] * xs * a[j];
+    for (int j = 0; j < V; ++j) {
+        v[j] = sum[j] * ws.g[j];
+        if constexpr (GATED) v[j] = swiglu(v[j], up[j] * ws.u[j]);
+        v[j] = rounded(v[j]);
     }
     row_t<OUT> *y = static_cast<row_t<OUT> *>(p.y) + (long long)t * p.y_stride + c;
+    if constexpr (INSIDE) {
+        if (residual) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = rounded((float)(*residual)[j] + v[j]);
+        }
+        store_row<OUT, V>(y, v);
+        return;
+    }
     const row_t<OUT> *res = GATED || !p.residual
                                 ? nullptr
                                 : static_cast<const row_t<OUT> *>(p.residual) + (long long)t * p.residual_stride + c;
-    if (p.vec_out && c + 3 < p.rows) {
+    if (p.vec_out && c + V <= p.rows) {
         if (res) {
-            float r[4];
-            load4<OUT>(res, r);
+            float r[V];
+            load_row<OUT, V>(res, r);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = r[j] + v[j];
+            for (int j = 0; j < V; ++j) v[j] = rounded(r[j] + v[j]);
         }
-        store4<OUT>(y, v);
+        store_row<OUT, V>(y, v);
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (c + j < p.rows) y[j] = (row_t<OUT>)(res ? (float)res[j] + v[j] : v[j]);
+        for (int j = 0; j < V; ++j)
+            if (c + j < p.rows) y[j] = (row_t<OUT>)rounded(res ? (float)res[j] + v[j] : v[j]);
     }
 }
 
@@ -146,90 +204,399 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t i8_rsrc(const void *base, long
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, (int)(uint32_t)bytes, 0x00020000);
 }
 
+// 16 bytes at a byte offset, zero past the resource's end.
+__device__ __forceinline__ i8_v4i i8_load(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+    return __builtin_bit_cast(i8_v4i, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+}
+
+// 16 bytes a lane straight to LDS, lane l's at to + 16 l.
+__device__ __forceinline__ void i8_copy(__amdgpu_buffer_rsrc_t r, uint8_t *to, uint32_t at, uint32_t uniform) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (i8_lds *)to, 16, at, uniform, 0, 0);
+}
+
 // ------------------------------------------------------- few tokens: streaming
 //
-// A workgroup takes one channel group (a gated pair's two) and up to 16 * TT
-// tokens; its eight waves take every eighth k tile and their integer sums are
-// joined in LDS.  Bound: the weights' bytes, each read once a token tile.
+// A workgroup takes R channel groups (gated: pairs of groups) and 16 * TT tokens
+// over all of k; its eight waves take every eighth k tile and their integer sums
+// are joined in LDS, so that a matrix of few channels still has every CU at work.
+// Weights go straight to operand registers; tokens through LDS: 16 tokens x 64
+// bytes read straight into operand registers touch 64 lines an instruction, which
+// costs the L1 four times what the bytes do, and copied to LDS in the order of
+// memory they touch 16 (64 tokens x 12288 channels x 4096: 25.9 -> 18.0 us; with
+// R = 2, 15.0).  Each wave has two buffers of its own, so nobody waits for another
+// wave before the join.  Bound: up to some 16 tokens the weights' bytes (one token
+// x 12288 x 4096: 9.3 us, 5.4 TB/s), then the L1's (R + TT) KiB a k tile.
 constexpr int ST_WAVES = 8;
 
-template <int OUT, bool GATED, int TT>
-__global__ void __launch_bounds__(64 * ST_WAVES) k_i8_stream(I8Args p) {
-    constexpr int G = GATED ? 2 : 1;
-    constexpr int U = TT == 1 ? 8 : 4;
-    __shared__ __align__(16) i8_v4i s_sum[ST_WAVES][G * TT][64];
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-    const int t0 = blockIdx.y * 16 * TT, nt = min(p.n_tokens - t0, 16 * TT);
-    const __amdgpu_buffer_rsrc_t rw =
-        i8_rsrc(p.w + (long long)blockIdx.x * G * p.kt * 1024, (long long)G * p.kt * 1024);
-    // Token rows end with their last byte: what a tile reads beyond is zero, and
-    // what it reads of the next row meets the weights' zeros.  (All offsets are
-    // vector offsets: the scalar one is left out of the range check.)
+template <int OUT, bool GATED, int TT, int R>
+__global__ void __launch_bounds__(64 * ST_WAVES, 4) k_i8_stream(I8Args p) {
+    constexpr int G = GATED ? 2 * R : R;
+    __shared__ __align__(1024) uint8_t x0[ST_WAVES][TT * 1024], x1[ST_WAVES][TT * 1024];
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int groups = (p.rows + 15) / 16 * (GATED ? 2 : 1), across = (groups + G - 1) / G;
+    const int bx = blockIdx.x % across;
+    const int t0 = (int)(blockIdx.x / across) * 16 * TT, nt = min(p.n_tokens - t0, 16 * TT);
+    const int g0 = bx * G, last = min(groups - g0, G);
+    const __amdgpu_buffer_rsrc_t rw = i8_rsrc(p.w + (long long)g0 * p.kt * 1024, (long long)last * p.kt * 1024);
     const __amdgpu_buffer_rsrc_t rx = i8_rsrc(p.x + (long long)t0 * p.x_stride, (long long)(nt - 1) * p.x_stride + p.k);
-    uint32_t xo[TT];
+    uint32_t from[TT];
 #pragma unroll
     for (int i = 0; i < TT; ++i)
-        xo[i] = (uint32_t)min(16 * i + (lane & 15), nt - 1) * (uint32_t)p.x_stride + 16 * (lane >> 4);
-    i8_v4i acc[G][TT] = {};
-    for (int k0 = wid; k0 < p.kt; k0 += ST_WAVES * U) {
-        i8_v4i a[U][G], b[U][TT];
+        from[i] = (uint32_t)min(16 * i + (lane >> 2), nt - 1) * (uint32_t)p.x_stride +
+                  16 * ((lane & 3) ^ token_swizzle(lane >> 2));
+    const int at = (lane & 15) * 64 + 16 * ((lane >> 4) ^ token_swizzle(lane & 15));
+    i8_v4i acc[G][TT] = {}, a0[G], a1[G];
+    auto ask = [&](uint8_t *x, i8_v4i (&a)[G], int kt) {
+        // past the last tile (or group): out of the resource's range, zero
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int kt = k0 + ST_WAVES * u;
+        for (int g = 0; g < G; ++g)
+            a[g] = i8_load(rw, lane * 16 + (kt < p.kt ? g * p.kt + kt : G * p.kt) * 1024);
 #pragma unroll
-            for (int g = 0; g < G; ++g)   // past the last tile: out of the resource's range, zero
-                a[u][g] = __builtin_bit_cast(
-                    i8_v4i, __builtin_amdgcn_raw_buffer_load_b128(
-                                rw, lane * 16 + (kt < p.kt ? (g * p.kt + kt) * 1024 : G * p.kt * 1024), 0, 0));
+        for (int i = 0; i < TT; ++i)
+            i8_copy(rx, x + i * 1024, from[i] + kt * 64, 0);
+    };
+    auto multiply = [&](const uint8_t *x, const i8_v4i (&a)[G]) {
+        // everything but the other buffer's loads has arrived
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(G + TT) : "memory");
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+            const i8_v4i b = *reinterpret_cast<const i8_v4i *>(x + i * 1024 + at);
+#pragma unroll
+            for (int g = 0; g < G; ++g) acc[g][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[g], b, acc[g][i], 0, 0, 0);
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int i = 0; i < TT; ++i)
-                b[u][i] = __builtin_bit_cast(
-                    i8_v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, xo[i] + (k0 + ST_WAVES * u) * 64, 0, 0));
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < TT; ++i)
-#pragma unroll
-                for (int g = 0; g < G; ++g)
-                    acc[g][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u][g], b[u][i], acc[g][i], 0, 0, 0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read before the next copy into this buffer sets out
+    };
+    ask(x0[wid], a0, wid);
+    for (int kt = wid; kt < p.kt; kt += 2 * ST_WAVES) {
+        ask(x1[wid], a1, kt + ST_WAVES);
+        multiply(x0[wid], a0);
+        ask(x0[wid], a0, kt + 2 * ST_WAVES);
+        multiply(x1[wid], a1);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no copy is on its way into what follows
+    __syncthreads();
+    // The join: each wave's sums in its own half of the buffers, G * TT KiB from wave to wave.
+    static_assert(G <= 2, "the sums of half the waves fit a buffer");
+    auto sums = [&](int w) -> i8_v4i * {
+        uint8_t *half = w < ST_WAVES / 2 ? x0[0] : x1[0];
+        return reinterpret_cast<i8_v4i *>(half + w % (ST_WAVES / 2) * G * TT * 1024);
+    };
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int i = 0; i < TT; ++i) s_sum[wid][g * TT + i][lane] = acc[g][i];
+        for (int i = 0; i < TT; ++i) sums(wid)[(g * TT + i) * 64 + lane] = acc[g][i];
     __syncthreads();
-    for (int i = wid; i < TT; i += ST_WAVES) {
+    for (int j = wid; j < R * TT; j += ST_WAVES) {
+        const int r = j / TT, i = j % TT;
         i8_v4i sum = {}, up = {};
 #pragma unroll
         for (int w = 0; w < ST_WAVES; ++w) {
-            sum += s_sum[w][i][lane];
-            if constexpr (GATED) up += s_sum[w][TT + i][lane];
+            sum += sums(w)[((GATED ? 2 * r : r) * TT + i) * 64 + lane];
+            if constexpr (GATED) up += sums(w)[((2 * r + 1) * TT + i) * 64 + lane];
         }
-        const int t = 16 * i + (lane & 15);
-        if (t < nt) finish4<OUT, GATED>(p, t0 + t, blockIdx.x * 16 + 4 * (lane >> 4), sum, up);
+        const int t = 16 * i + (lane & 15), c = (bx * R + r) * 16 + 4 * (lane >> 4);
+        const ChannelScales<GATED, 4> ws(p, c);
+        const float xs = p.xs[t0 + min(t, nt - 1)];
+        float u[4], v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)sum[e] * xs, u[e] = (float)up[e] * xs;
+        if (t < nt) finish<OUT, GATED, false, 4>(p, t0 + t, c, v, u, ws);
     }
 }
 
-template <int OUT, bool GATED>
-hipError_t launch_typed(const I8Args &a, hipStream_t s) {
-    const unsigned groups = (unsigned)((a.rows + 15) / 16);
-    if (a.n_tokens <= 16)
-        hipLaunchKernelGGL((k_i8_stream<OUT, GATED, 1>), dim3(groups, 1), dim3(64 * ST_WAVES), 0, s, a);
-    else if (a.n_tokens <= 32)
-        hipLaunchKernelGGL((k_i8_stream<OUT, GATED, 2>), dim3(groups, 1), dim3(64 * ST_WAVES), 0, s, a);
+// ------------------------------------------------------ many tokens: tiles
+//
+// A workgroup of four waves (2 x 2) computes 64 * CW channels x 64 * TW tokens,
+// each wave CW x TW products of 32 x 32 with v_mfma_i32_32x32x32_i8.  k runs in
+// stages of 64: both operands are copied to LDS three stages ahead into a ring
+// of four buffers (no registers in between).  Weights keep their tile order
+// there; a token's 64 bytes are four pieces, piece c stored at c ^ swizzle of
+// the token, so that 16 lanes reading one piece of 16 tokens touch every bank.
+template <int OUT, bool GATED, int CW, int TW>
+__global__ void __launch_bounds__(256, CW * TW > 8 ? 1 : 2) k_i8_tile(I8Args p) {
+    constexpr int CH = 64 * CW, TK = 64 * TW;
+    constexpr int A_BYTES = CH * 64, STAGE = (CH + TK) * 64;
+    // Four objects, so that a wait before a read of one leaves the copies into the others in flight.
+    __shared__ __align__(1024) uint8_t lds0[STAGE], lds1[STAGE], lds2[STAGE], lds3[STAGE];
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wc = wid & 1, wt = wid >> 1;
+    // Tiles of the grid: workgroups go to the eight XCDs in turn, and each XCD
+    // takes a contiguous run of tiles.  Within the run: panels of eight token
+    // tiles, channel tiles one after the other inside, so that the tiles at work
+    // at once share operands both ways.
+    const int groups = (p.rows + 15) / 16 * (GATED ? 2 : 1);       // channel groups in memory
+    const int n_tt = (p.n_tokens + TK - 1) / TK;
+    const int total = gridDim.x, per = (total + 7) / 8;
+    const int xcd = blockIdx.x & 7, ix = blockIdx.x >> 3;
+    const int whole = total & 7 ? total & 7 : 8;                  // XCDs with `per` tiles, the others one less
+    const int tile = xcd < whole ? xcd * per + ix : whole * per + (xcd - whole) * (per - 1) + ix;
+    const int n_tc = total / n_tt, panel = tile / (8 * n_tc), width = min(8, n_tt - 8 * panel);
+    const int in_panel = tile - panel * 8 * n_tc;
+    const int tc = in_panel / width, tt = panel * 8 + in_panel % width;
+    const int g0 = tc * (CH / 16), t0 = tt * TK;
+    const int nt = min(p.n_tokens - t0, TK);
+    const __amdgpu_buffer_rsrc_t rw =
+        i8_rsrc(p.w + (long long)g0 * p.kt * 1024, (long long)min(groups - g0, CH / 16) * p.kt * 1024);
+    const __amdgpu_buffer_rsrc_t rx = i8_rsrc(p.x + (long long)t0 * p.x_stride, (long long)(nt - 1) * p.x_stride + p.k);
+
+    // The epilogue's layout and scales.
+    constexpr int ROW = CW * 32 + 4;                              // floats; 16 tokens of one channel reach every bank
+    constexpr int V = OUT == T_F32 ? 4 : 8;                       // channels of a lane
+    constexpr int WIDE = GATED ? CW * 16 : CW * 32;               // channels of the wave
+    constexpr int PER = WIDE / V, AT_ONCE = 64 / PER;             // lanes a token, tokens a pass
+    const int lc = (lane % PER) * V;
+    const int c = (GATED ? g0 / 2 : g0) * 16 + wc * WIDE + lc;
+    const ChannelScales<GATED, V> ws(p, c);
+    float xs[TW];
+#pragma unroll
+    for (int n = 0; n < TW; ++n) xs[n] = p.xs[t0 + min((wt * TW + n) * 32 + (lane & 31), nt - 1)];
+
+    // What this wave copies of a stage: CW channel groups of 1 KiB (groups past the
+    // last one repeat it) and TW pieces of 16 tokens x 64 bytes (tokens past the
+    // last one lie behind the resource's end).
+    const uint32_t stride = (uint32_t)p.x_stride;
+    const uint32_t vb = (uint32_t)(wid * TW * 16 + (lane >> 2)) * stride + 16 * ((lane & 3) ^ token_swizzle(lane >> 2));
+    auto copy_weights = [&](uint8_t *buf, int kt) {
+#pragma unroll
+        for (int i = 0; i < CW; ++i) {
+            const int g = wid * CW + i;
+            i8_copy(rw, buf + g * 1024, lane * 16, (min(g, groups - g0 - 1) * p.kt + kt) * 1024);
+        }
+    };
+    auto copy_tokens = [&](uint8_t *buf, int kt) {
+#pragma unroll
+        for (int i = 0; i < TW; ++i)
+            i8_copy(rx, buf + A_BYTES + (wid * TW + i) * 1024, vb + (uint32_t)i * 16u * stride + kt * 64, 0);
+    };
+
+    // Operands of k piece j (32 of a stage's 64): lane l holds channel (token) l %
+    // 32 and k 16 (l / 32) .. + 15 of the 32.
+    const int l32 = lane & 31, hi = lane >> 5;
+    const int a_at = wc * CW * 2048 + (l32 >> 4) * 1024 + hi * 256 + (l32 & 15) * 16;
+    const int b_at = A_BYTES + (wt * TW * 32 + l32) * 64;
+    const int b_piece = hi ^ token_swizzle(l32);
+    i8_v4i a[2][CW], b[2][TW];
+    auto read = [&](const uint8_t *buf, int j, i8_v4i (&fa)[CW], i8_v4i (&fb)[TW]) {
+#pragma unroll
+        for (int i = 0; i < CW; ++i) fa[i] = *reinterpret_cast<const i8_v4i *>(buf + a_at + i * 2048 + j * 512);
+#pragma unroll
+        for (int i = 0; i < TW; ++i)
+            fb[i] = *reinterpret_cast<const i8_v4i *>(buf + b_at + i * 2048 + 16 * (b_piece ^ (2 * j)));
+    };
+    i8_v16i acc[CW][TW] = {};
+    auto multiply = [&](const i8_v4i (&fa)[CW], const i8_v4i (&fb)[TW]) {
+#pragma unroll
+        for (int i = 0; i < CW; ++i)
+#pragma unroll
+            for (int n = 0; n < TW; ++n)
+                acc[i][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[n], acc[i][n], 0, 0, 0);
+    };
+    // Reads and copies go between the products: a read after each of the first
+    // ones, then a copy after each further one.
+    auto mix = [&](int copies) {
+#pragma unroll
+        for (int i = 0; i < CW + TW; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // a read from LDS
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);     // a product
+            if (i < copies) __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);   // a copy
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, CW * TW, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // A stage: `cur` is read, `next` read ahead from, and `free` (the previous
+    // stage's) filled for the third stage from here.  The last stages copy the
+    // last one again.
+    auto stage = [&](const uint8_t *cur, const uint8_t *next, uint8_t *free, int kt) {
+        const int ahead = min(kt + 3, p.kt - 1);
+        read(cur, 1, a[1], b[1]);
+        copy_weights(free, ahead);
+        multiply(a[0], b[0]);
+        mix(CW);
+        // the next stage's copies of this wave are done (two stages' later ones may
+        // be on their way) and its reads of this stage, then everybody's
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * CW + TW) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        read(next, 0, a[0], b[0]);
+        copy_tokens(free, ahead);
+        multiply(a[1], b[1]);
+        mix(TW);
+    };
+    copy_weights(lds0, 0), copy_tokens(lds0, 0);
+    copy_weights(lds1, 1), copy_tokens(lds1, 1);
+    copy_weights(lds2, 2), copy_tokens(lds2, 2);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (CW + TW)) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(lds0, 0, a[0], b[0]);
+    for (int kt = 0; kt < p.kt; kt += 4) {   // a multiple of four: k is padded to 256
+        stage(lds0, lds1, lds3, kt);
+        stage(lds1, lds2, lds0, kt + 1);
+        stage(lds2, lds3, lds1, kt + 2);
+        stage(lds3, lds0, lds2, kt + 3);
+    }
+
+    // D of a 32 x 32 product: lane l holds token l % 32 and channels 8 q + 4 (l /
+    // 32) + 0 .. 3, q < 4.  Each wave scales them by their token and turns 32
+    // tokens at a time through its part of the LDS, so that a token's channels are
+    // read, scaled and stored in words of 16 bytes, whole lines at a time (stored
+    // straight from D, 16 bytes a token and line, the stores took a quarter of the
+    // kernel).
+    static_assert(32 * ROW * 4 <= STAGE, "a wave's part fits a buffer");
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    float *turn = reinterpret_cast<float *>(wid < 2 ? (wid ? lds1 : lds0) : (wid == 2 ? lds2 : lds3));
+    const int from = GATED ? (lc >> 4) * 32 + (lc & 15) : lc;     // a gated pair's groups alternate
+    auto put = [&](auto inside, auto with_residual) {
+        constexpr bool INSIDE = decltype(inside)::value, RES = decltype(with_residual)::value;
+        constexpr int PASSES = (32 + AT_ONCE - 1) / AT_ONCE;
+#pragma unroll
+        for (int n = 0; n < TW; ++n) {
+            // The passes' residuals, on their way while the sums are turned.
+            rvec<row_t<OUT>, V> res[RES ? PASSES : 1];
+            if constexpr (RES) {
+#pragma unroll
+                for (int k = 0; k < PASSES; ++k) {
+                    const int tl = min(k * AT_ONCE + lane / PER, 31);
+                    res[k] = *reinterpret_cast<const rvec<row_t<OUT>, V> *>(
+                        static_cast<const row_t<OUT> *>(p.residual) +
+                        (long long)(t0 + (wt * TW + n) * 32 + tl) * p.residual_stride + c);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < CW; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<float4 *>(turn + l32 * ROW + i * 32 + 8 * q + 4 * hi) =
+                        make_float4((float)acc[i][n][4 * q] * xs[n], (float)acc[i][n][4 * q + 1] * xs[n],
+                                    (float)acc[i][n][4 * q + 2] * xs[n], (float)acc[i][n][4 * q + 3] * xs[n]);
+            wave_sync();
+#pragma unroll
+            for (int r = 0; r < 32; r += AT_ONCE) {
+                const int tl = r + lane / PER, t = (wt * TW + n) * 32 + tl;
+                const float *row = turn + min(tl, 31) * ROW + from;
+                float g[V], u[V];
+                load_row<T_F32, V>(row, g);
+                if constexpr (GATED) load_row<T_F32, V>(row + 16, u);
+                const bool mine = (64 % PER == 0 || lane < PER * AT_ONCE) && (32 % AT_ONCE == 0 || tl < 32);
+                if (mine && (INSIDE || t < nt))
+                    finish<OUT, GATED, INSIDE, V>(p, t0 + t, c, g, u, ws, RES ? &res[r / AT_ONCE] : nullptr);
+            }
+            wave_sync();
+            __builtin_amdgcn_sched_barrier(0);   // the next tokens' residuals do not need registers yet
+        }
+    };
+    const bool inside = p.vec_out && nt == TK && (tc + 1) * (GATED ? CH / 2 : CH) <= p.rows;
+    if constexpr (!GATED && CW < 4) {
+        if (inside && p.residual) {
+            put(std::true_type{}, std::true_type{});
+            return;
+        }
+    }
+    // (The largest tile has no registers to hold residuals in: it takes them as the ragged tiles do.)
+    if (inside && (GATED || !p.residual))
+        put(std::true_type{}, std::false_type{});
     else
-        hipLaunchKernelGGL((k_i8_stream<OUT, GATED, 4>), dim3(groups, (unsigned)((a.n_tokens + 63) / 64)),
-                           dim3(64 * ST_WAVES), 0, s, a);
+        put(std::false_type{}, std::false_type{});
+}
+
+// The forms and what a call takes in each, in us.  Measured on k = 4096 (64 k tiles),
+// time of the whole call as a graph node; estimate() and plan() use them.
+struct Form {
+    int cw, tw;           // tile: 64 * cw channels x 64 * tw tokens (stream, cw = 0: tw = TT, r = R)
+    int r;
+    float fixed, step;    // a round of one workgroup per CU: fixed + step * k tiles
+};
+constexpr Form FORMS[] = {
+    {0, 1, 1, 0, 0},       {0, 2, 1, 0, 0},       {0, 2, 2, 0, 0},      {0, 4, 1, 0, 0},    {0, 4, 2, 0, 0},
+    {1, 1, 0, 1.5f, 0.10f}, {2, 1, 0, 2.0f, 0.16f}, {2, 2, 0, 2.5f, 0.235f}, {3, 2, 0, 3.5f, 0.32f}, {4, 4, 0, 8.5f, 0.73f}};
+constexpr int N_FORMS = sizeof(FORMS) / sizeof(FORMS[0]);
+static_assert(N_FORMS == I8_FORMS, "the forms a context can ask for");
+
+long long groups_of(const I8Args &a) { return ((long long)a.rows + 15) / 16 * (a.gated ? 2 : 1); }
+
+// Workgroups of a tile form.
+long long tiles_of(const I8Args &a, const Form &f) {
+    return (groups_of(a) + 4 * f.cw - 1) / (4 * f.cw) * ((a.n_tokens + 64 * f.tw - 1) / (64 * f.tw));
+}
+
+float estimate(const I8Args &a, const Form &f) {
+    const float cu = (float)a.cu_count, weights = (float)(groups_of(a) * a.kt) * 1024 / 5.2e6f;   // at 5.2 TB/s
+    if (f.cw) {
+        const float rounds = ceilf((float)tiles_of(a, f) / cu);
+        // the largest tile waits for its residuals (4096 x 12288: T44 227 us, T32 230)
+        const float wait = a.residual && f.cw == 4 ? 18.0f * rounds : 0.0f;
+        return 1.5f + wait + fmaxf(rounds * (f.fixed + f.step * (float)a.kt), weights);
+    }
+    // Two to four workgroups share a CU and its L1, which takes 17.6 ns for a KiB.
+    const int per = a.gated ? 2 * f.r : f.r;
+    const float n = (float)((groups_of(a) + per - 1) / per) * (float)((a.n_tokens + 16 * f.tw - 1) / (16 * f.tw));
+    return 2.5f + fmaxf(fmaxf(n / cu, 1.0f) * (float)a.kt * (float)(per + f.tw) * 0.0176f, weights);
+}
+
+// The form of the least estimate.  Measured / estimated, in us, for the choice and
+// the next ones (tokens x channels, k = 4096; S: stream TT, R; T: tile cw, tw):
+//   1 x 12288     S11 9.3 / 9.3      S12 9.6          32 x 12288    S22 11.4 / 9.3   S21 12.1
+//   64 x 4096     S22 6.3 / 7.0      S41 8.4          96 x 4096     S42 7.9 / 9.3    T11 11.1
+//   256 x 4096    T11 11.8 / 9.4     T21 12.9         128 x 12288   T21 16.0 / 13.7  T11 16.4, T22 18.1
+//   256 x 12288   T22 19.5 / 19.0    T21 23.2         512 x 12288   T32 28.2 / 25.5  T22 33.8, T44 43.5
+//   1024 x 4096 (k = 13312)  T22 57 / 53, T32 64      1024 x 12288  T32 48.8 / 48.5  T44 49.5, T22 56.4
+//   1024 x 26624  T44 116 / 112      T32 141          4096 x 12288  T44 175 / 167    T32 192, T22 219
+// Weights beyond the last cache (109 MB of 26624 channels, three matrices in turn)
+// arrive at some 2.2 TB/s in every tile form: 256 x 26624 takes 52 to 55 us in T22 and
+// T44, whichever is estimated less.
+int plan(const I8Args &a) {
+    int best = -1;
+    float least = 0.0f;
+    for (int i = 0; i < N_FORMS; ++i) {
+        if (a.gated && !FORMS[i].cw && FORMS[i].r > 1) continue;   // a pair is two groups already
+        const float t = estimate(a, FORMS[i]);
+        if (best < 0 || t < least) best = i, least = t;
+    }
+    return best;
+}
+
+template <int OUT, bool GATED, int CW, int TW>
+hipError_t launch_tile(const I8Args &a, hipStream_t s) {
+    const long long grid = tiles_of(a, Form{CW, TW, 0, 0, 0});
+    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_i8_tile<OUT, GATED, CW, TW>), dim3((unsigned)grid), dim3(256), 0, s, a);
     return hipGetLastError();
+}
+
+template <int OUT, bool GATED, int TT, int R>
+hipError_t launch_stream(const I8Args &a, hipStream_t s) {
+    const long long grid = ((long long)a.rows + 16 * R - 1) / (16 * R) * ((a.n_tokens + 16 * TT - 1) / (16 * TT));
+    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_i8_stream<OUT, GATED, TT, R>), dim3((unsigned)grid), dim3(64 * ST_WAVES), 0, s, a);
+    return hipGetLastError();
+}
+
+template <int OUT, bool GATED>
+hipError_t launch_form(const I8Args &a, int form, hipStream_t s) {
+    if (form < 0 || form >= N_FORMS) return hipErrorInvalidValue;
+    switch (form) {
+    case 0: return launch_stream<OUT, GATED, 1, 1>(a, s);
+    case 1: return launch_stream<OUT, GATED, 2, 1>(a, s);
+    case 3: return launch_stream<OUT, GATED, 4, 1>(a, s);
+    case 5: return launch_tile<OUT, GATED, 1, 1>(a, s);
+    case 6: return launch_tile<OUT, GATED, 2, 1>(a, s);
+    case 7: return launch_tile<OUT, GATED, 2, 2>(a, s);
+    case 8: return launch_tile<OUT, GATED, 3, 2>(a, s);
+    case 9: return launch_tile<OUT, GATED, 4, 4>(a, s);
+    }
+    if constexpr (!GATED) {
+        if (form == 2) return launch_stream<OUT, GATED, 2, 2>(a, s);
+        if (form == 4) return launch_stream<OUT, GATED, 4, 2>(a, s);
+    }
+    return launch_form<OUT, GATED>(a, form - 1, s);   // a forced form of two groups: a pair has them already
 }
 
 template <int OUT>
 hipError_t launch_out(const I8Args &a, hipStream_t s) {
-    return a.gated ? launch_typed<OUT, true>(a, s) : launch_typed<OUT, false>(a, s);
+    const int form = a.form ? a.form - 1 : plan(a);
+    return a.gated ? launch_form<OUT, true>(a, form, s) : launch_form<OUT, false>(a, form, s);
 }
 
 int grid_of(long long threads) {

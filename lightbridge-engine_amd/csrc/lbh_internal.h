@@ -253,9 +253,11 @@ struct I8Args {
     long long x_stride, y_stride, residual_stride;
     int32_t n_tokens, rows, k, kt;
     int32_t out_type, gated;
-    int32_t vec_out;         // y and residual: four elements at any multiple of four are one aligned word
+    int32_t vec_out;         // y and residual rows start at multiples of 16 bytes
     int32_t cu_count;
+    int32_t form;            // 0: the rule's; else the form's number (LBH_TUNE_I8_FORM)
 };
+constexpr int I8_FORMS = 10;
 
 // Batch selection: top-k of each token's finished logits (select_route).
 struct RouteBatchArgs {

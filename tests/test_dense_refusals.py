@@ -156,3 +156,10 @@ def test_matrix_refusals(ctx):
     assert status(read, ctx, C.byref(m), 0, A, 32, A, 5)[0] == "OutputLengthMismatch"
     assert status(L.lbh_i8_matrix_from_packed, ctx, None, None, C.byref(h))[0] == "NullArgument"
     assert L.lbh_i8_matrix_destroy(None) == 0
+
+
+def test_the_form_knob_s_range(ctx):
+    fn = lbhip.lib().lbh_ctx_set_tuning
+    be = lbhip.HipBackend
+    assert [fn(ctx, be.TUNE_I8_FORM, v) for v in (-1, 11)] == [25, 25]
+    assert [fn(ctx, be.TUNE_I8_FORM, v) for v in (1, 10, 0)] == [0, 0, 0]

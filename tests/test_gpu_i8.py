@@ -243,3 +243,49 @@ def test_from_packed_f32_and_refusals(be):
     with pytest.raises(lbhip.QuantError) as e:
         be.i8_from_packed(be.upload(lbhip.F32, 300, 512, w))
     assert (e.value.variant, e.value.row) == ("NonFiniteScale", 17)
+
+
+@pytest.mark.parametrize("form", range(1, 11))
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
+def test_every_form_gives_the_same_bits(be, form, gated, ty):
+    """Each form over ragged and whole tiles of its own size, against the rule's choice and the 64-bit value: with the
+    residual (in place and apart), rows at odd addresses, and rows behind the last token left alone."""
+    t = TYPES[ty]
+    for tokens, rows, k in ((1, 1, 1), (19, 272, 320), (64, 64, 64), (130, 200, 1040), (256, 512, 256), (300, 384, 576)):
+        q, s, w, ws = make(tokens, rows, k, seed=form)
+        _, _, v, vs = make(1, rows, k, seed=form + 50)
+        m = be.upload_i8_gated(w, ws, v, vs) if gated else be.upload_i8(w, ws)
+        space = torch.zeros(be.gemm_i8_workspace_bytes(m, tokens), dtype=torch.uint8, device="cuda")
+        x, sd = on_gpu(q, -k % 16), torch.from_numpy(s).cuda()
+        res = None if gated else torch.randn(tokens, rows, generator=torch.Generator().manual_seed(1)).to(t).cuda()
+
+        def call(form, pad, residual):
+            buf = torch.full((tokens + 3, rows + pad), 5.0, dtype=t, device="cuda")
+            y = buf[:tokens, :rows]
+            be.set_tuning(be.TUNE_I8_FORM, form)
+            try:
+                if gated:
+                    be.gemm_i8_swiglu(m, x, sd, y, space)
+                else:
+                    if residual == "place":
+                        y.copy_(res)
+                    be.gemm_i8(m, x, sd, y, space, residual={None: None, "apart": res, "place": y}[residual])
+            finally:
+                be.set_tuning(be.TUNE_I8_FORM, 0)
+            assert bool((buf[tokens:] == 5).all()) and bool((buf[:, rows:] == 5).all())
+            return y.clone()
+
+        first = call(0, 0, None)
+        for pad in (0, 8, 3):
+            assert torch.equal(call(form, pad, None), first), (tokens, rows, k, pad)
+        if gated:
+            g, u = value(q, s, w, ws), value(q, s, v, vs)
+            want = g / (1 + np.exp(-g)) * u
+            check(first, want, t, gated_off(g, u, want))
+        else:
+            check(first, value(q, s, w, ws), t, plain_off(value(q, s, w, ws)))
+            added = call(0, 0, "apart")
+            for pad in (0, 3):
+                assert torch.equal(call(form, pad, "apart"), added) and torch.equal(call(form, pad, "place"), added)
+        m.close()
