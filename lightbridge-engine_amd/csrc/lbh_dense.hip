@@ -113,6 +113,7 @@ lbh_status norm_rows(lbh_ctx *ctx, NormArgs a, size_t rows, size_t n, size_t hs,
     if (rows == 0) return ok(err);
     a.rows = (long long)rows;
     a.n = (int32_t)n;
+    a.inv_n = 1.0 / (double)n;
     a.hidden_stride = (long long)hs;
     a.delta_stride = (long long)ds;
     a.hidden_out_stride = (long long)os;

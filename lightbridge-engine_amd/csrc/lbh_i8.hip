@@ -527,12 +527,12 @@ float estimate(const I8Args &a, const Form &f) {
         const float rounds = ceilf((float)tiles_of(a, f) / cu);
         // the largest tile waits for its residuals (4096 x 12288: T44 227 us, T32 230)
         const float wait = a.residual && f.cw == 4 ? 18.0f * rounds : 0.0f;
-        return 1.5f + wait + fmaxf(rounds * (f.fixed + f.step * (float)a.kt), weights);
+        return 2.0f + wait + fmaxf(rounds * (f.fixed + f.step * (float)a.kt), weights);
     }
     // Two to four workgroups share a CU and its L1, which takes 17.6 ns for a KiB.
     const int per = a.gated ? 2 * f.r : f.r;
     const float n = (float)((groups_of(a) + per - 1) / per) * (float)((a.n_tokens + 16 * f.tw - 1) / (16 * f.tw));
-    return 2.5f + fmaxf(fmaxf(n / cu, 1.0f) * (float)a.kt * (float)(per + f.tw) * 0.0176f, weights);
+    return fmaxf(2.5f + fmaxf(n / cu, 1.0f) * (float)a.kt * (float)(per + f.tw) * 0.0176f, 1.0f + weights);
 }
 
 // The form of the least estimate.  Measured / estimated, in us, for the choice and

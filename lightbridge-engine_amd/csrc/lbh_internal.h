@@ -237,7 +237,7 @@ struct NormArgs {
     long long hidden_stride, delta_stride, hidden_out_stride, y_stride, q_stride;
     long long rows;
     int32_t n, type, y_type, norm;
-    double eps;
+    double eps, inv_n;            // inv_n = 1 / n
 };
 constexpr int NORM_MAX_Q8K = 16384;   // a row of Q8_K input waits in LDS
 

@@ -182,27 +182,34 @@ def _dev_ptr(t) -> int:
     return t.data_ptr()
 
 
-def _rows(t, dtype=None):
-    """(address, row stride) of a two-dimensional CUDA tensor with adjacent row elements; (None, 0) for None."""
-    import torch
+def _space(workspace):
+    """(address, bytes) of a workspace tensor; (None, 0) for None."""
+    return (None, 0) if workspace is None else (_dev_ptr(workspace), workspace.numel() * workspace.element_size())
+
+
+_ROW_TYPES = {}   # torch dtype -> type id of row operands, filled when a backend opens
+
+
+def _rows(t, shape, dtype=None):
+    """(address, row stride) of a CUDA tensor of `shape` = (rows, n) with adjacent row elements; (None, 0) for None."""
     if t is None:
         return None, 0
-    assert isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2, "expected a two-dimensional CUDA tensor"
-    assert t.shape[1] <= 1 or t.stride(1) == 1, "expected rows of adjacent elements"
+    stride = t.stride()
+    assert t.is_cuda and t.shape == shape and len(stride) == 2, f"expected a CUDA tensor of shape {tuple(shape)}"
+    assert stride[1] == 1 or shape[1] <= 1, "expected rows of adjacent elements"
     assert dtype is None or t.dtype == dtype, f"expected {dtype}, got {t.dtype}"
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return t.data_ptr(), stride[0] if shape[0] > 1 else shape[1]
 
 
 def _row_type(t) -> int:
-    import torch
-    ty = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype)
-    assert ty is not None, f"expected float32, float16 or bfloat16 rows, got {t.dtype}"
-    return ty
+    assert t.dtype in _ROW_TYPES, f"expected float32, float16 or bfloat16 rows, got {t.dtype}"
+    return _ROW_TYPES[t.dtype]
 
 
-def _like(t, shape, what: str):
-    assert t is None or tuple(t.shape) == tuple(shape), f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}"
-    return t
+def _vector(t, n: int, dtype, what: str) -> int:
+    """Address of n adjacent values."""
+    assert t.is_cuda and t.dtype == dtype and t.numel() == n and t.is_contiguous(), f"{what}: {n} values of {dtype}"
+    return t.data_ptr()
 
 
 def _call(fn, *args) -> None:
@@ -231,6 +238,8 @@ class HipBackend:
         if not torch.cuda.is_available():
             raise RuntimeError("HipBackend needs a ROCm GPU")
         self.device = device
+        self._f32, self._i8 = torch.float32, torch.int8
+        _ROW_TYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
         torch.cuda.set_device(device)
         self._stream = stream if stream is not None else torch.cuda.current_stream(device)
         h = C.c_void_p()
@@ -395,16 +404,11 @@ class HipBackend:
     # -- dense blocks in 8-bit integers ----------------------------------------------------
     def _norm_args(self, hidden, weight, eps, delta, hidden_out, y):
         """The arguments every norm call begins with, checked against hidden's shape."""
-        import torch
-        n_rows, n = hidden.shape
+        shape, dt = hidden.shape, hidden.dtype
         ty = _row_type(hidden)
-        hp, hs = _rows(hidden)
-        dp, ds = _rows(_like(delta, hidden.shape, "delta"), hidden.dtype)
-        op, os_ = _rows(_like(hidden_out, hidden.shape, "hidden_out"), hidden.dtype)
-        yp, ys = _rows(_like(y, hidden.shape, "y"))
-        assert weight.dtype == torch.float32 and weight.numel() == n, "weight: n float32 values"
-        return (self.ctx, ty, hp, hs, dp, ds, _dev_ptr(weight), eps, n_rows, n, op, os_,
-                _row_type(y) if y is not None else ty, yp, ys)
+        return (self.ctx, ty, *_rows(hidden, shape), *_rows(delta, shape, dt),
+                _vector(weight, shape[1], self._f32, "weight"), eps, shape[0], shape[1], *_rows(hidden_out, shape, dt),
+                ty if y is None else _row_type(y), *_rows(y, shape))
 
     def rms_norm_rows(self, hidden, weight, eps: float, y, delta=None, hidden_out=None) -> None:
         """y = RMS norm of hidden (+ delta, stored in hidden_out when given) [rows, n]; row strides are
@@ -420,20 +424,15 @@ class HipBackend:
 
     def rms_norm_i8_rows(self, hidden, weight, eps: float, q, scales, y=None, delta=None, hidden_out=None) -> None:
         """rms_norm_rows into int8 rows q [rows, n] with float32 scales [rows], and into y when given."""
-        import torch
-        qp, qs = _rows(_like(q, hidden.shape, "q"), torch.int8)
-        assert scales.dtype == torch.float32 and scales.numel() == hidden.shape[0], "scales: a float32 value a row"
-        _call(lib().lbh_rms_norm_i8_rows, *self._norm_args(hidden, weight, eps, delta, hidden_out, y), qp, qs,
-              _dev_ptr(scales))
+        _call(lib().lbh_rms_norm_i8_rows, *self._norm_args(hidden, weight, eps, delta, hidden_out, y),
+              *_rows(q, hidden.shape, self._i8), _vector(scales, hidden.shape[0], self._f32, "scales"))
 
     def quantize_i8_rows(self, x, q, scales) -> None:
         """int8 rows of x [rows, n] with one float32 scale each (max |x| / 127; asynchronous)."""
-        import torch
-        xp, xs = _rows(x)
-        qp, qs = _rows(_like(q, x.shape, "q"), torch.int8)
-        assert scales.dtype == torch.float32 and scales.numel() == x.shape[0], "scales: a float32 value a row"
-        _call(lib().lbh_quantize_i8_rows, self.ctx, _row_type(x), xp, xs, x.shape[0], x.shape[1], qp, qs,
-              _dev_ptr(scales))
+        shape = x.shape
+        xp, xs = _rows(x, shape)
+        _call(lib().lbh_quantize_i8_rows, self.ctx, _row_type(x), xp, xs, shape[0], shape[1],
+              *_rows(q, shape, self._i8), _vector(scales, shape[0], self._f32, "scales"))
 
     def upload_i8(self, weights, scales) -> "DeviceI8Matrix":
         """int8 weights [rows, k] with a float32 scale a row, numpy arrays or CUDA tensors."""
@@ -451,26 +450,20 @@ class HipBackend:
     def gemm_i8_workspace_bytes(m: "DeviceI8Matrix", n_tokens: int) -> int:
         return lib().lbh_gemm_i8_workspace_bytes(m.handle, n_tokens)
 
-    def _product_args(self, m, q, scales, y, workspace, residual=None):
-        import torch
+    def _product_args(self, m, q, scales, y):
         n = q.shape[0]
-        qp, qs = _rows(_like(q, (n, m.k), "q"), torch.int8)
-        yp, ys = _rows(_like(y, (n, m.rows), "y"))
-        rp, rs = _rows(_like(residual, y.shape, "residual"), y.dtype)
-        assert scales.dtype == torch.float32 and scales.numel() == n, "scales: a float32 value a token"
-        wp, wl = (None, 0) if workspace is None else (_dev_ptr(workspace), workspace.numel() * workspace.element_size())
-        return ((self.ctx, m.handle, qp, qs, _dev_ptr(scales), n, _row_type(y), yp, ys), (rp, rs), (wp, wl))
+        return (self.ctx, m.handle, *_rows(q, (n, m.k), self._i8), _vector(scales, n, self._f32, "scales"), n,
+                _row_type(y), *_rows(y, (n, m.rows)))
 
     def gemm_i8(self, m: "DeviceI8Matrix", q, scales, y, workspace=None, residual=None) -> None:
         """y [tokens, rows] = (residual +) int8 rows q [tokens, k] times the matrix, scaled by token and
         channel (asynchronous).  workspace: for rows off 16 bytes (gemm_i8_workspace_bytes)."""
-        head, res, ws = self._product_args(m, q, scales, y, workspace, residual)
-        _call(lib().lbh_gemm_i8, *head, *res, *ws)
+        _call(lib().lbh_gemm_i8, *self._product_args(m, q, scales, y), *_rows(residual, y.shape, y.dtype),
+              *_space(workspace))
 
     def gemm_i8_swiglu(self, m: "DeviceI8Matrix", q, scales, h, workspace=None) -> None:
         """h [tokens, rows] = silu(gate) * up of int8 rows q times a gated pair (asynchronous)."""
-        head, _, ws = self._product_args(m, q, scales, h, workspace)
-        _call(lib().lbh_gemm_i8_swiglu, *head, *ws)
+        _call(lib().lbh_gemm_i8_swiglu, *self._product_args(m, q, scales, h), *_space(workspace))
 
     def f16_to_f32(self, src, dst) -> None:
         _call(lib().lbh_debug_f16_to_f32, self.ctx, _dev_ptr(src), _dev_ptr(dst), src.numel())
