@@ -31,9 +31,11 @@ typedef int i8_v4i __attribute__((ext_vector_type(4)));
 typedef int i8_v16i __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void i8_lds;
 
-// Token rows in LDS: 64 bytes of a token are four pieces, piece c stored at c ^
-// token_swizzle, so that 16 lanes reading one piece of 16 tokens touch every bank.
+// Token rows in LDS: 64 (128) bytes of a token are four (eight) pieces, piece c
+// stored at c ^ swizzle, so that 16 lanes reading one piece of 16 tokens touch every
+// bank.
 __device__ __forceinline__ int token_swizzle(int t) { return (t >> 2) & 3; }
+__device__ __forceinline__ int pair_swizzle(int t) { return (t >> 1) & 7; }
 
 // ------------------------------------------------------------- weight layout
 
@@ -214,6 +216,19 @@ __device__ __forceinline__ void i8_copy(__amdgpu_buffer_rsrc_t r, uint8_t *to, u
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (i8_lds *)to, 16, at, uniform, 0, 0);
 }
 
+// The same with the wait left to the kernel, which counts its copies itself (the
+// compiler waits for every copy before a read that might be of its target).
+__device__ __forceinline__ i8_v4i i8_words(const void *base, long long bytes) {
+    const uint64_t a = reinterpret_cast<uint64_t>(base);
+    return i8_v4i{__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)(a >> 32)),
+                  __builtin_amdgcn_readfirstlane((int)(uint32_t)bytes), 0x00020000};
+}
+__device__ __forceinline__ void i8_copy_asm(const i8_v4i &r, uint32_t to, int plus, uint32_t at, uint32_t uniform) {
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds" ::"s"(to), "i"(plus),
+                 "v"(at), "s"(r), "s"(uniform)
+                 : "memory", "m0", "scc");
+}
+
 // ------------------------------------------------------- few tokens: streaming
 //
 // A workgroup takes R channel groups (gated: pairs of groups) and 16 * TT tokens
@@ -308,16 +323,20 @@ __global__ void __launch_bounds__(64 * ST_WAVES, 4) k_i8_stream(I8Args p) {
 //
 // A workgroup of four waves (2 x 2) computes 64 * CW channels x 64 * TW tokens,
 // each wave CW x TW products of 32 x 32 with v_mfma_i32_32x32x32_i8.  k runs in
-// stages of 64: both operands are copied to LDS three stages ahead into a ring
-// of four buffers (no registers in between).  Weights keep their tile order
-// there; a token's 64 bytes are four pieces, piece c stored at c ^ swizzle of
-// the token, so that 16 lanes reading one piece of 16 tokens touch every bank.
+// stages of 64; operands are copied to LDS ahead of their use, with no registers in
+// between: weights in their tile order, three stages ahead into a ring of four
+// buffers; tokens likewise in rows of 64 bytes, or, in the small tiles, in rows of
+// 128 bytes for a pair of stages, two pairs ahead into a ring of three.  (Rows of 64
+// ask for every cache line twice, and the requests to L2 are what bounds the small
+// tiles: 4096 x 12288 in T22 218 -> 199 us, 256 x 26624 53 -> 43.  The larger tiles
+// have less LDS to spare, and start later with the longer rows: 512 x 12288 in T32
+// 29.0 -> 30.2 us, T44 44.2 -> 47.1.)
 template <int OUT, bool GATED, int CW, int TW>
 __global__ void __launch_bounds__(256, CW * TW > 8 ? 1 : 2) k_i8_tile(I8Args p) {
     constexpr int CH = 64 * CW, TK = 64 * TW;
-    constexpr int A_BYTES = CH * 64, STAGE = (CH + TK) * 64;
-    // Four objects, so that a wait before a read of one leaves the copies into the others in flight.
-    __shared__ __align__(1024) uint8_t lds0[STAGE], lds1[STAGE], lds2[STAGE], lds3[STAGE];
+    constexpr bool PAIRS = CW * TW <= 4;   // token rows of 128 bytes
+    constexpr int W = CH * 64, X = TK * (PAIRS ? 128 : 64);   // a buffer of each ring
+    __shared__ __align__(1024) uint8_t lds[4 * W + (PAIRS ? 3 : 4) * X];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wc = wid & 1, wt = wid >> 1;
     // Tiles of the grid: workgroups go to the eight XCDs in turn, and each XCD
@@ -335,12 +354,12 @@ __global__ void __launch_bounds__(256, CW * TW > 8 ? 1 : 2) k_i8_tile(I8Args p) 
     const int tc = in_panel / width, tt = panel * 8 + in_panel % width;
     const int g0 = tc * (CH / 16), t0 = tt * TK;
     const int nt = min(p.n_tokens - t0, TK);
-    const __amdgpu_buffer_rsrc_t rw =
-        i8_rsrc(p.w + (long long)g0 * p.kt * 1024, (long long)min(groups - g0, CH / 16) * p.kt * 1024);
-    const __amdgpu_buffer_rsrc_t rx = i8_rsrc(p.x + (long long)t0 * p.x_stride, (long long)(nt - 1) * p.x_stride + p.k);
+    const i8_v4i rw = i8_words(p.w + (long long)g0 * p.kt * 1024, (long long)min(groups - g0, CH / 16) * p.kt * 1024);
+    const i8_v4i rx = i8_words(p.x + (long long)t0 * p.x_stride, (long long)(nt - 1) * p.x_stride + p.k);
 
     // The epilogue's layout and scales.
-    constexpr int ROW = CW * 32 + 4;                              // floats; 16 tokens of one channel reach every bank
+    constexpr int ROW = CW * 32;                                  // floats of a token, four by four at c ^ its mask
+    constexpr int MASK = CW % 2 ? 7 : 15;
     constexpr int V = OUT == T_F32 ? 4 : 8;                       // channels of a lane
     constexpr int WIDE = GATED ? CW * 16 : CW * 32;               // channels of the wave
     constexpr int PER = WIDE / V, AT_ONCE = 64 / PER;             // lanes a token, tokens a pass
@@ -351,89 +370,109 @@ __global__ void __launch_bounds__(256, CW * TW > 8 ? 1 : 2) k_i8_tile(I8Args p) 
 #pragma unroll
     for (int n = 0; n < TW; ++n) xs[n] = p.xs[t0 + min((wt * TW + n) * 32 + (lane & 31), nt - 1)];
 
-    // What this wave copies of a stage: CW channel groups of 1 KiB (groups past the
-    // last one repeat it) and TW pieces of 16 tokens x 64 bytes (tokens past the
-    // last one lie behind the resource's end).
+    // What this wave copies in a stage: CW channel groups of 1 KiB (groups past the
+    // last one repeat it), and TW pieces of 16 tokens x 64 bytes, or half of a pair's 2
+    // * TW pieces of 8 tokens x 128 (tokens past the last one lie behind the resource's
+    // end).
     const uint32_t stride = (uint32_t)p.x_stride;
-    const uint32_t vb = (uint32_t)(wid * TW * 16 + (lane >> 2)) * stride + 16 * ((lane & 3) ^ token_swizzle(lane >> 2));
-    auto copy_weights = [&](uint8_t *buf, int kt) {
+    constexpr int TP = PAIRS ? 8 : 16;   // tokens of a piece
+    uint32_t vb[2];   // even and odd pieces: the swizzles of tokens 8 apart differ
 #pragma unroll
-        for (int i = 0; i < CW; ++i) {
-            const int g = wid * CW + i;
-            i8_copy(rw, buf + g * 1024, lane * 16, (min(g, groups - g0 - 1) * p.kt + kt) * 1024);
-        }
-    };
-    auto copy_tokens = [&](uint8_t *buf, int kt) {
+    for (int i = 0; i < 2; ++i) {
+        const int t = PAIRS ? 8 * i + (lane >> 3) : lane >> 2;
+        vb[i] = (uint32_t)(wid * TW * 16 + (PAIRS ? lane >> 3 : lane >> 2)) * stride +
+                16 * (PAIRS ? (lane & 7) ^ pair_swizzle(t) : (lane & 3) ^ token_swizzle(t));
+    }
+    const uint32_t w_lds = (uint32_t)(uintptr_t)(i8_lds *)lds + wid * CW * 1024;
+    const uint32_t x_lds = (uint32_t)(uintptr_t)(i8_lds *)lds + 4 * W + wid * (16 / TP) * TW * 1024;
+    uint32_t row[CW];   // this wave's channel groups
 #pragma unroll
-        for (int i = 0; i < TW; ++i)
-            i8_copy(rx, buf + A_BYTES + (wid * TW + i) * 1024, vb + (uint32_t)i * 16u * stride + kt * 64, 0);
+    for (int i = 0; i < CW; ++i) row[i] = (uint32_t)(min(wid * CW + i, groups - g0 - 1) * p.kt) * 1024u;
+    auto copy_weights = [&](uint32_t buf, int i, uint32_t at) { i8_copy_asm(rw, w_lds + buf, i * 1024, lane * 16, row[i] + at); };
+    auto copy_tokens = [&](uint32_t buf, int i, uint32_t at) {
+        i8_copy_asm(rx, x_lds + buf, i * 1024, vb[i & 1] + ((uint32_t)(i * TP) * stride + at), 0);
     };
 
     // Operands of k piece j (32 of a stage's 64): lane l holds channel (token) l %
     // 32 and k 16 (l / 32) .. + 15 of the 32.
     const int l32 = lane & 31, hi = lane >> 5;
     const int a_at = wc * CW * 2048 + (l32 >> 4) * 1024 + hi * 256 + (l32 & 15) * 16;
-    const int b_at = A_BYTES + (wt * TW * 32 + l32) * 64;
-    const int b_piece = hi ^ token_swizzle(l32);
+    const int b_at = 4 * W + (wt * TW * 32 + l32) * (X / TK);
+    const int b_piece = hi ^ (PAIRS ? pair_swizzle(l32) : token_swizzle(l32));
     i8_v4i a[2][CW], b[2][TW];
-    auto read = [&](const uint8_t *buf, int j, i8_v4i (&fa)[CW], i8_v4i (&fb)[TW]) {
-#pragma unroll
-        for (int i = 0; i < CW; ++i) fa[i] = *reinterpret_cast<const i8_v4i *>(buf + a_at + i * 2048 + j * 512);
-#pragma unroll
-        for (int i = 0; i < TW; ++i)
-            fb[i] = *reinterpret_cast<const i8_v4i *>(buf + b_at + i * 2048 + 16 * (b_piece ^ (2 * j)));
+    // Operand i of a piece, in the order in which the products ask for them.
+    auto read = [&](int i, int wbuf, int xbuf, int half, int j, i8_v4i (&fa)[CW], i8_v4i (&fb)[TW]) {
+        if (i == 0 || i > TW)
+            fa[i ? i - TW : 0] = *reinterpret_cast<const i8_v4i *>(lds + wbuf * W + a_at + (i ? i - TW : 0) * 2048 + j * 512);
+        else
+            fb[i - 1] = *reinterpret_cast<const i8_v4i *>(lds + xbuf * X + b_at + (i - 1) * (X / TK * 32) +
+                                                          16 * (b_piece ^ (PAIRS ? 4 * half + 2 * j : 2 * j)));
     };
     i8_v16i acc[CW][TW] = {};
-    auto multiply = [&](const i8_v4i (&fa)[CW], const i8_v4i (&fb)[TW]) {
+    // The products of one piece, with the reads of the next one and `copies` copies
+    // set between them, one of each after a product.
+    auto piece = [&](const i8_v4i (&fa)[CW], const i8_v4i (&fb)[TW], auto &&next, int copies, auto &&copy) __attribute__((always_inline)) {
+        constexpr int N = CW * TW, READS = (CW + TW + N - 1) / N;
 #pragma unroll
-        for (int i = 0; i < CW; ++i)
+        for (int m = 0; m < N; ++m) {
 #pragma unroll
-            for (int n = 0; n < TW; ++n)
-                acc[i][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[n], acc[i][n], 0, 0, 0);
-    };
-    // Reads and copies go between the products: a read after each of the first
-    // ones, then a copy after each further one.
-    auto mix = [&](int copies) {
-#pragma unroll
-        for (int i = 0; i < CW + TW; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // a read from LDS
-            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);     // a product
-            if (i < copies) __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);   // a copy
+            for (int i = m * READS; i < (m + 1) * READS; ++i)
+                if (i < CW + TW) next(i);
+            acc[m / TW][m % TW] =
+                __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[m / TW], fb[m % TW], acc[m / TW][m % TW], 0, 0, 0);
+            if (m < copies) copy(m);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x8, CW * TW, 0);
-        __builtin_amdgcn_sched_barrier(0);
     };
-    // A stage: `cur` is read, `next` read ahead from, and `free` (the previous
-    // stage's) filled for the third stage from here.  The last stages copy the
-    // last one again.
-    auto stage = [&](const uint8_t *cur, const uint8_t *next, uint8_t *free, int kt) {
-        const int ahead = min(kt + 3, p.kt - 1);
-        read(cur, 1, a[1], b[1]);
-        copy_weights(free, ahead);
-        multiply(a[0], b[0]);
-        mix(CW);
-        // the next stage's copies of this wave are done (two stages' later ones may
-        // be on their way) and its reads of this stage, then everybody's
+    // Stage kt, the first or second `half` of its pair, in weight buffer wb and token
+    // buffer xb; xn: the next stage's token buffer.  The weights of the third stage from
+    // here go to the previous stage's buffer, and to buffer xf the tokens of that stage or
+    // half of those of the second pair from here.  The last stages copy the last ones
+    // again.
+    auto stage = [&](int wb, int xb, int xn, int xf, int kt, int half) __attribute__((always_inline)) {
+        const int ahead = min(kt + 3, p.kt - 1), at = PAIRS ? min(kt / 2 + 2, p.kt / 2 - 1) * 128 : ahead * 64;
+        piece(a[0], b[0], [&](int i) { read(i, wb, xb, half, 1, a[1], b[1]); }, CW,
+              [&](int i) { copy_weights(((wb + 3) & 3) * W, i, ahead * 1024); });
+        // This wave's copies for the next stage are done (younger are at least two
+        // stages' weights and one's tokens) and its reads of this one; then everybody's.
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * CW + TW) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        read(next, 0, a[0], b[0]);
-        copy_tokens(free, ahead);
-        multiply(a[1], b[1]);
-        mix(TW);
+        piece(a[1], b[1], [&](int i) { read(i, (wb + 1) & 3, xn, 1 - half, 0, a[0], b[0]); }, TW,
+              [&](int i) { copy_tokens(xf * X, PAIRS ? half * TW + i : i, at); });
     };
-    copy_weights(lds0, 0), copy_tokens(lds0, 0);
-    copy_weights(lds1, 1), copy_tokens(lds1, 1);
-    copy_weights(lds2, 2), copy_tokens(lds2, 2);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (CW + TW)) : "memory");
+    auto weights = [&](int kt) {
+#pragma unroll
+        for (int i = 0; i < CW; ++i) copy_weights(kt * W, i, kt * 1024);
+    };
+    auto tokens = [&](int n) {   // a stage's, or a pair's
+#pragma unroll
+        for (int i = 0; i < 16 / TP * TW; ++i) copy_tokens(n * X, i, n * (X / TK));
+    };
+    tokens(0), weights(0);
+    if constexpr (PAIRS)
+        weights(1), tokens(1), weights(2);
+    else
+        weights(1), tokens(1), weights(2), tokens(2);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (CW + TW)) : "memory");   // the first stage's are done
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    read(lds0, 0, a[0], b[0]);
-    for (int kt = 0; kt < p.kt; kt += 4) {   // a multiple of four: k is padded to 256
-        stage(lds0, lds1, lds3, kt);
-        stage(lds1, lds2, lds0, kt + 1);
-        stage(lds2, lds3, lds1, kt + 2);
-        stage(lds3, lds0, lds2, kt + 3);
+#pragma unroll
+    for (int i = 0; i < CW + TW; ++i) read(i, 0, 0, 0, 0, a[0], b[0]);
+    if constexpr (PAIRS) {
+        for (int kt = 0, wb = 0, x = 0, xn = 1, xf = 2; kt < p.kt; kt += 2, wb ^= 2) {
+            stage(wb, x, x, xf, kt, 0);
+            stage(wb + 1, x, xn, xf, kt + 1, 1);
+            const int done = x;
+            x = xn, xn = xf, xf = done;
+        }
+    } else {
+        for (int kt = 0; kt < p.kt; kt += 4) {   // k tiles are a multiple of four: k is padded to 256
+            stage(0, 0, 1, 3, kt, 0);
+            stage(1, 1, 2, 0, kt + 1, 1);
+            stage(2, 2, 3, 1, kt + 2, 0);
+            stage(3, 3, 0, 2, kt + 3, 1);
+        }
     }
 
     // D of a 32 x 32 product: lane l holds token l % 32 and channels 8 q + 4 (l /
@@ -442,11 +481,11 @@ __global__ void __launch_bounds__(256, CW * TW > 8 ? 1 : 2) k_i8_tile(I8Args p) 
     // read, scaled and stored in words of 16 bytes, whole lines at a time (stored
     // straight from D, 16 bytes a token and line, the stores took a quarter of the
     // kernel).
-    static_assert(32 * ROW * 4 <= STAGE, "a wave's part fits a buffer");
+    static_assert(32 * ROW * 4 == W, "a wave's part is a buffer of weights");
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    float *turn = reinterpret_cast<float *>(wid < 2 ? (wid ? lds1 : lds0) : (wid == 2 ? lds2 : lds3));
+    float *turn = reinterpret_cast<float *>(lds + wid * W);
     const int from = GATED ? (lc >> 4) * 32 + (lc & 15) : lc;     // a gated pair's groups alternate
     auto put = [&](auto inside, auto with_residual) {
         constexpr bool INSIDE = decltype(inside)::value, RES = decltype(with_residual)::value;
@@ -468,17 +507,24 @@ __global__ void __launch_bounds__(256, CW * TW > 8 ? 1 : 2) k_i8_tile(I8Args p) 
             for (int i = 0; i < CW; ++i)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    *reinterpret_cast<float4 *>(turn + l32 * ROW + i * 32 + 8 * q + 4 * hi) =
+                    *reinterpret_cast<float4 *>(turn + l32 * ROW + 4 * ((8 * i + 2 * q + hi) ^ (l32 & MASK))) =
                         make_float4((float)acc[i][n][4 * q] * xs[n], (float)acc[i][n][4 * q + 1] * xs[n],
                                     (float)acc[i][n][4 * q + 2] * xs[n], (float)acc[i][n][4 * q + 3] * xs[n]);
             wave_sync();
 #pragma unroll
             for (int r = 0; r < 32; r += AT_ONCE) {
                 const int tl = r + lane / PER, t = (wt * TW + n) * 32 + tl;
-                const float *row = turn + min(tl, 31) * ROW + from;
+                const int tr = min(tl, 31);
                 float g[V], u[V];
-                load_row<T_F32, V>(row, g);
-                if constexpr (GATED) load_row<T_F32, V>(row + 16, u);
+#pragma unroll
+                for (int j = 0; j < V; j += 4) {
+                    auto four = [&](int ch, float *to) {
+                        const float4 f = *reinterpret_cast<const float4 *>(turn + tr * ROW + 4 * ((ch / 4) ^ (tr & MASK)));
+                        to[0] = f.x, to[1] = f.y, to[2] = f.z, to[3] = f.w;
+                    };
+                    four(from + j, g + j);
+                    if constexpr (GATED) four(from + 16 + j, u + j);
+                }
                 const bool mine = (64 % PER == 0 || lane < PER * AT_ONCE) && (32 % AT_ONCE == 0 || tl < 32);
                 if (mine && (INSIDE || t < nt))
                     finish<OUT, GATED, INSIDE, V>(p, t0 + t, c, g, u, ws, RES ? &res[r / AT_ONCE] : nullptr);
@@ -510,7 +556,7 @@ struct Form {
 };
 constexpr Form FORMS[] = {
     {0, 1, 1, 0, 0},       {0, 2, 1, 0, 0},       {0, 2, 2, 0, 0},      {0, 4, 1, 0, 0},    {0, 4, 2, 0, 0},
-    {1, 1, 0, 1.5f, 0.10f}, {2, 1, 0, 2.0f, 0.16f}, {2, 2, 0, 2.5f, 0.235f}, {3, 2, 0, 3.5f, 0.32f}, {4, 4, 0, 8.5f, 0.73f}};
+    {1, 1, 0, 1.5f, 0.09f}, {2, 1, 0, 2.0f, 0.14f}, {2, 2, 0, 2.5f, 0.22f}, {3, 2, 0, 3.5f, 0.32f}, {4, 4, 0, 8.5f, 0.73f}};
 constexpr int N_FORMS = sizeof(FORMS) / sizeof(FORMS[0]);
 static_assert(N_FORMS == I8_FORMS, "the forms a context can ask for");
 
@@ -536,16 +582,16 @@ float estimate(const I8Args &a, const Form &f) {
 }
 
 // The form of the least estimate.  Measured / estimated, in us, for the choice and
-// the next ones (tokens x channels, k = 4096; S: stream TT, R; T: tile cw, tw):
-//   1 x 12288     S11 9.3 / 9.3      S12 9.6          32 x 12288    S22 11.4 / 9.3   S21 12.1
-//   64 x 4096     S22 6.3 / 7.0      S41 8.4          96 x 4096     S42 7.9 / 9.3    T11 11.1
-//   256 x 4096    T11 11.8 / 9.4     T21 12.9         128 x 12288   T21 16.0 / 13.7  T11 16.4, T22 18.1
-//   256 x 12288   T22 19.5 / 19.0    T21 23.2         512 x 12288   T32 28.2 / 25.5  T22 33.8, T44 43.5
-//   1024 x 4096 (k = 13312)  T22 57 / 53, T32 64      1024 x 12288  T32 48.8 / 48.5  T44 49.5, T22 56.4
-//   1024 x 26624  T44 116 / 112      T32 141          4096 x 12288  T44 175 / 167    T32 192, T22 219
-// Weights beyond the last cache (109 MB of 26624 channels, three matrices in turn)
-// arrive at some 2.2 TB/s in every tile form: 256 x 26624 takes 52 to 55 us in T22 and
-// T44, whichever is estimated less.
+// measured for the next ones (tokens x channels, k = 4096; S: stream TT, R; T: tile
+// cw, tw):
+//   1 x 12288     S11 9.3 / 10.7     S12 9.6          32 x 12288    S22 11.4 / 10.7   S21 12.1
+//   64 x 4096     S22 6.3 / 7.0      S41 8.4          96 x 4096     S42 7.9 / 9.3     T11 11.6
+//   256 x 4096    T11 12.1 / 9.3     T21 12.9         128 x 12288   T21 15.9 / 13.0   T11 16.0, T22 18
+//   256 x 12288   T22 19.5 / 18.6    T21 21.4         512 x 12288   T32 29.2 / 26.0   T22 32.5, T44 42
+//   1024 x 4096 (k = 13312)  T22 61 / 50, T32 64      1024 x 12288  T32 52.5 / 50     T44 54, T22 56
+//   1024 x 26624  T44 120 / 112      T32 145          4096 x 12288  T44 180 / 167     T22 202, T32 200
+// (Two machines' times; one runs everything some 5% faster than the other.)  Weights
+// beyond the last cache arrive later: 256 x 26624, three matrices in turn, 43 us in T22.
 int plan(const I8Args &a) {
     int best = -1;
     float least = 0.0f;
