@@ -100,9 +100,9 @@ lbh_status check_norm(const NormArgs &a, lbh_error *err) {
 }
 
 // What the four entry points have in common.
-lbh_status norm_rows(lbh_ctx *ctx, NormArgs a, size_t rows, size_t n, size_t hs, size_t ds, size_t os, size_t ys,
-                     size_t qs, lbh_error *err) {
-    if (!ctx || !a.hidden || (a.norm && !a.weight)) return fail(err, LBH_NULL_ARGUMENT);
+lbh_status norm_rows(lbh_ctx *ctx, NormArgs a, bool outputs_missing, size_t rows, size_t n, size_t hs, size_t ds,
+                     size_t os, size_t ys, size_t qs, lbh_error *err) {
+    if (!ctx) return fail(err, LBH_NULL_ARGUMENT);
     if (!float_rows_type(a.type)) return fail(err, LBH_UNSUPPORTED_TYPE, a.type);
     if (a.y && !float_rows_type(a.y_type)) return fail(err, LBH_UNSUPPORTED_TYPE, a.y_type);
     if (n == 0) return fail(err, LBH_ZERO_LOGICAL_ELEMENTS, a.type);
@@ -110,7 +110,8 @@ lbh_status norm_rows(lbh_ctx *ctx, NormArgs a, size_t rows, size_t n, size_t hs,
     if (n > MAX_STRIDE || rows > MAX_TOKENS) return fail(err, LBH_UNSUPPORTED_SHAPE, a.type, 0, MAX_STRIDE, n);
     for (size_t s : {hs, ds, os, ys, qs})
         if (s > ((size_t)1 << 40)) return fail(err, LBH_UNSUPPORTED_SHAPE, a.type, 0, (size_t)1 << 40, s);
-    if (rows == 0) return ok(err);
+    if (rows == 0) return ok(err);   // no row, and no address asked for
+    if (!a.hidden || (a.norm && !a.weight) || outputs_missing) return fail(err, LBH_NULL_ARGUMENT);
     a.rows = (long long)rows;
     a.n = (int32_t)n;
     a.inv_n = 1.0 / (double)n;
@@ -231,11 +232,12 @@ lbh_status create_i8(lbh_ctx *ctx, const int8_t *const *w, const float *const *s
 lbh_status product(lbh_ctx *ctx, const lbh_i8_matrix *m, int gated, const int8_t *x, size_t x_stride, const float *xs,
                    size_t n_tokens, int32_t y_type, void *y, size_t y_stride, const void *residual,
                    size_t residual_stride, void *workspace, size_t workspace_len, lbh_error *err) {
-    if (!ctx || !m || !x || !xs || !y) return fail(err, LBH_NULL_ARGUMENT);
+    if (!ctx || !m) return fail(err, LBH_NULL_ARGUMENT);
     if (m->gated != gated || m->device != ctx->device) return fail(err, LBH_INVALID_PARAMETER, y_type);
     const size_t e = row_elem_bytes(y_type);
     if (!e) return fail(err, LBH_UNSUPPORTED_TYPE, y_type);
-    if (n_tokens == 0) return ok(err);
+    if (n_tokens == 0) return ok(err);   // no token, and no address asked for
+    if (!x || !xs || !y) return fail(err, LBH_NULL_ARGUMENT);
     if (n_tokens > MAX_TOKENS) return fail(err, LBH_UNSUPPORTED_SHAPE, y_type, 0, MAX_TOKENS, n_tokens);
     if (n_tokens == 1) x_stride = m->k, y_stride = m->rows, residual_stride = m->rows;
     if (x_stride < m->k) return fail(err, LBH_DIMENSION_MISMATCH, y_type, 0, m->k, x_stride);
@@ -296,43 +298,41 @@ lbh_status lbh_rms_norm_rows(lbh_ctx *ctx, int32_t type, const void *hidden, siz
                              size_t delta_stride, const float *weight, double eps, size_t rows, size_t n,
                              void *hidden_out, size_t hidden_out_stride, int32_t y_type, void *y, size_t y_stride,
                              lbh_error *err) {
-    if (!y) return fail(err, LBH_NULL_ARGUMENT);
     NormArgs a{};
     a.hidden = hidden, a.delta = delta, a.hidden_out = hidden_out, a.weight = weight, a.y = y;
     a.type = type, a.y_type = y_type, a.norm = 1, a.eps = eps;
-    return norm_rows(ctx, a, rows, n, hidden_stride, delta_stride, hidden_out_stride, y_stride, 0, err);
+    return norm_rows(ctx, a, !y, rows, n, hidden_stride, delta_stride, hidden_out_stride, y_stride, 0, err);
 }
 
 lbh_status lbh_rms_norm_q8_k_rows(lbh_ctx *ctx, int32_t type, const void *hidden, size_t hidden_stride,
                                   const void *delta, size_t delta_stride, const float *weight, double eps, size_t rows,
                                   size_t n, void *hidden_out, size_t hidden_out_stride, int32_t y_type, void *y,
                                   size_t y_stride, uint8_t *encoded, lbh_error *err) {
-    if (!encoded) return fail(err, LBH_NULL_ARGUMENT);
+    if (!ctx) return fail(err, LBH_NULL_ARGUMENT);
     if (n % 256) return fail(err, LBH_LOGICAL_ELEMENTS_NOT_DIVISIBLE, LBH_Q8_K, 0, 256, n);
     if (n > (size_t)NORM_MAX_Q8K) return fail(err, LBH_UNSUPPORTED_SHAPE, LBH_Q8_K, 0, NORM_MAX_Q8K, n);
     NormArgs a{};
     a.hidden = hidden, a.delta = delta, a.hidden_out = hidden_out, a.weight = weight, a.y = y, a.q8k = encoded;
     a.type = type, a.y_type = y_type, a.norm = 1, a.eps = eps;
-    return norm_rows(ctx, a, rows, n, hidden_stride, delta_stride, hidden_out_stride, y_stride, 0, err);
+    return norm_rows(ctx, a, !encoded, rows, n, hidden_stride, delta_stride, hidden_out_stride, y_stride, 0, err);
 }
 
 lbh_status lbh_rms_norm_i8_rows(lbh_ctx *ctx, int32_t type, const void *hidden, size_t hidden_stride, const void *delta,
                                 size_t delta_stride, const float *weight, double eps, size_t rows, size_t n,
                                 void *hidden_out, size_t hidden_out_stride, int32_t y_type, void *y, size_t y_stride,
                                 int8_t *q, size_t q_stride, float *scales, lbh_error *err) {
-    if (!q || !scales) return fail(err, LBH_NULL_ARGUMENT);
     NormArgs a{};
     a.hidden = hidden, a.delta = delta, a.hidden_out = hidden_out, a.weight = weight, a.y = y, a.q = q, a.scale = scales;
     a.type = type, a.y_type = y_type, a.norm = 1, a.eps = eps;
-    return norm_rows(ctx, a, rows, n, hidden_stride, delta_stride, hidden_out_stride, y_stride, q_stride, err);
+    return norm_rows(ctx, a, !q || !scales, rows, n, hidden_stride, delta_stride, hidden_out_stride, y_stride, q_stride,
+                     err);
 }
 
 lbh_status lbh_quantize_i8_rows(lbh_ctx *ctx, int32_t type, const void *x, size_t x_stride, size_t rows, size_t n,
                                 int8_t *q, size_t q_stride, float *scales, lbh_error *err) {
-    if (!q || !scales) return fail(err, LBH_NULL_ARGUMENT);
     NormArgs a{};
     a.hidden = x, a.q = q, a.scale = scales, a.type = type;
-    return norm_rows(ctx, a, rows, n, x_stride, 0, 0, 0, q_stride, err);
+    return norm_rows(ctx, a, !q || !scales, rows, n, x_stride, 0, 0, 0, q_stride, err);
 }
 
 lbh_status lbh_i8_matrix_create(lbh_ctx *ctx, size_t rows, size_t k, const int8_t *weights, const float *scales,

@@ -144,12 +144,13 @@ __device__ __forceinline__ float rounded(float v) {
 
 // g / (1 + exp(-g)) * u.  exp(-g) = 2^z with z = -g log2(e) to some 40 bits (hi +
 // lo), so the argument's rounding does not grow with |g|; below g = -88 the
-// exponent stays there (what is right is below 2^-118 |u|), and 1 / d is the
-// reciprocal with one Newton step.  The library's exp and division cost twice
+// exponent stays there (what is right is below 2^-118 |u|), as above g = 104 (1 + e is
+// 1), which also keeps infinities out of it; and 1 / d is the reciprocal with one
+// Newton step.  The library's exp and division cost twice
 // as many instructions, which is what bounds the epilogue.
 __device__ __forceinline__ float swiglu(float g, float u) {
     constexpr float LOG2E = 0x1.715476p+0f, LOG2E_LO = 0x1.4ae0cp-26f, LN2 = 0x1.62e43p-1f;
-    const float x = fminf(-g, 88.0f);
+    const float x = __builtin_amdgcn_fmed3f(-g, -104.0f, 88.0f);
     const float hi = x * LOG2E;
     const float lo = __builtin_fmaf(x, LOG2E_LO, __builtin_fmaf(x, LOG2E, -hi));
     float e = __builtin_amdgcn_exp2f(hi);

@@ -189,15 +189,64 @@ def test_block_from_packed_weights_next_to_the_q8_k_path(be):
 
 
 def test_empty_calls_leave_everything(be):
+    """No token: nothing happens, with empty tensors (whose address is null) as with none."""
     blk = Block(be, 64, 48, seed=1)
-    y = torch.full((4, 48), 3.0, device="cuda")
-    q, s = torch.zeros(0, 64, dtype=torch.int8, device="cuda"), torch.zeros(0, device="cuda")
-    keep = torch.zeros(16, dtype=torch.uint8, device="cuda")
-    import ctypes as C
-    import lbhip
-    L, err = lbhip.lib(), lbhip.LbhError()
-    some = keep.data_ptr()
-    assert L.lbh_gemm_i8_swiglu(be.ctx, blk.pair.handle, some, 64, some, 0, 0, y.data_ptr(), 48, None, 0, C.byref(err)) == 0
-    assert L.lbh_quantize_i8_rows(be.ctx, 0, some, 64, 0, 64, some, 64, some, C.byref(err)) == 0
+    x, b = torch.zeros(0, 64, device="cuda"), blk.buffers(be, 0, torch.float32)
+    blk.run(be, x, x, b)
+    be.rms_norm_rows(x, blk.weight, EPS, torch.zeros_like(x))
+    be.rms_norm_q8_k_rows(torch.zeros(0, 256, device="cuda"), torch.ones(256, device="cuda"), EPS,
+                          torch.zeros(0, dtype=torch.uint8, device="cuda"))
     torch.cuda.synchronize()
-    assert bool((y == 3).all())
+
+
+def test_calls_on_a_side_stream_wait_for_their_own_stream_alone(be):
+    """The context's stream orders the work: a run on a side stream over inputs written there just before."""
+    ty, tokens = torch.float32, 130
+    blk = Block(be, 512, 640, seed=6)
+    x, d = stream_rows(tokens, 512, ty, 9)
+    want, got = blk.buffers(be, tokens, ty), blk.buffers(be, tokens, ty)
+    blk.run(be, x, d, want)
+    torch.cuda.synchronize()
+    side, before = torch.cuda.Stream(), torch.cuda.current_stream()
+    be.set_stream(side)
+    try:
+        with torch.cuda.stream(side):
+            a, c = torch.zeros_like(x), torch.zeros_like(d)
+            for _ in range(5):
+                a.copy_(x), c.copy_(d)
+                blk.run(be, a, c, got)
+                a.zero_()
+        side.synchronize()
+    finally:
+        be.set_stream(before)
+    assert torch.equal(want.out, got.out) and torch.equal(want.hq, got.hq)
+
+
+def test_two_graphs_with_workspaces_of_their_own(be):
+    """Rows off 16 bytes go through the workspace: two captured runs, each with its own, replayed on two streams at once."""
+    import lbhip
+    ty, tokens = torch.float32, 24
+    blk = Block(be, 300, 333, seed=8)
+    runs = []
+    for i in range(2):
+        x, d = stream_rows(tokens, 300, ty, 20 + i)
+        want, b, stream = blk.buffers(be, tokens, ty), blk.buffers(be, tokens, ty), torch.cuda.Stream()
+        blk.run(be, x, d, want)
+        torch.cuda.synchronize()
+        own = lbhip.HipBackend(0, stream=stream)
+        with torch.cuda.stream(stream):
+            blk.run(own, x, d, b)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            blk.run(own, x, d, b)
+        runs.append((graph, stream, want, b, own, x, d))
+    for _ in range(10):
+        for graph, stream, _, b, *_ in runs:
+            with torch.cuda.stream(stream):
+                b.out.zero_()
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, want, b, own, *_ in runs:
+        assert torch.equal(want.out, b.out)
+        own.close()

@@ -161,6 +161,27 @@ def test_gated_far_arguments(be, tokens):
     check(h, want, torch.float32, gated_off(g, u, want))
 
 
+@pytest.mark.parametrize("tokens", [1, 40, 300])
+def test_gated_products_beyond_the_range(be, tokens):
+    """A gate that overflows to +inf gives inf times the up's sign, one that overflows to -inf is -inf / inf = NaN, as the
+    formula says; the other channels stay as they are."""
+    rows, k = 32, 16
+    q = np.full((tokens, k), 100, np.int8)
+    w, v = np.ones((rows, k), np.int8), np.full((rows, k), 2, np.int8)
+    w[3], w[5], w[6] = 127, -127, 127
+    v[6] = -2
+    s, ws, vs = np.full(tokens, 1e30, np.float32), np.full(rows, 1e-33, np.float32), np.full(rows, 1e-33, np.float32)
+    ws[[3, 5, 6]] = 1e20
+    m = be.upload_i8_gated(w, ws, v, vs)
+    h = torch.zeros(tokens, rows, device="cuda")
+    be.gemm_i8_swiglu(m, on_gpu(q), torch.from_numpy(s).cuda(), h)
+    got = h.cpu().numpy()
+    assert (got[:, 3] == np.inf).all() and (got[:, 6] == -np.inf).all() and np.isnan(got[:, 5]).all()
+    fine = [c for c in range(rows) if c not in (3, 5, 6)]
+    g, u = value(q, s, w, ws)[:, fine], value(q, s, v, vs)[:, fine]
+    check(h[:, fine], g / (1 + np.exp(-g)) * u, torch.float32, gated_off(g, u, g / (1 + np.exp(-g)) * u))
+
+
 @pytest.mark.parametrize("tokens", [1, 40, 130])
 def test_largest_sums(be, tokens):
     """k = 131071 of -128 times -128: 2147467264, the largest sum that int32 has to hold; and its negative."""
@@ -289,3 +310,21 @@ def test_every_form_gives_the_same_bits(be, form, gated, ty):
             for pad in (0, 3):
                 assert torch.equal(call(form, pad, "apart"), added) and torch.equal(call(form, pad, "place"), added)
         m.close()
+
+
+@pytest.mark.parametrize("form", [0, 1, 4, 6, 8, 9, 10])
+def test_rows_far_apart(be, form):
+    """Strides that take the last rows beyond 32 bits: x rows 2^23 bytes apart (2.5 GB), y rows 2^24 elements (10 GB)."""
+    tokens, rows, k = 300, 64, 64
+    q, s, w, ws = make(tokens, rows, k, seed=77)
+    x = torch.empty(tokens * (1 << 23), dtype=torch.int8, device="cuda").view(tokens, 1 << 23)[:, :k]
+    x.copy_(torch.from_numpy(q))
+    y = torch.empty(tokens * (1 << 24), dtype=torch.bfloat16, device="cuda").view(tokens, 1 << 24)[:, :rows]
+    m = be.upload_i8(w, ws)
+    be.set_tuning(be.TUNE_I8_FORM, form)
+    try:
+        be.gemm_i8(m, x, torch.from_numpy(s).cuda(), y)
+    finally:
+        be.set_tuning(be.TUNE_I8_FORM, 0)
+    want = value(q, s, w, ws)
+    check(y, want, torch.bfloat16, plain_off(want))

@@ -221,3 +221,19 @@ def test_many_rows_give_each_row_s_own_bits(be):
         outs.append((q, s, y))
     for a, b in zip(*outs):
         assert torch.equal(a[1234], b[0])
+
+
+def test_rows_far_apart(be):
+    """Rows 2^24 elements apart: the last ones lie beyond 32 bits."""
+    hidden, delta, weight = inputs(200, 640, torch.bfloat16, 9)
+    h, v = oracle_norm(hidden, delta, weight, EPS)
+    x = torch.empty(200 << 24, dtype=torch.bfloat16, device="cuda").view(200, 1 << 24)[:, :640]
+    x.copy_(hidden)
+    q, s = torch.zeros(200, 640, dtype=torch.int8, device="cuda"), torch.zeros(200, device="cuda")
+    y = torch.empty(200 << 23, device="cuda").view(200, 1 << 23)[:, :640]
+    be.rms_norm_i8_rows(x, weight.cuda(), EPS, q, s, y=y, delta=delta.cuda(), hidden_out=x)
+    assert torch.equal(x.cpu(), h)
+    near(y, v, torch.float32)
+    q_want, s_want = oracle_i8(v)
+    np.testing.assert_array_equal(s.cpu().numpy(), s_want)
+    np.testing.assert_array_equal(q.cpu().numpy(), q_want)
