@@ -184,7 +184,10 @@ def _dev_ptr(t) -> int:
 
 def _space(workspace):
     """(address, bytes) of a workspace tensor; (None, 0) for None."""
-    return (None, 0) if workspace is None else (_dev_ptr(workspace), workspace.numel() * workspace.element_size())
+    if workspace is None:
+        return None, 0
+    assert workspace.is_cuda and workspace.is_contiguous(), "expected a contiguous CUDA tensor"
+    return workspace.data_ptr(), workspace.nbytes
 
 
 _ROW_TYPES = {}   # torch dtype -> type id of row operands, filled when a backend opens
@@ -194,21 +197,22 @@ def _rows(t, shape, dtype=None):
     """(address, row stride) of a CUDA tensor of `shape` = (rows, n) with adjacent row elements; (None, 0) for None."""
     if t is None:
         return None, 0
-    stride = t.stride()
-    assert t.is_cuda and t.shape == shape and len(stride) == 2, f"expected a CUDA tensor of shape {tuple(shape)}"
-    assert stride[1] == 1 or shape[1] <= 1, "expected rows of adjacent elements"
-    assert dtype is None or t.dtype == dtype, f"expected {dtype}, got {t.dtype}"
-    return t.data_ptr(), stride[0] if shape[0] > 1 else shape[1]
+    assert t.is_cuda and t.shape == shape, f"expected a CUDA tensor of shape {tuple(shape)}"
+    pitch, step = t.stride()
+    assert step == 1 or shape[1] <= 1, "expected rows of adjacent elements"
+    assert dtype is None or t.dtype is dtype, f"expected {dtype}, got {t.dtype}"
+    return t.data_ptr(), pitch if shape[0] > 1 else shape[1]
 
 
 def _row_type(t) -> int:
-    assert t.dtype in _ROW_TYPES, f"expected float32, float16 or bfloat16 rows, got {t.dtype}"
-    return _ROW_TYPES[t.dtype]
+    ty = _ROW_TYPES.get(t.dtype)
+    assert ty is not None, f"expected float32, float16 or bfloat16 rows, got {t.dtype}"
+    return ty
 
 
 def _vector(t, n: int, dtype, what: str) -> int:
     """Address of n adjacent values."""
-    assert t.is_cuda and t.dtype == dtype and t.numel() == n and t.is_contiguous(), f"{what}: {n} values of {dtype}"
+    assert t.is_cuda and t.dtype is dtype and t.numel() == n and t.is_contiguous(), f"{what}: {n} values of {dtype}"
     return t.data_ptr()
 
 
