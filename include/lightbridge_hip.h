@@ -2,7 +2,8 @@
  * lightbridge_hip.h — C ABI of the MI355X (gfx950) backend for LightBridge's
  * quantized-dot hot path: Q8_K activation quantization, the
  * {IQ2_S, IQ3_S, Q4_K, Q5_K} x Q8_K integer-dot matvecs and the SwiGLU MoE
- * expert FFN built from them.
+ * expert FFN built from them; and of the dense block around such matrices in
+ * plain 8-bit integers (norm, product, gated product).
  *
  * Plain C types only.  Every buffer argument named *_dev is a device pointer
  * (hipMalloc / torch CUDA memory) on the context's device; work is ordered on
@@ -619,10 +620,11 @@ lbh_status lbh_moe_forward_leased(lbh_ctx *ctx, lbh_moe *moe, const lbh_expert_l
 /* ---- dense blocks in 8-bit integers ---------------------------------------------
  * What stands before and around the matrices of a dense layer: the RMS norm of
  * the residual stream with 8-bit outputs, and products of int8 rows (one scale a
- * token) with int8 channels (one scale a channel).  The reference's dense block
- * is residual_add_in_place and rms_norm_into (crates/bridge-kernels-reference/
- * src/norm.rs) around gemv_into on Q8_K rows; the Q8_K form below feeds this
- * header's Q8_K products bit for bit, the int8 forms have no counterpart there.
+ * token) with int8 channels (one scale a channel).  The reference has its norm and
+ * residual addition in crates/bridge-kernels-reference/src/norm.rs, in 32 bits; the
+ * norm here is held to its formula in 64 bits instead, its Q8_K form gives the bytes
+ * that lbh_quantize_q8_k_rows gives for its float32 rows, and the int8 forms have no
+ * counterpart there.
  *
  * Row operands are float32, binary16 or bfloat16 (LBH_F32, LBH_F16, LBH_BF16);
  * strides count elements, are at least the row's length, and bytes between the
