@@ -72,6 +72,16 @@ __device__ __forceinline__ int nearest_of_product(double a, double b) {
     return (int)(uint32_t)__builtin_bit_cast(uint64_t, __builtin_fma(a, b, 0x1.8p52));
 }
 
+// The nearest integer of x / s, ties to even, of 32-bit x and s with |x / s| <= 127
+// (1 + 2^-24), from inv = 1 / s in 64 bits.  The product is off by 2^-45 at most, so a
+// quotient that is a tie may land beside it; one that is none is at least 2^-26 away
+// from a tie (2 x - (2 i + 1) s is a multiple of x's or s's last bit).  The first sum
+// rounds to multiples of 2^-30, which puts the former on the tie and leaves the latter on
+// their side; the second one is nearest_of_product's.
+__device__ __forceinline__ int nearest_of_quotient(double x, double inv) {
+    return (int)(uint32_t)__builtin_bit_cast(uint64_t, __builtin_fma(x, inv, 0x1.8p22) + (0x1.8p52 - 0x1.8p22));
+}
+
 // Eight consecutive elements at an address of 16 bytes.
 template <int TY>
 __device__ __forceinline__ void load8(const row_t<TY> *p, float (&v)[8]) {
@@ -237,6 +247,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_rows(NormArgs p)
         if (tid == 0 && live) p.scale[rr] = scale;
     }
     const bool blank = to_q == 0.0;   // zeros, whatever the row holds
+    auto int8_of = [&](Product x) { return NORM ? nearest_of_product(x, to_q) : nearest_of_quotient(x, to_q); };
 
     auto emit = [&](int i, const Product (&hw)[8]) {
         if constexpr (VEC) {
@@ -246,7 +257,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_rows(NormArgs p)
                 uint32_t q[2] = {0, 0};
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    q[j >> 2] |= (uint32_t)(nearest_of_product((double)hw[j], to_q) & 0xff) << (8 * (j & 3));
+                    q[j >> 2] |= (uint32_t)(int8_of(hw[j]) & 0xff) << (8 * (j & 3));
                 *reinterpret_cast<uint2 *>(p.q + rr * p.q_stride + e) = blank ? make_uint2(0, 0) : make_uint2(q[0], q[1]);
             }
             if (p.y || p.q8k) {
@@ -269,7 +280,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_rows(NormArgs p)
             for (int j = 0; j < 8; ++j) {
                 const int e = at(i, j);
                 if (e >= n || !live) continue;
-                if (p.q) p.q[rr * p.q_stride + e] = (int8_t)(blank ? 0 : nearest_of_product((double)hw[j], to_q));
+                if (p.q) p.q[rr * p.q_stride + e] = (int8_t)(blank ? 0 : int8_of(hw[j]));
                 if (p.y || p.q8k) {
                     const float v = (float)((double)hw[j] * r);
                     if (p.y && p.y_type == T_F32)
@@ -316,7 +327,7 @@ hipError_t launch_norm_form(const NormArgs &a, hipStream_t s) {
     // workgroup on a CU: 333 rows of 7168 took two rounds), of 16384 in 1024
     // threads'.  Q8_K blocks go through LDS, which only the workgroup-per-row forms
     // have.  Measured, input and output bytes a second: 6007 x 4096 bf16 with the
-    // residual to int8 4.3 TB/s, int8 of 1024 x 13312 f32 5.0 TB/s; one row of 4096
+    // residual to int8 4.3 TB/s, int8 of 1024 x 13312 f32 4.8 TB/s; one row of 4096
     // 3.5 us and 64 rows 4.1 us, which is latency.
     const size_t lds = a.q8k ? (size_t)a.n * 4 : 0;
     if (a.n <= 512 && !a.q8k)

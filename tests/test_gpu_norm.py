@@ -179,6 +179,41 @@ def test_ties_zeros_and_values_that_are_not_finite(be, n):
     np.testing.assert_array_equal(np.isnan(y.cpu().numpy()), np.isnan(v))
 
 
+@pytest.mark.parametrize("ty", ["f32", "f16"])
+@pytest.mark.parametrize("scale", [3.0, 5.0, 7.0, 13.0])
+@pytest.mark.parametrize("n", [255, 256, 4096, 17000])
+def test_quantize_ties_of_scales_that_are_no_power_of_two(be, n, scale, ty):
+    """x = scale * (i + 1/2): the quotient is a tie exactly, though 1 / scale is no float of any width."""
+    x = ((torch.arange(n) % 253 - 126.5) * scale).to(TYPES[ty]).repeat(3, 1)
+    x[:, 0] = 127 * scale
+    x[1] = -x[1]
+    x[2] = x[2] * 2.0 ** -9
+    q_want, s_want = oracle_i8(x.double().numpy())
+    assert s_want[0] == scale and s_want[2] == scale / 512 and q_want[0, 127] == 0 and q_want[0, 128] == 2
+    for pad, offset in ((0, 0), (3, 1)):
+        _, xd = strided(x, pad, offset)
+        q, s = torch.zeros(3, n, dtype=torch.int8, device="cuda"), torch.zeros(3, device="cuda")
+        be.quantize_i8_rows(xd, q, s)
+        np.testing.assert_array_equal(s.cpu().numpy(), s_want)
+        np.testing.assert_array_equal(q.cpu().numpy(), q_want)
+
+
+def test_quantize_values_next_to_ties(be):
+    """The float32 neighbours of scale * (i + 1/2) fall to their own sides."""
+    for scale in (3.0, 2.0 ** -100 * 1.7, 0.1, 12345.678):
+        s32 = np.float32(127 * np.float64(scale))
+        s32 = np.float32(np.float64(s32) / 127)
+        mid = (np.arange(254) - 126.5) * np.float64(s32)
+        x = np.stack([np.float32(mid), np.nextafter(np.float32(mid), np.float32(np.inf)),
+                      np.nextafter(np.float32(mid), np.float32(-np.inf))])
+        x[:, 0] = np.float32(127 * np.float64(s32))
+        q_want, s_want = oracle_i8(x.astype(np.float64))
+        q, s = torch.zeros(3, 254, dtype=torch.int8, device="cuda"), torch.zeros(3, device="cuda")
+        be.quantize_i8_rows(torch.from_numpy(x).cuda(), q, s)
+        np.testing.assert_array_equal(s.cpu().numpy(), s_want)
+        np.testing.assert_array_equal(q.cpu().numpy(), q_want)
+
+
 def test_weight_that_is_not_finite(be):
     x, _, w = inputs(3, 700, torch.float32, 4, delta=False)
     w[9] = float("nan")
