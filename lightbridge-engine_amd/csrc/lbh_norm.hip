@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_rows(NormArgs p)
     if (p.q) {
         const double s = top * r * (1.0 / 127.0);
         float scale = (float)s;
-        if (any_odd || !(ssq < __builtin_inf()) || !(s < 0x1.fffffep127))
+        if (any_odd || !(ssq < __builtin_inf()) || !(scale < __builtin_inff()))
             scale = __builtin_nanf("");
         else if (scale < 0x1p-126f)
             scale = 0.0f;

@@ -214,6 +214,27 @@ def test_quantize_values_next_to_ties(be):
         np.testing.assert_array_equal(q.cpu().numpy(), q_want)
 
 
+def test_largest_scale(be):
+    """A scale that is the largest float32 is finite; one past it is not."""
+    n, top = 127 * 127, np.finfo(np.float32).max
+    x = torch.zeros(2, n)
+    x[:, 5] = 1.0                              # times 127 after the norm
+    x[1, 6] = 1.0                              # and times 127 / sqrt(2)
+    weight = torch.ones(n)
+    weight[5] = float(top)
+    q, s = torch.zeros(2, n, dtype=torch.int8, device="cuda"), torch.zeros(2, device="cuda")
+    be.rms_norm_i8_rows(x.cuda(), weight.cuda(), 1e-300, q, s)
+    assert s[0].item() == top and q[0, 5].item() == 127 and int(q[0].abs().sum()) == 127
+    assert s[1].item() < top and q[1, 5].item() == 127 and q[1, 6].item() == 0
+    x = torch.zeros(1, 128 * 128)
+    x[0, 5] = 1.0                              # times 128: 128 / 127 of the largest scale
+    weight = torch.ones(128 * 128)
+    weight[5] = float(top)
+    q = torch.ones(1, 128 * 128, dtype=torch.int8, device="cuda")
+    be.rms_norm_i8_rows(x.cuda(), weight.cuda(), 1e-300, q, s[:1])
+    assert bool(torch.isnan(s[0])) and not bool(q.any())
+
+
 def test_weight_that_is_not_finite(be):
     x, _, w = inputs(3, 700, torch.float32, 4, delta=False)
     w[9] = float("nan")
