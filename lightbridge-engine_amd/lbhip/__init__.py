@@ -762,7 +762,8 @@ class DeviceI8Matrix:
                 continue
             if on_device:
                 assert w.dtype == torch.int8 and s.dtype == torch.float32, "int8 weights with float32 scales"
-                w, s = w.contiguous(), s.contiguous()
+                with torch.cuda.stream(be._stream):   # a copy is made where the upload reads it
+                    w, s = w.contiguous(), s.contiguous()
                 args += [_dev_ptr(w), _dev_ptr(s)]
             else:
                 w, s = np.ascontiguousarray(w), np.ascontiguousarray(s)

@@ -182,6 +182,24 @@ def test_gated_products_beyond_the_range(be, tokens):
     check(h[:, fine], g / (1 + np.exp(-g)) * u, torch.float32, gated_off(g, u, g / (1 + np.exp(-g)) * u))
 
 
+@pytest.mark.parametrize("tokens", [1, 40, 300])
+def test_gated_far_arguments_times_large_values(be, tokens):
+    """Gates below -104, where exp(-g) lies beyond float32 and the gate's factor below 2^-142, next to ups of 1e36:
+    the products lie below 1e-5, as 0 does."""
+    rows, k = 32, 16
+    q = np.zeros((tokens, k), np.int8)
+    q[:, 0], q[:, 1] = 100, 100
+    w, v = np.zeros((rows, k), np.int8), np.zeros((rows, k), np.int8)
+    w[:, 0], v[:, 1] = np.linspace(-127, -104, rows).astype(np.int8), 100
+    s, ws, vs = np.ones(tokens, np.float32), np.full(rows, 0.01001, np.float32), np.full(rows, 1e32, np.float32)
+    g = value(q, s, w, ws)
+    assert g.max() < -104 and g.min() > -128
+    m = be.upload_i8_gated(w, ws, v, vs)
+    h = torch.zeros(tokens, rows, device="cuda")
+    be.gemm_i8_swiglu(m, on_gpu(q), torch.from_numpy(s).cuda(), h)
+    assert float(h.abs().max()) < 1e-5
+
+
 @pytest.mark.parametrize("tokens", [1, 40, 130])
 def test_largest_sums(be, tokens):
     """k = 131071 of -128 times -128: 2147467264, the largest sum that int32 has to hold; and its negative."""
@@ -264,6 +282,25 @@ def test_from_packed_f32_and_refusals(be):
     with pytest.raises(lbhip.QuantError) as e:
         be.i8_from_packed(be.upload(lbhip.F32, 300, 512, w))
     assert (e.value.variant, e.value.row) == ("NonFiniteScale", 17)
+
+
+def test_strided_device_weights_are_copied_in_the_backend_s_stream(be):
+    """The copy that makes device weights contiguous runs where the upload reads it, whatever waits on the stream that
+    is current."""
+    import lbhip
+    r = np.random.default_rng(3)
+    wide = torch.from_numpy(r.integers(-128, 128, (512, 4096), dtype=np.int8)).cuda()
+    scales = torch.from_numpy(r.random((512, 2)).astype(np.float32)).cuda()
+    w, s = wide[:, 1000:3000], scales[:, 1]
+    torch.cuda.synchronize()
+    other = lbhip.HipBackend(0, stream=torch.cuda.Stream())
+    torch.cuda._sleep(200_000_000)   # some 0.1 s of work in the current stream
+    m = other.upload_i8(w, s)
+    got = m.read()
+    assert np.array_equal(got[0], w.cpu().numpy()) and np.array_equal(got[1], s.cpu().numpy())
+    m.close()
+    torch.cuda.synchronize()
+    other.close()
 
 
 @pytest.mark.parametrize("form", range(1, 11))
