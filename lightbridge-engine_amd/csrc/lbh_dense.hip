@@ -193,6 +193,8 @@ lbh_status create_i8(lbh_ctx *ctx, const int8_t *const *w, const float *const *s
     *out = nullptr;
     for (int i = 0; i < parts; ++i)
         if (!w[i] || !scales[i]) return fail(err, LBH_NULL_ARGUMENT);
+    for (int i = 0; i < parts; ++i)
+        if (on_device && !aligned_to(scales[i], 4)) return fail(err, LBH_INVALID_PARAMETER);
     lbh_status st = check_i8_shape(rows, k, err);
     if (st) return st;
     DeviceGuard g(ctx->device);
@@ -389,12 +391,14 @@ lbh_status lbh_i8_matrix_from_packed(lbh_ctx *ctx, const lbh_matrix *m, const lb
                                               (long long)k, 0, ctx->stream));
                 else
                     HIP_TRY(launch_dequant_rows(v, (long long)r0, (long long)n, f, ctx->stream));
-                NormArgs a{};
-                a.hidden = f, a.hidden_stride = (long long)k, a.type = T_F32;
-                a.q = static_cast<int8_t *>(codes.p) + r0 * k, a.q_stride = (long long)k;
-                a.scale = static_cast<float *>(scales.p) + r0;
-                a.rows = (long long)n, a.n = (int32_t)k;
-                HIP_TRY(launch_norm_rows(a, ctx->stream));
+                for (size_t r = 0; r < n; r += MAX_TOKENS) {   // one launch's rows at a time
+                    NormArgs a{};
+                    a.hidden = f + r * k, a.hidden_stride = (long long)k, a.type = T_F32;
+                    a.q = static_cast<int8_t *>(codes.p) + (r0 + r) * k, a.q_stride = (long long)k;
+                    a.scale = static_cast<float *>(scales.p) + r0 + r;
+                    a.rows = (long long)(n - r < MAX_TOKENS ? n - r : MAX_TOKENS), a.n = (int32_t)k;
+                    HIP_TRY(launch_norm_rows(a, ctx->stream));
+                }
             }
             const float *sc = static_cast<const float *>(scales.p);
             const lbh_status s2 = check_i8_scales(ctx, sc, rows, (uint32_t)i, err);

@@ -182,22 +182,24 @@ def _dev_ptr(t) -> int:
     return t.data_ptr()
 
 
-def _space(workspace):
+def _space(device, workspace):
     """(address, bytes) of a workspace tensor; (None, 0) for None."""
     if workspace is None:
         return None, 0
-    assert workspace.is_cuda and workspace.is_contiguous(), "expected a contiguous CUDA tensor"
+    assert workspace.get_device() == device, f"expected a tensor on GPU {device}"
+    assert workspace.is_contiguous(), "expected a contiguous tensor"
     return workspace.data_ptr(), workspace.nbytes
 
 
 _ROW_TYPES = {}   # torch dtype -> type id of row operands, filled when a backend opens
 
 
-def _rows(t, shape, dtype=None):
-    """(address, row stride) of a CUDA tensor of `shape` = (rows, n) with adjacent row elements; (None, 0) for None."""
+def _rows(device, t, shape, dtype=None):
+    """(address, row stride) of a tensor of `shape` = (rows, n) with adjacent row elements on GPU `device`; (None, 0)
+    for None."""
     if t is None:
         return None, 0
-    assert t.is_cuda and t.shape == shape, f"expected a CUDA tensor of shape {tuple(shape)}"
+    assert t.get_device() == device and t.shape == shape, f"expected a tensor of shape {tuple(shape)} on GPU {device}"
     pitch, step = t.stride()
     assert step == 1 or shape[1] <= 1, "expected rows of adjacent elements"
     assert dtype is None or t.dtype is dtype, f"expected {dtype}, got {t.dtype}"
@@ -210,9 +212,10 @@ def _row_type(t) -> int:
     return ty
 
 
-def _vector(t, n: int, dtype, what: str) -> int:
+def _vector(device, t, n: int, dtype, what: str) -> int:
     """Address of n adjacent values."""
-    assert t.is_cuda and t.dtype is dtype and t.numel() == n and t.is_contiguous(), f"{what}: {n} values of {dtype}"
+    assert t.get_device() == device and t.dtype is dtype and t.numel() == n and t.is_contiguous(), \
+        f"{what}: expected {n} values of {dtype} on GPU {device}"
     return t.data_ptr()
 
 
@@ -408,11 +411,11 @@ class HipBackend:
     # -- dense blocks in 8-bit integers ----------------------------------------------------
     def _norm_args(self, hidden, weight, eps, delta, hidden_out, y):
         """The arguments every norm call begins with, checked against hidden's shape."""
-        shape, dt = hidden.shape, hidden.dtype
+        dev, shape, dt = self.device, hidden.shape, hidden.dtype
         ty = _row_type(hidden)
-        return (self.ctx, ty, *_rows(hidden, shape), *_rows(delta, shape, dt),
-                _vector(weight, shape[1], self._f32, "weight"), eps, shape[0], shape[1], *_rows(hidden_out, shape, dt),
-                ty if y is None else _row_type(y), *_rows(y, shape))
+        return (self.ctx, ty, *_rows(dev, hidden, shape), *_rows(dev, delta, shape, dt),
+                _vector(dev, weight, shape[1], self._f32, "weight"), eps, shape[0], shape[1],
+                *_rows(dev, hidden_out, shape, dt), ty if y is None else _row_type(y), *_rows(dev, y, shape))
 
     def rms_norm_rows(self, hidden, weight, eps: float, y, delta=None, hidden_out=None) -> None:
         """y = RMS norm of hidden (+ delta, stored in hidden_out when given) [rows, n]; row strides are
@@ -421,6 +424,7 @@ class HipBackend:
 
     def rms_norm_q8_k_rows(self, hidden, weight, eps: float, encoded, y=None, delta=None, hidden_out=None) -> None:
         """rms_norm_rows into Q8_K blocks (rows * n / 256 * 292 bytes), and into y when given."""
+        assert encoded.get_device() == self.device, f"expected a tensor on GPU {self.device}"
         n_rows, n = hidden.shape
         assert n % 256 or encoded.numel() * encoded.element_size() == n_rows * (n // 256) * Q8_K_BLOCK_BYTES, "encoded"
         _call(lib().lbh_rms_norm_q8_k_rows, *self._norm_args(hidden, weight, eps, delta, hidden_out, y),
@@ -428,15 +432,16 @@ class HipBackend:
 
     def rms_norm_i8_rows(self, hidden, weight, eps: float, q, scales, y=None, delta=None, hidden_out=None) -> None:
         """rms_norm_rows into int8 rows q [rows, n] with float32 scales [rows], and into y when given."""
+        dev = self.device
         _call(lib().lbh_rms_norm_i8_rows, *self._norm_args(hidden, weight, eps, delta, hidden_out, y),
-              *_rows(q, hidden.shape, self._i8), _vector(scales, hidden.shape[0], self._f32, "scales"))
+              *_rows(dev, q, hidden.shape, self._i8), _vector(dev, scales, hidden.shape[0], self._f32, "scales"))
 
     def quantize_i8_rows(self, x, q, scales) -> None:
         """int8 rows of x [rows, n] with one float32 scale each (max |x| / 127; asynchronous)."""
-        shape = x.shape
-        xp, xs = _rows(x, shape)
+        dev, shape = self.device, x.shape
+        xp, xs = _rows(dev, x, shape)
         _call(lib().lbh_quantize_i8_rows, self.ctx, _row_type(x), xp, xs, shape[0], shape[1],
-              *_rows(q, shape, self._i8), _vector(scales, shape[0], self._f32, "scales"))
+              *_rows(dev, q, shape, self._i8), _vector(dev, scales, shape[0], self._f32, "scales"))
 
     def upload_i8(self, weights, scales) -> "DeviceI8Matrix":
         """int8 weights [rows, k] with a float32 scale a row, numpy arrays or CUDA tensors."""
@@ -455,19 +460,21 @@ class HipBackend:
         return lib().lbh_gemm_i8_workspace_bytes(m.handle, n_tokens)
 
     def _product_args(self, m, q, scales, y):
-        n = q.shape[0]
-        return (self.ctx, m.handle, *_rows(q, (n, m.k), self._i8), _vector(scales, n, self._f32, "scales"), n,
-                _row_type(y), *_rows(y, (n, m.rows)))
+        dev, n = self.device, q.shape[0]
+        return (self.ctx, m.handle, *_rows(dev, q, (n, m.k), self._i8), _vector(dev, scales, n, self._f32, "scales"), n,
+                _row_type(y), *_rows(dev, y, (n, m.rows)))
 
     def gemm_i8(self, m: "DeviceI8Matrix", q, scales, y, workspace=None, residual=None) -> None:
         """y [tokens, rows] = (residual +) int8 rows q [tokens, k] times the matrix, scaled by token and
         channel (asynchronous).  workspace: for rows off 16 bytes (gemm_i8_workspace_bytes)."""
-        _call(lib().lbh_gemm_i8, *self._product_args(m, q, scales, y), *_rows(residual, y.shape, y.dtype),
-              *_space(workspace))
+        dev = self.device
+        _call(lib().lbh_gemm_i8, *self._product_args(m, q, scales, y), *_rows(dev, residual, y.shape, y.dtype),
+              *_space(dev, workspace))
 
     def gemm_i8_swiglu(self, m: "DeviceI8Matrix", q, scales, h, workspace=None) -> None:
         """h [tokens, rows] = silu(gate) * up of int8 rows q times a gated pair (asynchronous)."""
-        _call(lib().lbh_gemm_i8_swiglu, *self._product_args(m, q, scales, h), *_space(workspace))
+        _call(lib().lbh_gemm_i8_swiglu, *self._product_args(m, q, scales, h),
+              *_space(self.device, workspace))
 
     def f16_to_f32(self, src, dst) -> None:
         _call(lib().lbh_debug_f16_to_f32, self.ctx, _dev_ptr(src), _dev_ptr(dst), src.numel())
@@ -762,6 +769,7 @@ class DeviceI8Matrix:
                 continue
             if on_device:
                 assert w.dtype == torch.int8 and s.dtype == torch.float32, "int8 weights with float32 scales"
+                assert w.get_device() == s.get_device() == be.device, f"expected tensors on GPU {be.device}"
                 with torch.cuda.stream(be._stream):   # a copy is made where the upload reads it
                     w, s = w.contiguous(), s.contiguous()
                 args += [_dev_ptr(w), _dev_ptr(s)]

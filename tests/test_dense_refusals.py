@@ -148,6 +148,8 @@ def test_matrix_refusals(ctx):
     assert status(pair, ctx, 4, 4, A, A, 0, A, 1, C.byref(h))[0] == "NullArgument"
     assert status(pair, ctx, 4, 4, A, A, A, 0, 1, C.byref(h))[0] == "NullArgument"
     assert not h.value
+    assert status(new, ctx, 4, 4, A, A + 2, 1, C.byref(h))[0] == "InvalidParameter"
+    assert status(pair, ctx, 4, 4, A, A, A, A + 1, 1, C.byref(h))[0] == "InvalidParameter"
     m = Matrix(rows=4, k=8, kt=2, groups=1)
     read = L.lbh_i8_matrix_read
     assert status(read, ctx, None, 0, A, 32, A, 4)[0] == "NullArgument"
@@ -163,3 +165,30 @@ def test_the_form_knob_s_range(ctx):
     be = lbhip.HipBackend
     assert [fn(ctx, be.TUNE_I8_FORM, v) for v in (-1, 11)] == [25, 25]
     assert [fn(ctx, be.TUNE_I8_FORM, v) for v in (1, 10, 0)] == [0, 0, 0]
+
+
+def test_tensors_of_another_device():
+    """The Python calls take tensors of their backend's GPU only."""
+    torch = pytest.importorskip("torch")
+
+    class Elsewhere:
+        def __init__(self, t, device):
+            self.t, self.device = t, device
+
+        def get_device(self):
+            return self.device
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+    rows, scales = torch.zeros(2, 4), torch.zeros(2)
+    assert lbhip._rows(1, Elsewhere(rows, 1), (2, 4)) == (rows.data_ptr(), 4)
+    assert lbhip._vector(1, Elsewhere(scales, 1), 2, torch.float32, "scales") == scales.data_ptr()
+    assert lbhip._space(1, Elsewhere(rows, 1)) == (rows.data_ptr(), 32)
+    for device in (-1, 1):
+        with pytest.raises(AssertionError):
+            lbhip._rows(0, Elsewhere(rows, device), (2, 4))
+        with pytest.raises(AssertionError):
+            lbhip._vector(0, Elsewhere(scales, device), 2, torch.float32, "scales")
+        with pytest.raises(AssertionError):
+            lbhip._space(0, Elsewhere(rows, device))
