@@ -119,9 +119,9 @@ enum lbh_tuning_key {
     LBH_TUNE_I8_FORM = 5,          /* int8 product kernel: 0 = default (by rows, tokens and k); 1-5 =
                                       streaming, k split over a workgroup's waves, of (16-token tiles,
                                       16-channel groups) (1,1), (2,1), (2,2), (4,1), (4,2); 6-10 = tiles
-                                      of 64 * (1,1), (2,1), (2,2), (3,2), (4,4) channels x tokens.  A
-                                      gated pair runs 3 as 2 and 5 as 4.  Every choice gives the same
-                                      bits */
+                                      of 64 * (1,1), (2,1), (2,2), (3,2), (4,4) channels x tokens; 11 =
+                                      streaming of (1,2).  A gated pair runs 3 as 2, 5 as 4 and 11 as 1.
+                                      Every choice gives the same bits */
 };
 lbh_status lbh_ctx_set_tuning(lbh_ctx *ctx, int32_t key, int32_t value);
 /* Compute units of the context's device. */

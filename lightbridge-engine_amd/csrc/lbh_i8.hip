@@ -208,9 +208,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t i8_rsrc(const void *base, long
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, (int)(uint32_t)bytes, 0x00020000);
 }
 
-// 16 bytes at a byte offset, zero past the resource's end.
+// 16 bytes at a byte offset, zero past the resource's end.  ONCE: non-temporal.
+template <bool ONCE>
 __device__ __forceinline__ i8_v4i i8_load(__amdgpu_buffer_rsrc_t r, uint32_t at) {
-    return __builtin_bit_cast(i8_v4i, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+    return __builtin_bit_cast(i8_v4i, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, ONCE ? 2 : 0));
 }
 
 // 16 bytes a lane straight to LDS, lane l's at to + 16 l.
@@ -239,13 +240,15 @@ __device__ __forceinline__ void i8_copy_asm(const i8_v4i &r, uint32_t to, int pl
 // Weights go straight to operand registers; tokens through LDS: 16 tokens x 64
 // bytes read straight into operand registers touch 64 lines an instruction, which
 // costs the L1 four times what the bytes do, and copied to LDS in the order of
-// memory they touch 16 (64 tokens x 12288 channels x 4096: 25.9 -> 18.0 us; with
-// R = 2, 15.0).  Each wave has two buffers of its own, so nobody waits for another
+// memory they touch 16 (64 tokens x 12288 channels x 4096: 25.9 -> 18.0 us).  With R =
+// 2 the tokens of 32 channels are copied once: where the weights come from HBM, each
+// workgroup's tokens beside them cost as much as a quarter of the weights (16 x 24000:
+// 24.4 -> 20.0 us).  Each wave has two buffers of its own, so nobody waits for another
 // wave before the join.  Bound: up to some 16 tokens the weights' bytes (one token
 // x 12288 x 4096: 9.3 us, 5.4 TB/s), then the L1's (R + TT) KiB a k tile.
 constexpr int ST_WAVES = 8;
 
-template <int OUT, bool GATED, int TT, int R>
+template <int OUT, bool GATED, int TT, int R, bool ONCE>
 __global__ void __launch_bounds__(64 * ST_WAVES, 4) k_i8_stream(I8Args p) {
     constexpr int G = GATED ? 2 * R : R;
     __shared__ __align__(1024) uint8_t x0[ST_WAVES][TT * 1024], x1[ST_WAVES][TT * 1024];
@@ -267,7 +270,7 @@ __global__ void __launch_bounds__(64 * ST_WAVES, 4) k_i8_stream(I8Args p) {
         // past the last tile (or group): out of the resource's range, zero
 #pragma unroll
         for (int g = 0; g < G; ++g)
-            a[g] = i8_load(rw, lane * 16 + (kt < p.kt ? g * p.kt + kt : G * p.kt) * 1024);
+            a[g] = i8_load<ONCE>(rw, lane * 16 + (kt < p.kt ? g * p.kt + kt : G * p.kt) * 1024);
 #pragma unroll
         for (int i = 0; i < TT; ++i)
             i8_copy(rx, x + i * 1024, from[i] + kt * 64, 0);
@@ -558,7 +561,8 @@ struct Form {
 };
 constexpr Form FORMS[] = {
     {0, 1, 1, 0, 0},       {0, 2, 1, 0, 0},       {0, 2, 2, 0, 0},      {0, 4, 1, 0, 0},    {0, 4, 2, 0, 0},
-    {1, 1, 0, 1.5f, 0.09f}, {2, 1, 0, 2.0f, 0.14f}, {2, 2, 0, 2.5f, 0.22f}, {3, 2, 0, 3.5f, 0.32f}, {4, 4, 0, 8.5f, 0.73f}};
+    {1, 1, 0, 1.5f, 0.12f}, {2, 1, 0, 2.0f, 0.14f}, {2, 2, 0, 2.5f, 0.22f}, {3, 2, 0, 3.5f, 0.32f}, {4, 4, 0, 8.5f, 0.73f},
+    {0, 1, 2, 0, 0}};
 constexpr int N_FORMS = sizeof(FORMS) / sizeof(FORMS[0]);
 static_assert(N_FORMS == I8_FORMS, "the forms a context can ask for");
 
@@ -570,30 +574,46 @@ long long tiles_of(const I8Args &a, const Form &f) {
 }
 
 float estimate(const I8Args &a, const Form &f) {
-    const float cu = (float)a.cu_count, weights = (float)(groups_of(a) * a.kt) * 1024 / 5.2e6f;   // at 5.2 TB/s
+    const float cu = (float)a.cu_count, bytes = (float)(groups_of(a) * a.kt) * 1024, k = (float)a.kt;
     if (f.cw) {
-        const float rounds = ceilf((float)tiles_of(a, f) / cu);
+        const float tiles = (float)tiles_of(a, f), rounds = ceilf(tiles / cu);
         // the largest tile waits for its residuals (4096 x 12288: T44 227 us, T32 230)
         const float wait = a.residual && f.cw == 4 ? 18.0f * rounds : 0.0f;
-        return 2.0f + wait + fmaxf(rounds * (f.fixed + f.step * (float)a.kt), weights);
+        // Weights that only one tile of tokens reads come from memory at what a CU has
+        // in flight: 17.5 KB/us with three stages of the smallest tile, 25.5 with more.
+        float weights = bytes / 5.2e6f;
+        if (a.n_tokens <= 64 * f.tw)
+            weights = rounds * k * (float)f.cw * 4096 / (f.cw == 1 && rounds == 1 ? 17.5e3f : 25.5e3f);
+        return 2.0f + wait + fmaxf(rounds * (f.fixed + f.step * k), weights);
     }
-    // Two to four workgroups share a CU and its L1, which takes 17.6 ns for a KiB.
+    // Two to four workgroups share a CU and its L1, which takes 19.5 ns for a KiB.
+    // Tokens come from L2 beside the weights, each workgroup's its own: 17 TB/s
+    // (10 to 17 where the weights come from HBM, 16 to 30 from the last cache).
     const int per = a.gated ? 2 * f.r : f.r;
-    const float n = (float)((groups_of(a) + per - 1) / per) * (float)((a.n_tokens + 16 * f.tw - 1) / (16 * f.tw));
-    return fmaxf(2.5f + fmaxf(n / cu, 1.0f) * (float)a.kt * (float)(per + f.tw) * 0.0176f, 1.0f + weights);
+    const float across = (float)((groups_of(a) + per - 1) / per);
+    const float n = across * (float)((a.n_tokens + 16 * f.tw - 1) / (16 * f.tw));
+    // too little in flight: 16 x 4096 (k = 13312) S12 20 us, S11 14
+    if (f.tw == 1 && f.r == 2 && n < 0.75f * cu) return HUGE_VALF;
+    const float tokens = across * (float)a.n_tokens * k * 64;
+    const float memory = (f.r == 2 ? 1.75f : 1.0f) + bytes / 5.5e6f + tokens / 17e6f;
+    return fmaxf(2.5f + ceilf(n / cu) * k * (float)(per + f.tw) * 0.0195f, memory);
 }
 
-// The form of the least estimate.  Measured / estimated, in us, for the choice and
-// measured for the next ones (tokens x channels, k = 4096; S: stream TT, R; T: tile
-// cw, tw):
-//   1 x 12288     S11 9.3 / 10.7     S12 9.6          32 x 12288    S22 11.4 / 10.7   S21 12.1
-//   64 x 4096     S22 6.3 / 7.0      S41 8.4          96 x 4096     S42 7.9 / 9.3     T11 11.6
-//   256 x 4096    T11 12.1 / 9.3     T21 12.9         128 x 12288   T21 15.9 / 13.0   T11 16.0, T22 18
-//   256 x 12288   T22 19.5 / 18.6    T21 21.4         512 x 12288   T32 29.2 / 26.0   T22 32.5, T44 42
-//   1024 x 4096 (k = 13312)  T22 61 / 50, T32 64      1024 x 12288  T32 52.5 / 50     T44 54, T22 56
-//   1024 x 26624  T44 120 / 112      T32 145          4096 x 12288  T44 180 / 167     T22 202, T32 200
-// (Two machines' times; one runs everything some 5% faster than the other.)  Weights
-// beyond the last cache arrive later: 256 x 26624, three matrices in turn, 43 us in T22.
+// The form of the least estimate.  Measured in us, two matrices in turn (in the last
+// cache) / ten of them (from HBM), for the choice and for the next one (tokens x
+// channels, k = 4096, g: a gated pair; S: stream TT, R; T: tile cw, tw):
+//   1 x 12288     S11 9.8 / 11.3    S12 10.1 / 12.2     16 x 12288    S12 10.5 / 13.1   S11 10.1 / 13.6
+//   16 x 24000    S12 16.4 / 20.0   S11 16.8 / 24.4     32 x 12288    S22 11.8 / 15.9   T11 14.8 / 17.7
+//   64 x 12288    T11 15.1 / 17.7   S22 16.8 / 20.0     128 x 12288   T21 15.8 / 19.9   T11 15.8 / 20.6
+//   64 x 4096     S22 7.0 / 7.0     S12 8.0 / 8.1       96 x 4096     S42 8.3 / 8.4     S22 10.1 / 10.2
+//   256 x 4096    T11 12.4 / 12.5   T21 13.5 / 13.6     300 x 8192    T22 19.6 / 21.6   T21 20.3 / 25.2
+//   16 x 13312 g  T11 18.5 / 22.4   S11 19.0 / 23.0     32 x 8000 g   S21 12.6 / 16.2   T11 15.2 / 19.1
+//   32 x 13312 g  T11 18.9 / 23.0   S21 20.7 / 28.6     128 x 13312 g T22 21.6 / 27.5   T21 23.0 / 33.3
+// and with three matrices in turn:
+//   512 x 12288   T32 29.2, T22 32.5                    1024 x 4096 (k = 13312)  T22 61, T32 64
+//   1024 x 12288  T32 52.5, T44 54, T22 56              1024 x 26624  T44 120, T32 145
+//   4096 x 12288  T44 180, T32 200, T22 202
+// (Machines differ by some 5%.)
 int plan(const I8Args &a) {
     int best = -1;
     float least = 0.0f;
@@ -613,11 +633,23 @@ hipError_t launch_tile(const I8Args &a, hipStream_t s) {
     return hipGetLastError();
 }
 
+// Weights of up to four tokens are read non-temporally from 64 MiB on: four such
+// matrices fill the last cache (256 MB), so those of a model come from HBM at every
+// step.  From HBM, one token: 2 * 13312 x 4096 21.8 -> 20.3 us, 24000 x 4096 18.8 ->
+// 17.2, 8192 x 8192 15.0 -> 13.2; in a loop over one matrix, which stays in the cache,
+// 18.9 -> 20.1, 15.7 -> 16.7, 11.8 -> 12.7.  With 16 tokens it gained 6% and lost 17%.
+constexpr long long ONCE_BYTES = 64ll << 20;
+
 template <int OUT, bool GATED, int TT, int R>
 hipError_t launch_stream(const I8Args &a, hipStream_t s) {
     const long long grid = ((long long)a.rows + 16 * R - 1) / (16 * R) * ((a.n_tokens + 16 * TT - 1) / (16 * TT));
     if (grid > 0x7fffffff) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_i8_stream<OUT, GATED, TT, R>), dim3((unsigned)grid), dim3(64 * ST_WAVES), 0, s, a);
+    if constexpr (TT == 1)
+        if (a.n_tokens <= 4 && groups_of(a) * a.kt * 1024 >= ONCE_BYTES) {
+            hipLaunchKernelGGL((k_i8_stream<OUT, GATED, TT, R, true>), dim3((unsigned)grid), dim3(64 * ST_WAVES), 0, s, a);
+            return hipGetLastError();
+        }
+    hipLaunchKernelGGL((k_i8_stream<OUT, GATED, TT, R, false>), dim3((unsigned)grid), dim3(64 * ST_WAVES), 0, s, a);
     return hipGetLastError();
 }
 
@@ -637,7 +669,9 @@ hipError_t launch_form(const I8Args &a, int form, hipStream_t s) {
     if constexpr (!GATED) {
         if (form == 2) return launch_stream<OUT, GATED, 2, 2>(a, s);
         if (form == 4) return launch_stream<OUT, GATED, 4, 2>(a, s);
+        if (form == 10) return launch_stream<OUT, GATED, 1, 2>(a, s);
     }
+    if (form == 10) return launch_stream<OUT, GATED, 1, 1>(a, s);
     return launch_form<OUT, GATED>(a, form - 1, s);   // a forced form of two groups: a pair has them already
 }
 

@@ -257,7 +257,7 @@ struct I8Args {
     int32_t cu_count;
     int32_t form;            // 0: the rule's; else the form's number (LBH_TUNE_I8_FORM)
 };
-constexpr int I8_FORMS = 10;
+constexpr int I8_FORMS = 11;
 
 // Batch selection: top-k of each token's finished logits (select_route).
 struct RouteBatchArgs {

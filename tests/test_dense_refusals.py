@@ -163,8 +163,8 @@ def test_matrix_refusals(ctx):
 def test_the_form_knob_s_range(ctx):
     fn = lbhip.lib().lbh_ctx_set_tuning
     be = lbhip.HipBackend
-    assert [fn(ctx, be.TUNE_I8_FORM, v) for v in (-1, 11)] == [25, 25]
-    assert [fn(ctx, be.TUNE_I8_FORM, v) for v in (1, 10, 0)] == [0, 0, 0]
+    assert [fn(ctx, be.TUNE_I8_FORM, v) for v in (-1, 12)] == [25, 25]
+    assert [fn(ctx, be.TUNE_I8_FORM, v) for v in (1, 11, 0)] == [0, 0, 0]
 
 
 def test_tensors_of_another_device():

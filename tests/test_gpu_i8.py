@@ -303,7 +303,7 @@ def test_strided_device_weights_are_copied_in_the_backend_s_stream(be):
     other.close()
 
 
-@pytest.mark.parametrize("form", range(1, 11))
+@pytest.mark.parametrize("form", range(1, 12))
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
 def test_every_form_gives_the_same_bits(be, form, gated, ty):
@@ -349,7 +349,42 @@ def test_every_form_gives_the_same_bits(be, form, gated, ty):
         m.close()
 
 
-@pytest.mark.parametrize("form", [0, 1, 4, 6, 8, 9, 10])
+@pytest.mark.parametrize("tokens", [1, 3, 4, 5, 16])
+@pytest.mark.parametrize("gated", [False, True])
+def test_large_matrices(be, tokens, gated):
+    """Matrices from 64 MiB on, which few tokens read past the caches: the same bits as in the smallest tiles."""
+    rows, k = (16500, 2060) if gated else (16500, 4112)
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    w, v = (torch.randint(-128, 128, (rows, k), dtype=torch.int8, device="cuda", generator=g) for _ in range(2))
+    ws = torch.rand(rows, device="cuda", generator=g) / 1e5
+    q = torch.randint(-128, 128, (tokens, k), dtype=torch.int8, device="cuda", generator=g)
+    s = torch.rand(tokens, device="cuda", generator=g) + 0.5
+    m = be.upload_i8_gated(w, ws, v, ws) if gated else be.upload_i8(w, ws)
+    assert m.device_bytes > 64 << 20
+    space = torch.zeros(be.gemm_i8_workspace_bytes(m, tokens), dtype=torch.uint8, device="cuda")
+    outs = []
+    for form in (0, 1, 11, 6):
+        outs.append(torch.zeros(tokens, rows, device="cuda"))
+        be.set_tuning(be.TUNE_I8_FORM, form)
+        try:
+            (be.gemm_i8_swiglu if gated else be.gemm_i8)(m, q, s, outs[-1], space)
+        finally:
+            be.set_tuning(be.TUNE_I8_FORM, 0)
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    c = torch.randint(0, rows, (50,), generator=torch.Generator().manual_seed(1)).numpy()
+    q, s, w, v, ws = (t.cpu().numpy() for t in (q, s, w, v, ws))
+    g, u = value(q, s, w[c], ws[c]), value(q, s, v[c], ws[c])
+    got = outs[0][:, torch.from_numpy(c).cuda()]
+    if gated:
+        with np.errstate(over="ignore"):
+            want = g / (1 + np.exp(-g)) * u
+        check(got, want, torch.float32, gated_off(g, u, want))
+    else:
+        check(got, g, torch.float32, plain_off(g))
+    m.close()
+
+
+@pytest.mark.parametrize("form", [0, 1, 4, 6, 8, 9, 10, 11])
 def test_rows_far_apart(be, form):
     """Strides that take the last rows beyond 32 bits: x rows 2^23 bytes apart (2.5 GB), y rows 2^24 elements (10 GB)."""
     tokens, rows, k = 300, 64, 64
