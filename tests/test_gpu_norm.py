@@ -243,6 +243,24 @@ def test_weight_that_is_not_finite(be):
     assert bool(torch.isnan(s).all()) and not bool(q.any())
 
 
+@pytest.mark.parametrize("n", [512, 4352, 16384])
+def test_norm_q8_k_of_rows_that_are_zero_or_not_finite(be, n):
+    """Each row's blocks are what the row quantizer makes of its float32 values, whatever they are."""
+    x, _, w = inputs(6, n, torch.float32, n, delta=False)
+    x[0] = 0.0
+    x[1, 3] = float("nan")
+    x[2, n - 1] = float("inf")
+    x[3, 256:512] = 0.0
+    x[4, :256] = 5.0
+    y = torch.zeros(6, n, device="cuda")
+    enc, want = (torch.full((6, n // 256 * 292), 9, dtype=torch.uint8, device="cuda") for _ in range(2))
+    be.rms_norm_q8_k_rows(x.cuda(), w.cuda(), EPS, enc, y=y)
+    be.quantize_q8_k_rows(y, want, 6, n)
+    assert torch.equal(enc, want)
+    _, v = oracle_norm(x, None, w, EPS)
+    near(y[torch.tensor([0, 3, 4, 5])], v[[0, 3, 4, 5]], torch.float32)
+
+
 @pytest.mark.parametrize("n", [512, 4096, 4097, 30000])
 @pytest.mark.parametrize("into", ["hidden", "delta"])
 def test_in_place(be, n, into):
