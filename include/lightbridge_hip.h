@@ -629,8 +629,8 @@ lbh_status lbh_moe_forward_leased(lbh_ctx *ctx, lbh_moe *moe, const lbh_expert_l
  * Row operands are float32, binary16 or bfloat16 (LBH_F32, LBH_F16, LBH_BF16);
  * strides count elements, are at least the row's length, and bytes between the
  * rows are neither read for their value nor written.  Pointers need the alignment
- * of their element; rows whose address and stride are multiples of 16 bytes are
- * the fast ones.  Outputs may share no byte with each other or with an input,
+ * of their element; rows of a multiple of 8 elements, and products' rows whose
+ * address and stride are multiples of 16 bytes, are the fast ones.  Outputs may share no byte with each other or with an input,
  * except where "in place" is said.  rows / n_tokens == 0 does nothing.  At most
  * 2^20 rows a call. */
 #define LBH_F16 1
@@ -641,8 +641,10 @@ lbh_status lbh_moe_forward_leased(lbh_ctx *ctx, lbh_moe *moe, const lbh_expert_l
  *   v = h * weight / sqrt(mean(h^2) + eps)
  * hidden_out (optional) receives h; it may be hidden or delta themselves, in
  * place.  y receives v in y_type.  Sums and products are in 64 bits, and v is
- * rounded to float32 and from there to y_type: results do not depend on the
- * launch shape.  eps > 0.  n up to 2^23. */
+ * rounded to float32 and from there to y_type.  A row gets the same bits among any
+ * number of rows, at any addresses and strides; the Q8_K form adds rows of up to
+ * 512 elements in another order than the others, which may move a float32 value
+ * next to a rounding border by one step.  eps > 0.  n up to 2^23. */
 lbh_status lbh_rms_norm_rows(lbh_ctx *ctx, int32_t type, const void *hidden_dev, size_t hidden_stride,
                              const void *delta_dev, size_t delta_stride, const float *weight_dev, double eps,
                              size_t rows, size_t n, void *hidden_out_dev, size_t hidden_out_stride, int32_t y_type,

@@ -10,10 +10,10 @@
 //
 // Everything between the loads and the roundings is in 64 bits: the product
 // of two 32-bit values is exact there, and the sum's order moves r by some
-// 1e-16 only, so an 8-bit value does not depend on how a row is split over
-// lanes (in 32 bits one value in ten thousand falls on the other side of a
-// rounding border when the order of the sum changes).  The 64-bit rate of a CU
-// equals its 32-bit rate, and the kernel stays bound by memory.
+// 1e-16 only (in 32 bits one 8-bit value in ten thousand falls on the other side
+// of a rounding border when the order changes).  What order is left hangs on n
+// alone.  The 64-bit rate of a CU equals its 32-bit rate, and the kernel stays
+// bound by memory.
 //
 // max|v| = r * max|h * weight|, so the sum and the maximum come from one pass
 // over the row, which stays in registers for the second one.
@@ -82,13 +82,15 @@ __device__ __forceinline__ int nearest_of_quotient(double x, double inv) {
     return (int)(uint32_t)__builtin_bit_cast(uint64_t, __builtin_fma(x, inv, 0x1.8p22) + (0x1.8p52 - 0x1.8p22));
 }
 
-// Eight consecutive elements at an address of 16 bytes.
+// Eight consecutive elements in memory at any address of their type, as words of 16
+// bytes (global memory takes a word at any address).
 template <int TY>
 __device__ __forceinline__ void load8(const row_t<TY> *p, float (&v)[8]) {
     constexpr int N = 16 / (int)sizeof(row_t<TY>);
 #pragma unroll
     for (int i = 0; i < 8; i += N) {
-        const rvec<row_t<TY>, N> a = *reinterpret_cast<const rvec<row_t<TY>, N> *>(p + i);
+        rvec<row_t<TY>, N> a;
+        __builtin_memcpy(&a, p + i, sizeof a);
 #pragma unroll
         for (int j = 0; j < N; ++j) v[i + j] = (float)a[j];
     }
@@ -101,17 +103,20 @@ __device__ __forceinline__ void store8(row_t<TY> *p, const float (&v)[8]) {
         rvec<row_t<TY>, N> a;
 #pragma unroll
         for (int j = 0; j < N; ++j) a[j] = (row_t<TY>)v[i + j];
-        *reinterpret_cast<rvec<row_t<TY>, N> *>(p + i) = a;
+        __builtin_memcpy(p + i, &a, sizeof a);
     }
 }
 
 // One row by TPR threads, 8 * NV of its products h * weight in each thread's
 // registers; longer rows are read a second time beyond those.  VEC: a thread's
-// eight elements of a step are consecutive and moved as 16-byte words (every row of
-// every operand aligned for it, n a multiple of 8); otherwise they lie TPR apart,
-// one element a lane, at any alignment and length.  (Words at any alignment with a
-// scalar tail, in one form for both, put every load behind a branch of its own:
-// 6007 x 4096 bf16 took 52 us instead of 38, and 333 x 7167 no less than this.)
+// eight elements of a step are consecutive and moved as 16-byte words (n a multiple
+// of 8); otherwise they lie TPR apart, one element a lane.  The choice hangs on n
+// alone: the order of a row's sum moves r by 1e-16, and with it one float32 value in
+// some 10^8 over a rounding border, so operands at other addresses and strides get
+// the same form and the same bits.  (6007 x 4096 bf16 with the residual to int8 at odd
+// addresses: 42 us in words, 129 in single elements.  Words with a scalar tail, in one form for both,
+// put every load behind a branch of its own: 6007 x 4096 bf16 took 52 us instead of
+// 38, and 333 x 7167 no less than this.)
 template <int TY, int TPR, int NV, bool VEC, bool NORM>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_rows(NormArgs p) {
     using T = row_t<TY>;
@@ -258,7 +263,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_rows(NormArgs p)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     q[j >> 2] |= (uint32_t)(int8_of(hw[j]) & 0xff) << (8 * (j & 3));
-                *reinterpret_cast<uint2 *>(p.q + rr * p.q_stride + e) = blank ? make_uint2(0, 0) : make_uint2(q[0], q[1]);
+                const uint2 word = blank ? make_uint2(0, 0) : make_uint2(q[0], q[1]);
+                __builtin_memcpy(p.q + rr * p.q_stride + e, &word, sizeof word);
             }
             if (p.y || p.q8k) {
                 float v[8];
@@ -272,7 +278,10 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_rows(NormArgs p)
                     store8<T_BF16>(static_cast<__bf16 *>(p.y) + rr * p.y_stride + e, v);
                 if constexpr (TPR > 64) {
                     extern __shared__ __align__(16) float s_v[];
-                    if (p.q8k) store8<T_F32>(s_v + e, v);
+                    if (p.q8k) {
+                        *reinterpret_cast<float4 *>(s_v + e) = make_float4(v[0], v[1], v[2], v[3]);
+                        *reinterpret_cast<float4 *>(s_v + e + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                    }
                 }
             }
         } else {
@@ -349,20 +358,12 @@ hipError_t launch_norm_typed(const NormArgs &a, bool vec, hipStream_t s) {
     return vec ? launch_norm_form<TY, true, false>(a, s) : launch_norm_form<TY, false, false>(a, s);
 }
 
-bool aligned_rows(const void *p, long long stride, int elem, int bytes) {
-    return !p || ((reinterpret_cast<uintptr_t>(p) % bytes) == 0 && (stride * elem) % bytes == 0);
-}
-
 }  // namespace
 
 hipError_t launch_norm_rows(const NormArgs &a, hipStream_t s) {
     if (a.rows <= 0) return hipSuccess;
     if (a.n < 1 || a.rows > 0x7fffffff) return hipErrorInvalidValue;
-    const int e = row_elem_bytes(a.type);
-    const bool vec = a.n % 8 == 0 && aligned_rows(a.hidden, a.hidden_stride, e, 16) &&
-                     aligned_rows(a.delta, a.delta_stride, e, 16) &&
-                     aligned_rows(a.hidden_out, a.hidden_out_stride, e, 16) && aligned_rows(a.weight, 0, 4, 16) &&
-                     aligned_rows(a.y, a.y_stride, row_elem_bytes(a.y_type), 16) && aligned_rows(a.q, a.q_stride, 1, 8);
+    const bool vec = a.n % 8 == 0;
     switch (a.type) {
     case T_F32: return launch_norm_typed<T_F32>(a, vec, s);
     case T_F16: return launch_norm_typed<T_F16>(a, vec, s);

@@ -311,3 +311,59 @@ def test_rows_far_apart(be):
     q_want, s_want = oracle_i8(v)
     np.testing.assert_array_equal(s.cpu().numpy(), s_want)
     np.testing.assert_array_equal(q.cpu().numpy(), q_want)
+
+
+def placements(be, hidden, delta, weight, y_ty):
+    """hidden_out, y, int8 rows, their scales and (for widths that have them) Q8_K blocks of the same rows, at aligned
+    addresses and strides and at odd ones."""
+    rows, n = hidden.shape
+    w_at = torch.empty(n + 1, device="cuda")
+    outs = []
+    for pad, offset in ((0, 0), (3, 1), (8, 5)):
+        _, hd = strided(hidden, pad, offset)
+        _, dd = strided(delta, pad, offset)
+        w = w_at[offset & 1:][:n]
+        w.copy_(weight)
+        _, out = strided(torch.zeros_like(hidden), pad, offset)
+        _, y = strided(torch.zeros(rows, n, dtype=y_ty), pad, offset)
+        _, q = strided(torch.zeros(rows, n, dtype=torch.int8), pad, offset)
+        s = torch.zeros(rows, device="cuda")
+        be.rms_norm_i8_rows(hd, w, EPS, q, s, y=y, delta=dd, hidden_out=out)
+        got = [out, y, q, s]
+        if n % 256 == 0 and n <= 16384:
+            enc = torch.zeros(rows, n // 256 * 292, dtype=torch.uint8, device="cuda")
+            be.rms_norm_q8_k_rows(hd, w, EPS, enc, delta=dd)
+            got.append(enc)
+        outs.append([t.clone() for t in got])
+    return outs
+
+
+@pytest.mark.parametrize("ty,y_ty", [("f32", "f32"), ("f16", "bf16"), ("bf16", "f32"), ("f32", "f16")])
+@pytest.mark.parametrize("rows,n", [(70, 8), (66, 255), (65, 512), (40, 1024), (31, 4096), (9, 8192), (5, 16384), (3, 33000)])
+def test_bits_do_not_depend_on_the_placement(be, rows, n, ty, y_ty):
+    hidden, delta, weight = inputs(rows, n, TYPES[ty], seed=n + 5)
+    first, *others = placements(be, hidden, delta, weight, TYPES[y_ty])
+    for other in others:
+        assert all(torch.equal(a, b) for a, b in zip(first, other))
+
+
+def test_sums_that_depend_on_their_order(be):
+    """One value whose square is 1 among four million whose squares are just below half of that one's last bit in 64 bits: those
+    that its lane adds to it one by one are lost, so r shows which elements a lane has.  With the elements of words of
+    eight that share the large value's lane at zero, another assignment of elements to lanes moves r by 2^-43, which
+    takes some 30 of these 16 million values over a rounding border of float32."""
+    n, rows = 1 << 22, 4
+    g = torch.Generator().manual_seed(1)
+    x = 2.0 ** -27 * (1 + 0.35 * torch.rand(rows, n, generator=g))
+    x.view(rows, n // 8192, 1024, 8)[:, :, 0] = 0.0
+    x[:, 0] = 1.0
+    weight = 1.0 + torch.rand(n, generator=g)
+    outs = []
+    for pad, offset in ((0, 0), (3, 1)):
+        _, xd = strided(x, pad, offset)
+        _, y = strided(torch.zeros(rows, n), pad, offset)
+        be.rms_norm_rows(xd, weight.cuda(), 1e-30, y)
+        outs.append(y.clone())
+    assert torch.equal(outs[0], outs[1])
+    _, v = oracle_norm(x, None, weight, 1e-30)
+    near(outs[0], v, torch.float32)
