@@ -685,7 +685,8 @@ lbh_status lbh_i8_matrix_create_gated(lbh_ctx *ctx, size_t rows, size_t k, const
 /* [sync] The int8 form of an uploaded matrix (Q4_K, Q5_K, IQ2_S, IQ3_S or F32), each
  * row's decoded values quantized as by lbh_quantize_i8_rows; with `up`, the gated
  * pair of m (the gate) and up, of one shape.  An F32 row with a value that is not
- * finite is refused as above.  The packed matrices stay as they are. */
+ * finite is refused as above.  The packed matrices stay as they are.  While it runs, the
+ * call holds rows * (k + 4) bytes and 64 MiB beside the result. */
 lbh_status lbh_i8_matrix_from_packed(lbh_ctx *ctx, const lbh_matrix *m, const lbh_matrix *up, lbh_i8_matrix **out,
                                      lbh_error *err);
 lbh_status lbh_i8_matrix_destroy(lbh_i8_matrix *m);

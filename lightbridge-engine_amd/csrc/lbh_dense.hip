@@ -371,12 +371,12 @@ lbh_status lbh_i8_matrix_from_packed(lbh_ctx *ctx, const lbh_matrix *m, const lb
     st = alloc_i8(ctx, rows, k, parts == 2, &q, err);
     if (st) return st;
     auto fill = [&]() -> lbh_status {
-        // Rows decoded some 64 MiB at a time, quantized, then laid out together.
+        // Rows decoded 64 MiB at a time (2^16 rows at most: k is 256 or more), quantized, then laid
+        // out together.
         for (int i = 0; i < parts; ++i) {
             const lbh_matrix *s = src[i];
-            const bool f32 = s->type == LBH_F32;
             size_t chunk = ((size_t)64 << 20) / (k * sizeof(float));
-            chunk = f32 || chunk > rows ? rows : chunk < 1 ? 1 : chunk;
+            chunk = chunk > rows ? rows : chunk;
             Temp values, codes, scales;
             HIP_TRY(values.get(chunk * k * sizeof(float)));
             HIP_TRY(codes.get(rows * k));
@@ -386,19 +386,16 @@ lbh_status lbh_i8_matrix_from_packed(lbh_ctx *ctx, const lbh_matrix *m, const lb
             for (size_t r0 = 0; r0 < rows; r0 += chunk) {
                 const size_t n = rows - r0 < chunk ? rows - r0 : chunk;
                 float *f = static_cast<float *>(values.p);
-                if (f32)
-                    HIP_TRY(launch_f32_layout(reinterpret_cast<const float *>(s->planes), f, (long long)rows,
-                                              (long long)k, 0, ctx->stream));
+                if (s->type == LBH_F32)
+                    HIP_TRY(launch_f32_rows(reinterpret_cast<const float *>(s->planes), (long long)rows, (long long)k,
+                                            (long long)r0, (long long)n, f, ctx->stream));
                 else
                     HIP_TRY(launch_dequant_rows(v, (long long)r0, (long long)n, f, ctx->stream));
-                for (size_t r = 0; r < n; r += MAX_TOKENS) {   // one launch's rows at a time
-                    NormArgs a{};
-                    a.hidden = f + r * k, a.hidden_stride = (long long)k, a.type = T_F32;
-                    a.q = static_cast<int8_t *>(codes.p) + (r0 + r) * k, a.q_stride = (long long)k;
-                    a.scale = static_cast<float *>(scales.p) + r0 + r;
-                    a.rows = (long long)(n - r < MAX_TOKENS ? n - r : MAX_TOKENS), a.n = (int32_t)k;
-                    HIP_TRY(launch_norm_rows(a, ctx->stream));
-                }
+                NormArgs a{};
+                a.hidden = f, a.hidden_stride = (long long)k, a.type = T_F32;
+                a.q = static_cast<int8_t *>(codes.p) + r0 * k, a.q_stride = (long long)k;
+                a.scale = static_cast<float *>(scales.p) + r0, a.rows = (long long)n, a.n = (int32_t)k;
+                HIP_TRY(launch_norm_rows(a, ctx->stream));
             }
             const float *sc = static_cast<const float *>(scales.p);
             const lbh_status s2 = check_i8_scales(ctx, sc, rows, (uint32_t)i, err);

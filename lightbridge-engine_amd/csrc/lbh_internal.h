@@ -313,6 +313,8 @@ hipError_t launch_f32_chains(const RouterArgs &a, hipStream_t s);
 // (w[(j * rows + r) * 4 + c] = row r, input 4j + c); to_device selects the
 // direction.  k % 4 == 0.
 hipError_t launch_f32_layout(const float *src, float *dst, long long rows, long long k, int to_device, hipStream_t s);
+hipError_t launch_f32_rows(const float *planes, long long rows, long long k, long long r0, long long n, float *out,
+                           hipStream_t s);
 // First non-finite weight of an F32 matrix in the router layout, as the
 // row-major index r * k + i (atomicMin into *first).
 hipError_t launch_find_nonfinite_f32w(const float *w, long long rows, long long k, unsigned long long *first,

@@ -39,6 +39,18 @@ __global__ void k_f32_layout(const float *__restrict__ src, float *__restrict__ 
     }
 }
 
+// Rows r0 .. r0 + n - 1 of a laid-out matrix, row-major.
+__global__ void k_f32_rows(const float *__restrict__ src, float *__restrict__ dst, long long rows, long long k,
+                           long long r0, long long n) {
+    const long long total = n * (k / 4);
+    for (long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x; t < total;
+         t += (long long)gridDim.x * blockDim.x) {
+        const long long j = t / n, r = t - j * n;
+        *reinterpret_cast<float4 *>(dst + r * k + 4 * j) =
+            *reinterpret_cast<const float4 *>(src + (j * rows + r0 + r) * 4);
+    }
+}
+
 __global__ void k_find_nonfinite_f32w(const float *__restrict__ w, long long rows, long long k,
                                       unsigned long long *first) {
     const long long n = rows * k;
@@ -318,6 +330,15 @@ hipError_t launch_f32_layout(const float *src, float *dst, long long rows, long 
     long long grid = (rows * (k / 4) + 255) / 256;
     grid = grid > 65536 ? 65536 : grid;
     hipLaunchKernelGGL(k_f32_layout, dim3((int)grid), dim3(256), 0, s, src, dst, rows, k, to_device);
+    return hipGetLastError();
+}
+
+hipError_t launch_f32_rows(const float *planes, long long rows, long long k, long long r0, long long n, float *out,
+                           hipStream_t s) {
+    if (n <= 0 || r0 < 0 || r0 + n > rows || k <= 0 || k % 4) return hipErrorInvalidValue;
+    long long grid = (n * (k / 4) + 255) / 256;
+    grid = grid > 65536 ? 65536 : grid;
+    hipLaunchKernelGGL(k_f32_rows, dim3((int)grid), dim3(256), 0, s, planes, out, rows, k, r0, n);
     return hipGetLastError();
 }
 

@@ -400,3 +400,45 @@ def test_rows_far_apart(be, form):
         be.set_tuning(be.TUNE_I8_FORM, 0)
     want = value(q, s, w, ws)
     check(y, want, torch.bfloat16, plain_off(want))
+
+
+def test_from_packed_f32_in_pieces(be):
+    """A matrix of 1 GiB with more rows than one launch takes: exact, and beside the result and its codes only a piece of
+    the decoded values is held (the free memory is read all the while)."""
+    import threading
+
+    import lbhip
+    rows, k = (1 << 20) + 37, 256
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn(rows, k, device="cuda", generator=g)
+    scale = (x.abs().amax(1).double() / 127).float()
+    want = torch.empty(rows, k, dtype=torch.int8, device="cuda")
+    for at in range(0, rows, 1 << 17):
+        part = slice(at, at + (1 << 17))
+        want[part] = torch.round(x[part].double() / scale[part].double()[:, None]).to(torch.int8)
+    want, scale, host = want.cpu().numpy(), scale.cpu().numpy(), x.cpu().numpy()
+    m = be.upload(lbhip.F32, rows, k, host)
+    del x, host
+    torch.cuda.empty_cache()
+    torch.cuda.synchronize()
+    before, least, done = torch.cuda.mem_get_info()[0], [1 << 62], threading.Event()
+
+    def watch():
+        while not done.is_set():
+            least[0] = min(least[0], torch.cuda.mem_get_info()[0])
+
+    thread = threading.Thread(target=watch)
+    thread.start()
+    try:
+        m8 = be.i8_from_packed(m)
+    finally:
+        done.set()
+        thread.join()
+    least[0] = min(least[0], torch.cuda.mem_get_info()[0])
+    q, s = m8.read()
+    assert np.array_equal(s, scale) and np.array_equal(q, want)
+    held = before - least[0]
+    assert held >= m8.device_bytes
+    # the result, the codes, the scales, a piece of 64 MiB, and room for the allocator's own granularity
+    assert held <= m8.device_bytes + rows * (k + 4) + (64 << 20) + (64 << 20), held >> 20
+    m8.close(), m.close()
