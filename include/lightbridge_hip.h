@@ -714,8 +714,8 @@ lbh_status lbh_gemm_i8(lbh_ctx *ctx, const lbh_i8_matrix *m, const int8_t *x_dev
                        const void *residual_dev, size_t residual_stride, void *workspace_dev, size_t workspace_len,
                        lbh_error *err);
 /* [async] The gated pair's SwiGLU: h[t][c] = g / (1 + exp(-g)) * u with g and u the
- * products above of the gate and the up, in float32, rounded to h_type once.  Where
- * the factor of u is below 2^-118 (g < -87) it is 0. */
+ * products above of the gate and the up, in float32, rounded to h_type once.  From
+ * g = -126 ln 2 (-87.34) down, where the factor of u is below 2^-119, it is 0. */
 lbh_status lbh_gemm_i8_swiglu(lbh_ctx *ctx, const lbh_i8_matrix *m, const int8_t *x_dev, size_t x_stride,
                               const float *x_scales_dev, size_t n_tokens, int32_t h_type, void *h_dev, size_t h_stride,
                               void *workspace_dev, size_t workspace_len, lbh_error *err);

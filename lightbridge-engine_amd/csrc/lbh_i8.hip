@@ -143,10 +143,10 @@ __device__ __forceinline__ float rounded(float v) {
 }
 
 // g / (1 + exp(-g)) * u.  exp(-g) = 2^z with z = -g log2(e) to some 40 bits (hi +
-// lo), so the argument's rounding does not grow with |g|; below g = -88 the exponent
-// stays there, where the reciprocal of 1 + e lies below the least normal float and is
-// 0 (what is right is below 2^-118 |u|), as above g = 104 (1 + e is 1), which also keeps
-// infinities out of it; and 1 / d is the reciprocal with one
+// lo), so the argument's rounding does not grow with |g|; from g = -126 ln 2 = -87.34
+// down the reciprocal of 1 + e lies below the least normal float and is 0 (what is right
+// is below 2^-119 |u|), so the exponent stays at g = -88, and above g = 104 (1 + e is 1),
+// which also keeps infinities out of it; and 1 / d is the reciprocal with one
 // Newton step.  The library's exp and division cost twice
 // as many instructions, which is what bounds the epilogue.
 __device__ __forceinline__ float swiglu(float g, float u) {

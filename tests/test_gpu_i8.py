@@ -442,3 +442,27 @@ def test_from_packed_f32_in_pieces(be):
     # the result, the codes, the scales, a piece of 64 MiB, and room for the allocator's own granularity
     assert held <= m8.device_bytes + rows * (k + 4) + (64 << 20) + (64 << 20), held >> 20
     m8.close(), m.close()
+
+
+@pytest.mark.parametrize("tokens", [1, 20, 70, 200, 300])
+def test_gated_down_to_the_least_factor(be, tokens):
+    """Gates from -80 to -95 in steps of 0.05 next to ups of 1e36, which bring the factors into sight: good to its roundings
+    above -126 ln 2 = -87.34, where the factor is 2^-119.6, and 0 from there on (g itself is off by 2e-5)."""
+    rows, k = 300, 16
+    q, w, v = np.zeros((tokens, k), np.int8), np.zeros((rows, k), np.int8), np.zeros((rows, k), np.int8)
+    q[:, 0], q[:, 1], q[:, 2] = 100, 1, 100
+    total = -8000 - 5 * np.arange(rows)
+    w[:, 0], w[:, 1], v[:, 2] = -(-total // 100), -(-total % 100), 100
+    s, ws, vs = np.ones(tokens, np.float32), np.full(rows, 0.01, np.float32), np.full(rows, 1e32, np.float32)
+    g, u = value(q, s, w, ws), value(q, s, v, vs)
+    assert g.max() > -80.01 and g.min() < -94.9
+    want = g / (1 + np.exp(-g)) * u
+    m = be.upload_i8_gated(w, ws, v, vs)
+    h = torch.zeros(tokens, rows, device="cuda")
+    be.gemm_i8_swiglu(m, on_gpu(q), torch.from_numpy(s).cuda(), h)
+    got, border = h.double().cpu().numpy(), -126 * np.log(2)
+    seen, gone = g > border + 1e-3, g < border - 1e-3
+    limit = np.abs(want) * (3 * (1 + np.abs(g)) + 8) * 1.01 * U
+    assert seen.any() and (np.abs(got - want) <= limit)[seen].all()
+    assert gone.any() and (got[gone] == 0).all()
+    assert (np.abs(want[gone]) < 2.0 ** -119 * u[gone]).all()
