@@ -466,3 +466,123 @@ def test_gated_down_to_the_least_factor(be, tokens):
     assert seen.any() and (np.abs(got - want) <= limit)[seen].all()
     assert gone.any() and (got[gone] == 0).all()
     assert (np.abs(want[gone]) < 2.0 ** -119 * u[gone]).all()
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 4])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
+def test_large_matrices_in_every_type(be, tokens, gated, ty):
+    """What few tokens read past the caches, in each output type: with the residual apart and in place, rows of y apart,
+    and the bytes around them left alone."""
+    t = TYPES[ty]
+    rows, k = (16500, 2064) if gated else (16500, 4112)
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    w, v = (torch.randint(-128, 128, (rows, k), dtype=torch.int8, device="cuda", generator=g) for _ in range(2))
+    ws = (torch.rand(rows, device="cuda", generator=g) + 0.5) / (5000 * k ** 0.5)
+    q = torch.randint(-128, 128, (tokens, k), dtype=torch.int8, device="cuda", generator=g)
+    s = torch.rand(tokens, device="cuda", generator=g) + 0.5
+    m = be.upload_i8_gated(w, ws, v, ws) if gated else be.upload_i8(w, ws)
+    assert m.device_bytes > 64 << 20
+    res = torch.randn(tokens, rows, device="cuda", generator=g).to(t)
+
+    def call(form, pad, residual):
+        buf = torch.full((tokens + 1, rows + pad), 5.0, dtype=t, device="cuda")
+        y = buf[:tokens, :rows]
+        be.set_tuning(be.TUNE_I8_FORM, form)
+        try:
+            if gated:
+                be.gemm_i8_swiglu(m, q, s, y)
+            else:
+                if residual == "place":
+                    y.copy_(res)
+                be.gemm_i8(m, q, s, y, residual={None: None, "apart": res, "place": y}[residual])
+        finally:
+            be.set_tuning(be.TUNE_I8_FORM, 0)
+        assert bool((buf[tokens:] == 5).all()) and bool((buf[:, rows:] == 5).all())
+        return y.clone()
+
+    plain = call(6, 0, None)
+    added = None if gated else call(6, 0, "apart")
+    for form in (0, 1, 11):
+        for pad in (0, 4, 3):
+            assert torch.equal(call(form, pad, None), plain)
+            if not gated:
+                assert torch.equal(call(form, pad, "apart"), added) and torch.equal(call(form, pad, "place"), added)
+    c = np.random.default_rng(1).integers(0, rows, 60)
+    at = torch.from_numpy(c).cuda()
+    res, q, s, w, v, ws = (a.cpu() for a in (res[:, at], q, s, w[at], v[at], ws[at]))
+    q, s, w, v, ws = (a.numpy() for a in (q, s, w, v, ws))
+    a, u = value(q, s, w, ws), value(q, s, v, ws)
+    if gated:
+        want = a / (1 + np.exp(-a)) * u
+        check(plain[:, at], want, t, gated_off(a, u, want))
+    else:
+        check(plain[:, at], a, t, plain_off(a))
+        total = a + res.double().numpy()
+        check(added[:, at], total, t, plain_off(a) + (np.abs(total) + plain_off(a)) * U)
+    m.close()
+
+
+@pytest.mark.parametrize("form,cw,tw", [(6, 1, 1), (7, 2, 1), (8, 2, 2), (9, 3, 2), (10, 4, 4)])
+@pytest.mark.parametrize("kind", ["plain", "residual", "gated"])
+def test_grids_of_many_tiles(be, form, cw, tw, kind):
+    """Each tile form over 18 token tiles (two whole panels of eight and a narrow one) and six channel tiles, the last of
+    both ragged: 108 tiles, which do not divide evenly among eight XCDs; and over 17 x 5 = 85 whole ones."""
+    gated = kind == "gated"
+    ch, k = 64 * cw // (2 if gated else 1), 272
+    for tokens, rows in ((17 * 64 * tw + 3, 5 * ch + 9), (17 * 64 * tw, 5 * ch)):
+        g = torch.Generator(device="cuda").manual_seed(form + tokens)
+        w, v = (torch.randint(-128, 128, (rows, k), dtype=torch.int8, device="cuda", generator=g) for _ in range(2))
+        q = torch.randint(-128, 128, (tokens, k), dtype=torch.int8, device="cuda", generator=g)
+        ws, s = torch.rand(rows, device="cuda", generator=g) / 9e4, torch.rand(tokens, device="cuda", generator=g) + 0.5
+        res = torch.randn(tokens, rows, device="cuda", generator=g).bfloat16() if kind == "residual" else None
+        m = be.upload_i8_gated(w, ws, v, ws) if gated else be.upload_i8(w, ws)
+        outs = []
+        for f in (form, 1):
+            buf = torch.full((tokens + 2, rows + 8), 5.0, dtype=torch.bfloat16, device="cuda")
+            y = buf[:tokens, :rows]
+            be.set_tuning(be.TUNE_I8_FORM, f)
+            try:
+                if gated:
+                    be.gemm_i8_swiglu(m, q, s, y)
+                else:
+                    be.gemm_i8(m, q, s, y, residual=res)
+            finally:
+                be.set_tuning(be.TUNE_I8_FORM, 0)
+            assert bool((buf[tokens:] == 5).all()) and bool((buf[:, rows:] == 5).all())
+            outs.append(y.clone())
+        assert torch.equal(outs[0], outs[1])
+        q, s, w, v, ws = (a.cpu().numpy() for a in (q, s, w, v, ws))
+        a = value(q, s, w, ws)
+        if gated:
+            u = value(q, s, v, ws)
+            want = a / (1 + np.exp(-a)) * u
+            check(outs[0], want, torch.bfloat16, gated_off(a, u, want))
+        else:
+            want = a if res is None else a + res.double().cpu().numpy()
+            check(outs[0], want, torch.bfloat16, plain_off(a) + (np.abs(want) + plain_off(a)) * U)
+        m.close()
+
+
+@pytest.mark.parametrize("rows,k", [(5, 1), (40, 255), (17, 256), (64, 257), (16, 1000)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_workspace_sizes(be, rows, k, gated):
+    """Rows are padded to 256 bytes; one byte less than the stated size is refused, the size itself is enough."""
+    import lbhip
+    tokens = 9
+    q, s, w, ws = make(tokens, rows, k, 4)
+    m = be.upload_i8_gated(w, ws, w, ws) if gated else be.upload_i8(w, ws)
+    need = be.gemm_i8_workspace_bytes(m, tokens)
+    assert need == tokens * (-(-k // 256) * 256)
+    assert m.device_bytes == (2 if gated else 1) * -(-rows // 16) * (16 * (-(-k // 256) * 256) + 64)
+    x, sd, y = on_gpu(q, 3, 1), torch.from_numpy(s).cuda(), torch.zeros(tokens, rows, device="cuda")
+    call = be.gemm_i8_swiglu if gated else be.gemm_i8
+    buf = torch.full((need + 64,), 3, dtype=torch.uint8, device="cuda")
+    with pytest.raises(lbhip.KernelError) as e:
+        call(m, x, sd, y, buf[:need - 1])
+    assert e.value.variant == "ScratchTooSmall"
+    call(m, x, sd, y, buf[:need])
+    assert bool((buf[need:] == 3).all())
+    g = value(q, s, w, ws)
+    want = g / (1 + np.exp(-g)) * g if gated else g
+    check(y, want, torch.float32, gated_off(g, g, want) if gated else plain_off(g))
