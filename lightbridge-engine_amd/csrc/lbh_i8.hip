@@ -573,7 +573,17 @@ long long tiles_of(const I8Args &a, const Form &f) {
     return (groups_of(a) + 4 * f.cw - 1) / (4 * f.cw) * ((a.n_tokens + 64 * f.tw - 1) / (64 * f.tw));
 }
 
+// Workgroups of a streaming form of 16 * tt tokens and r channel groups (or pairs).
+long long streams_of(const I8Args &a, int tt, int r) {
+    return ((long long)a.rows + 16 * r - 1) / (16 * r) * ((a.n_tokens + 16 * tt - 1) / (16 * tt));
+}
+
+// A launch counts its threads in 32 bits.
+bool fits_a_launch(long long workgroups, int threads) { return workgroups * threads < 1ll << 32; }
+
 float estimate(const I8Args &a, const Form &f) {
+    if (!(f.cw ? fits_a_launch(tiles_of(a, f), 256) : fits_a_launch(streams_of(a, f.tw, f.r), 64 * ST_WAVES)))
+        return HUGE_VALF;   // 2 * 2^26 channels x 23 tokens in the streaming form of 16
     const float cu = (float)a.cu_count, bytes = (float)(groups_of(a) * a.kt) * 1024, k = (float)a.kt;
     if (f.cw) {
         const float tiles = (float)tiles_of(a, f), rounds = ceilf(tiles / cu);
@@ -628,7 +638,7 @@ int plan(const I8Args &a) {
 template <int OUT, bool GATED, int CW, int TW>
 hipError_t launch_tile(const I8Args &a, hipStream_t s) {
     const long long grid = tiles_of(a, Form{CW, TW, 0, 0, 0});
-    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    if (!fits_a_launch(grid, 256)) return hipErrorInvalidValue;
     hipLaunchKernelGGL((k_i8_tile<OUT, GATED, CW, TW>), dim3((unsigned)grid), dim3(256), 0, s, a);
     return hipGetLastError();
 }
@@ -642,8 +652,8 @@ constexpr long long ONCE_BYTES = 64ll << 20;
 
 template <int OUT, bool GATED, int TT, int R>
 hipError_t launch_stream(const I8Args &a, hipStream_t s) {
-    const long long grid = ((long long)a.rows + 16 * R - 1) / (16 * R) * ((a.n_tokens + 16 * TT - 1) / (16 * TT));
-    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    const long long grid = streams_of(a, TT, R);
+    if (!fits_a_launch(grid, 64 * ST_WAVES)) return hipErrorInvalidValue;
     if constexpr (TT == 1)
         if (a.n_tokens <= 4 && groups_of(a) * a.kt * 1024 >= ONCE_BYTES) {
             hipLaunchKernelGGL((k_i8_stream<OUT, GATED, TT, R, true>), dim3((unsigned)grid), dim3(64 * ST_WAVES), 0, s, a);

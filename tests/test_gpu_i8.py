@@ -586,3 +586,37 @@ def test_workspace_sizes(be, rows, k, gated):
     g = value(q, s, w, ws)
     want = g / (1 + np.exp(-g)) * g if gated else g
     check(y, want, torch.float32, gated_off(g, g, want) if gated else plain_off(g))
+
+
+def test_the_tallest_matrix(be):
+    """2^26 channels, the most there may be, of a gated pair: a launch counts its threads in 32 bits, so 23 tokens do not fit
+    one in the streaming form of 16 tokens, which is refused where it is asked for and not chosen otherwise."""
+    import lbhip
+    rows, k, tokens = 1 << 26, 16, 23
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w, v = (torch.randint(-128, 128, (rows, k), dtype=torch.int8, device="cuda", generator=g) for _ in range(2))
+    ws = (torch.rand(rows, device="cuda", generator=g) + 0.5) / 4e4
+    q = torch.randint(-128, 128, (tokens, k), dtype=torch.int8, device="cuda", generator=g)
+    s = torch.rand(tokens, device="cuda", generator=g) + 0.5
+    m = be.upload_i8_gated(w, ws, v, ws)
+    h, tiles = (torch.zeros(tokens, rows, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    be.gemm_i8_swiglu(m, q, s, h)
+    try:
+        be.set_tuning(be.TUNE_I8_FORM, 1)
+        with pytest.raises(lbhip.KernelError):
+            be.gemm_i8_swiglu(m, q, s, tiles)
+        be.set_tuning(be.TUNE_I8_FORM, 6)
+        be.gemm_i8_swiglu(m, q, s, tiles)
+    finally:
+        be.set_tuning(be.TUNE_I8_FORM, 0)
+    assert torch.equal(h, tiles)
+    c = torch.cat([torch.randint(0, rows, (500,), generator=torch.Generator().manual_seed(1)), torch.arange(rows - 40, rows)])
+    at = c.cuda()
+    got = h[:, at]
+    q, s, w, v, ws = (a.cpu().numpy() for a in (q, s, w[at], v[at], ws[at]))
+    a, u = value(q, s, w, ws), value(q, s, v, ws)
+    want = a / (1 + np.exp(-a)) * u
+    check(got, want, torch.bfloat16, gated_off(a, u, want))
+    m.close()
+    del w, v, h, tiles, got
+    torch.cuda.empty_cache()
