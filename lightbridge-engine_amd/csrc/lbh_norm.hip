@@ -335,9 +335,9 @@ hipError_t launch_norm_form(const NormArgs &a, hipStream_t s) {
     // 4096 in 256 threads', of 8192 in 512 threads' (1024 threads leave room for one
     // workgroup on a CU: 333 rows of 7168 took two rounds), of 16384 in 1024
     // threads'.  Q8_K blocks go through LDS, which only the workgroup-per-row forms
-    // have.  Measured, input and output bytes a second: 6007 x 4096 bf16 with the
-    // residual to int8 4.3 TB/s, int8 of 1024 x 13312 f32 4.8 TB/s; one row of 4096
-    // 3.5 us and 64 rows 4.1 us, which is latency.
+    // have.  Measured as graph nodes, input and output bytes a second: 6007 x 4096 bf16
+    // with the residual to int8 4.3 TB/s, int8 of 1024 x 13312 f32 5.0 TB/s; one row of
+    // 4096 to int8 3.6 us and 64 rows to Q8_K 4.8 us, which is latency.
     const size_t lds = a.q8k ? (size_t)a.n * 4 : 0;
     if (a.n <= 512 && !a.q8k)
         hipLaunchKernelGGL((k_norm_rows<TY, 64, 1, VEC, NORM>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a);
