@@ -630,9 +630,9 @@ lbh_status lbh_moe_forward_leased(lbh_ctx *ctx, lbh_moe *moe, const lbh_expert_l
  * strides count elements, are at least the row's length, and bytes between the
  * rows are neither read for their value nor written.  Pointers need the alignment
  * of their element; rows of a multiple of 8 elements, and products' rows whose
- * address and stride are multiples of 16 bytes, are the fast ones.  Outputs may share no byte with each other or with an input,
- * except where "in place" is said.  rows / n_tokens == 0 does nothing.  At most
- * 2^20 rows a call. */
+ * address and stride are multiples of 16 bytes, are the fast ones.  Outputs may
+ * share no byte with each other or with an input, except where "in place" is said.
+ * rows / n_tokens == 0 does nothing.  At most 2^20 rows a call. */
 #define LBH_F16 1
 #define LBH_BF16 30
 
