@@ -720,6 +720,107 @@ lbh_status lbh_gemm_i8_swiglu(lbh_ctx *ctx, const lbh_i8_matrix *m, const int8_t
                               const float *x_scales_dev, size_t n_tokens, int32_t h_type, void *h_dev, size_t h_stride,
                               void *workspace_dev, size_t workspace_len, lbh_error *err);
 
+/* Activations of lbh_gemm_i8_act. */
+enum lbh_activation {
+    LBH_ACT_NONE = 0,
+    LBH_ACT_RELU = 1,
+    LBH_ACT_RELU2 = 2,     /* max(v, 0)^2 */
+    LBH_ACT_SILU = 3,      /* v / (1 + exp(-v)) */
+    LBH_ACT_GELU = 4,      /* v times the normal distribution's function of v */
+    LBH_ACT_GELU_TANH = 5, /* v / 2 (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) */
+};
+/* [async] The product with a bias, an activation and a scaled way into the residual:
+ *   y = residual + scale * act(v + bias)                  v as in lbh_gemm_i8
+ *   y = scale * act(gate + bias) * (up + up_bias)         a gated pair, without a residual
+ * bias and up_bias (optional, up_bias a pair's only) are float32 [rows].  In float32
+ * between the sum and y_type, to which it is rounded once; the activations are good to
+ * a few roundings of their value and their argument, and 0 where that is below
+ * 2^-119 |v|.  y may be the residual itself, in place.  The same bits for any number
+ * of tokens in the call.  Workspace as for lbh_gemm_i8. */
+lbh_status lbh_gemm_i8_act(lbh_ctx *ctx, const lbh_i8_matrix *m, const int8_t *x_dev, size_t x_stride,
+                           const float *x_scales_dev, size_t n_tokens, int32_t activation, const float *bias_dev,
+                           const float *up_bias_dev, double scale, int32_t y_type, void *y_dev, size_t y_stride,
+                           const void *residual_dev, size_t residual_stride, void *workspace_dev, size_t workspace_len,
+                           lbh_error *err);
+
+/* ---- a layer's experts in 8-bit integers ------------------------------------------
+ * What a mixture-of-experts layer has around and behind its router, for a batch of
+ * rows: the norms around a block, the routing, and the routed and shared experts
+ * over int8 matrices.  No counterpart in the reference, which computes these steps in
+ * 32 bits one token at a time (crates/bridge-kernels-reference/src/{norm,layer,moe}.rs);
+ * they are held to their formulas in 64 bits.  Operands as in the dense block above. */
+
+/* What a gate row goes through before it multiplies the block's output. */
+enum lbh_gate_act {
+    LBH_GATE_AS_IS = 0,
+    LBH_GATE_SIGMOID = 1,
+    LBH_GATE_SILU = 2,
+};
+/* [async] A block's output into the residual stream, and the norm in front of the next
+ * block, of `rows` rows of n elements (n <= 16384):
+ *   p = block * post_weight / sqrt(mean(block^2) + post_eps)   (post_weight NULL: block)
+ *   h = hidden + scale * a(gate) * p            (gate NULL: 1; gate_stride 0: one row for all)
+ *   v = h * weight / sqrt(mean(h^2) + eps)
+ * hidden_out receives h, rounded to float32 and to `type`; it may be hidden or block
+ * themselves, in place.  v goes to any of y (in y_type), int8 rows with scales (q and
+ * scales together) and Q8_K blocks (encoded; n % 256 == 0), each as in
+ * lbh_rms_norm_rows and its siblings; without weight there is no v and no such
+ * output.  Everything between the loads and the roundings is in 64 bits.  A row gets
+ * the same bits among any number of rows, at any addresses and strides (Q8_K: as
+ * lbh_rms_norm_q8_k_rows). */
+lbh_status lbh_block_norm_rows(lbh_ctx *ctx, int32_t type, const void *block_dev, size_t block_stride,
+                               const float *post_weight_dev, double post_eps, const void *gate_dev, size_t gate_stride,
+                               int32_t gate_act, double scale, const void *hidden_dev, size_t hidden_stride,
+                               void *hidden_out_dev, size_t hidden_out_stride, const float *weight_dev, double eps,
+                               size_t rows, size_t n, int32_t y_type, void *y_dev, size_t y_stride, int8_t *q_dev,
+                               size_t q_stride, float *scales_dev, uint8_t *encoded_dev, lbh_error *err);
+
+/* [async] Routing of a batch of rows x [n_tokens][hidden] (float32, binary16 or
+ * bfloat16): logits of every expert, the top_k (<= 16) best and their coefficients,
+ * ids ascending, in device memory:
+ *   mode 0: by logit, coefs = weight_scale * softmax over the chosen logits
+ *   mode 1: by sigmoid(logit) + bias, coefs = weight_scale * sigmoid / max(their sum, 2^-14)
+ * in 64 bits, ties to the lower id, coefs and logits (optional, [n_tokens][n_experts])
+ * rounded to float32.  A row with a logit (or score) that is not finite gets the ids
+ * 0 .. top_k - 1 with NaN coefficients.  The same bits for any number of rows, at most
+ * 2^19.  Unlike lbh_router_route_into and lbh_route_experts_batch it does not reproduce
+ * the reference's 32-bit sums.  Calls that may run at once need a workspace (8-byte
+ * aligned) each. */
+lbh_status lbh_router_route_rows(lbh_ctx *ctx, const lbh_router *router, int32_t type, const void *x_dev, size_t x_stride,
+                                 size_t n_tokens, size_t top_k, int32_t mode, double weight_scale, uint32_t *ids_dev,
+                                 float *coefs_dev, float *logits_dev, void *workspace_dev, size_t workspace_len,
+                                 lbh_error *err);
+/* For calls of exactly n_tokens rows (few rows take more than many). */
+size_t lbh_router_route_rows_workspace_bytes(const lbh_router *router, size_t n_tokens);
+
+/* The experts of a layer: for each a gated pair [ffn x n] and a down matrix [n x ffn], all
+ * of one shape, and optionally a shared expert of its own ffn.  The matrices stay the
+ * caller's and have to outlive the layer.  At most 1024 experts. */
+typedef struct lbh_moe_i8 lbh_moe_i8;
+/* [sync] */
+lbh_status lbh_moe_i8_create(lbh_ctx *ctx, const lbh_i8_matrix *const *gate_up, const lbh_i8_matrix *const *down,
+                             size_t n_experts, const lbh_i8_matrix *shared_gate_up, const lbh_i8_matrix *shared_down,
+                             lbh_moe_i8 **out, lbh_error *err);
+lbh_status lbh_moe_i8_destroy(lbh_moe_i8 *moe);
+/* Workspace bytes of a call (16-byte aligned); calls that may run at once need one each. */
+size_t lbh_moe_i8_workspace_bytes(const lbh_moe_i8 *moe, size_t n_tokens, size_t top_k);
+/* [async] The layer's experts for int8 rows x [n_tokens][n] with a scale each:
+ *   h = silu(gate) * up                      of each slot's expert, in 64 bits, rounded to float32
+ *   y[t] = residual[t] + sum over slots coefs[t][slot] * down(int8 row of h) + shared expert of x[t]
+ * int8 rows as lbh_quantize_i8_rows makes them, the sums over an expert's products
+ * exact, the sum over slots in 64 bits in their order, y rounded to float32 and to
+ * y_type.  ids and coefs [n_tokens][top_k] in device memory (lbh_router_route_rows,
+ * lbh_route_experts_batch); ids need no order, may repeat, and one that is no expert
+ * (as 0xffffffff) is an empty slot, whose coefficient is not used.  residual
+ * (optional) may be y itself, in place.  The same bits for any number of tokens and
+ * any order of the others.  n_tokens <= 256, n_tokens * top_k <= 2048, top_k <= 16;
+ * made for few tokens: every used expert's weights are read once. */
+lbh_status lbh_moe_i8_forward(lbh_ctx *ctx, const lbh_moe_i8 *moe, const int8_t *x_dev, size_t x_stride,
+                              const float *x_scales_dev, const uint32_t *ids_dev, const float *coefs_dev,
+                              size_t n_tokens, size_t top_k, int32_t y_type, void *y_dev, size_t y_stride,
+                              const void *residual_dev, size_t residual_stride, void *workspace_dev,
+                              size_t workspace_len, lbh_error *err);
+
 /* ---- diagnostics ------------------------------------------------------------- */
 
 /* Polls of the router chains' bounded LDS-ring waits before they give up (0: the

@@ -1900,22 +1900,6 @@ lbh_status lbh_route_experts_batch(lbh_ctx *ctx, const float *logits, size_t n_t
 
 // ================================================================== router
 
-struct lbh_router {
-    int device;
-    size_t n_experts, hidden;
-    float *w;            // transposed, interleaved by four (RouterArgs::w)
-    float *bias;         // [n_experts] or NULL
-    float *logits;
-    MoeRoute *route;     // device
-    MoeRoute *route_host;
-    // [0] first invalid selection input of route_into, [1] ring give-up of the
-    // block decodes (sticky until lbh_router_take_status), [2..4] their
-    // rejected selections (RouterArgs::reject), [5] ring give-up of route_into.
-    unsigned long long *status;
-    unsigned long long *status_host;
-    long long spin_limit;              // RouterArgs::spin_limit (0: default)
-};
-
 namespace {
 
 void free_router(lbh_router *r) {

@@ -6,6 +6,7 @@
 // nothing and leaves its outputs as they were.
 #include <hip/hip_runtime.h>
 
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -13,56 +14,12 @@
 #include "../../include/lightbridge_hip.h"
 #include "lbh_host.h"
 #include "lbh_internal.h"
+#include "lbh_operands.h"
 #include "lbh_rowtypes.h"
 
 using namespace lbh;
 
-// 8-bit integer channels in the product's tiles (lbh_i8.hip); gated: the gate's
-// and the up's channel groups alternate.
-struct lbh_i8_matrix {
-    int device;
-    size_t rows, k, kt, groups;   // groups: channel groups of one matrix
-    int gated;
-    uint8_t *tiles;
-    float *scales;
-    size_t bytes;
-};
-
 namespace {
-
-constexpr size_t MAX_TOKENS = (size_t)1 << 20;
-constexpr size_t MAX_STRIDE = (size_t)1 << 23;     // 256 rows stay below 2^31 bytes
-constexpr size_t MAX_K = 131071;                   // k * 128 * 128 < 2^31: the sums are exact
-constexpr size_t MAX_ROWS = (size_t)1 << 26;
-
-bool float_rows_type(int ty) { return row_elem_bytes(ty) != 0; }
-
-// Rows of an operand: `bytes` used bytes of every `pitch`.
-struct Span {
-    const void *p;
-    size_t pitch, bytes, rows;
-};
-Span span_of(const void *p, size_t stride, size_t elem, size_t cols, size_t rows) {
-    return {p, stride * elem, cols * elem, rows};
-}
-
-// Whether two operands share a byte.  Rows of one pitch may lie side by side
-// in a wider buffer; different pitches are taken by their whole extent.
-bool share(const Span &a, const Span &b) {
-    if (!a.p || !b.p || !a.rows || !b.rows) return false;
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
-    const uintptr_t xe = x + (a.rows - 1) * a.pitch + a.bytes, ye = y + (b.rows - 1) * b.pitch + b.bytes;
-    if (xe <= y || ye <= x) return false;
-    if (a.pitch != b.pitch || a.rows == 1 || b.rows == 1) return true;
-    const size_t d = y >= x ? (y - x) % a.pitch : (a.pitch - (x - y) % a.pitch) % a.pitch;
-    return d < a.bytes || a.pitch - d < b.bytes;
-}
-// The same operand twice (an update in place), or no byte in common.
-bool same_or_apart(const Span &a, const Span &b) {
-    return (a.p == b.p && (a.pitch == b.pitch || a.rows <= 1) && a.bytes == b.bytes) || !share(a, b);
-}
-
-bool aligned_to(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 lbh_status check_norm(const NormArgs &a, lbh_error *err) {
     const size_t n = (size_t)a.n, rows = (size_t)a.rows;
@@ -178,15 +135,6 @@ lbh_status check_i8_scales(lbh_ctx *ctx, const float *scales, size_t rows, uint3
     return fail(err, LBH_NON_FINITE_SCALE, 0, 0, 0, 0, bits, which, bad);
 }
 
-// Device memory of one creation call, released on every way out.
-struct Temp {
-    void *p = nullptr;
-    hipError_t get(size_t n) { return hipMalloc(&p, n); }
-    ~Temp() {
-        if (p) (void)hipFree(p);
-    }
-};
-
 lbh_status create_i8(lbh_ctx *ctx, const int8_t *const *w, const float *const *scales, int parts, size_t rows, size_t k,
                      int on_device, lbh_i8_matrix **out, lbh_error *err) {
     if (!ctx || !out) return fail(err, LBH_NULL_ARGUMENT);
@@ -231,11 +179,26 @@ lbh_status create_i8(lbh_ctx *ctx, const int8_t *const *w, const float *const *s
     return ok(err);
 }
 
+// What lbh_gemm_i8_act adds to a product.
+struct Epilogue {
+    int act;
+    const float *bias, *up_bias;
+    double scale;
+};
+
+// gated: the call's kind of matrix; -1: either, with the epilogue.
 lbh_status product(lbh_ctx *ctx, const lbh_i8_matrix *m, int gated, const int8_t *x, size_t x_stride, const float *xs,
                    size_t n_tokens, int32_t y_type, void *y, size_t y_stride, const void *residual,
-                   size_t residual_stride, void *workspace, size_t workspace_len, lbh_error *err) {
+                   size_t residual_stride, void *workspace, size_t workspace_len, lbh_error *err,
+                   const Epilogue *ep = nullptr) {
     if (!ctx || !m) return fail(err, LBH_NULL_ARGUMENT);
-    if (m->gated != gated || m->device != ctx->device) return fail(err, LBH_INVALID_PARAMETER, y_type);
+    if ((gated >= 0 && m->gated != gated) || m->device != ctx->device) return fail(err, LBH_INVALID_PARAMETER, y_type);
+    if (ep) {
+        if (ep->act < ACT_NONE || ep->act > ACT_GELU_TANH || !std::isfinite(ep->scale) || std::fabs(ep->scale) > FLT_MAX)
+            return fail(err, LBH_INVALID_PARAMETER, y_type);
+        if (m->gated ? residual != nullptr : ep->up_bias != nullptr) return fail(err, LBH_INVALID_PARAMETER, y_type);
+        if (!aligned_to(ep->bias, 4) || !aligned_to(ep->up_bias, 4)) return fail(err, LBH_INVALID_PARAMETER, y_type);
+    }
     const size_t e = row_elem_bytes(y_type);
     if (!e) return fail(err, LBH_UNSUPPORTED_TYPE, y_type);
     if (n_tokens == 0) return ok(err);   // no token, and no address asked for
@@ -253,6 +216,9 @@ lbh_status product(lbh_ctx *ctx, const lbh_i8_matrix *m, int gated, const int8_t
     const Span sy = span_of(y, y_stride, e, m->rows, n_tokens), sx = span_of(x, x_stride, 1, m->k, n_tokens),
                ss = {xs, 4, 4, n_tokens}, sr = span_of(residual, residual_stride, e, m->rows, n_tokens);
     if (share(sy, sx) || share(sy, ss) || !same_or_apart(sy, sr)) return fail(err, LBH_INVALID_PARAMETER, y_type);
+    const Span sb = {ep ? ep->bias : nullptr, 4 * m->rows, 4 * m->rows, 1},
+               su = {ep ? ep->up_bias : nullptr, 4 * m->rows, 4 * m->rows, 1};
+    if (share(sy, sb) || share(sy, su)) return fail(err, LBH_INVALID_PARAMETER, y_type);
     DeviceGuard g(ctx->device);
     I8Args a{};
     a.w = m->tiles;
@@ -269,7 +235,8 @@ lbh_status product(lbh_ctx *ctx, const lbh_i8_matrix *m, int gated, const int8_t
     a.k = (int32_t)m->k;
     a.kt = (int32_t)m->kt;
     a.out_type = y_type;
-    a.gated = gated;
+    a.gated = m->gated;
+    if (ep) a.epilogue = 1, a.act = ep->act, a.bias = ep->bias, a.up_bias = ep->up_bias, a.scale = (float)ep->scale;
     a.cu_count = ctx->cu_count;
     a.form = ctx->i8_form;
     a.vec_out = aligned_to(y, 16) && y_stride * e % 16 == 0 &&
@@ -281,7 +248,8 @@ lbh_status product(lbh_ctx *ctx, const lbh_i8_matrix *m, int gated, const int8_t
         if (!aligned_to(workspace, 16)) return fail(err, LBH_INVALID_PARAMETER);
         if (workspace_len < need) return fail(err, LBH_SCRATCH_TOO_SMALL, 0, n_tokens, need, workspace_len);
         const Span sw = {workspace, need, need, 1};
-        if (share(sw, sx) || share(sw, ss) || share(sw, sy) || share(sw, sr)) return fail(err, LBH_INVALID_PARAMETER, y_type);
+        if (share(sw, sx) || share(sw, ss) || share(sw, sy) || share(sw, sr) || share(sw, sb) || share(sw, su))
+            return fail(err, LBH_INVALID_PARAMETER, y_type);
         HIP_TRY(launch_i8_align_rows(x, a.x_stride, a.k, (int)pitch, (long long)n_tokens,
                                      static_cast<uint8_t *>(workspace), ctx->stream));
         a.x = static_cast<const int8_t *>(workspace);
@@ -460,6 +428,15 @@ lbh_status lbh_gemm_i8_swiglu(lbh_ctx *ctx, const lbh_i8_matrix *m, const int8_t
                               void *workspace, size_t workspace_len, lbh_error *err) {
     return product(ctx, m, 1, x, x_stride, x_scales, n_tokens, h_type, h, h_stride, nullptr, 0, workspace, workspace_len,
                    err);
+}
+
+lbh_status lbh_gemm_i8_act(lbh_ctx *ctx, const lbh_i8_matrix *m, const int8_t *x, size_t x_stride, const float *x_scales,
+                           size_t n_tokens, int32_t activation, const float *bias, const float *up_bias, double scale,
+                           int32_t y_type, void *y, size_t y_stride, const void *residual, size_t residual_stride,
+                           void *workspace, size_t workspace_len, lbh_error *err) {
+    const Epilogue ep{activation, bias, up_bias, scale};
+    return product(ctx, m, -1, x, x_stride, x_scales, n_tokens, y_type, y, y_stride, residual, residual_stride, workspace,
+                   workspace_len, err, &ep);
 }
 
 }  // extern "C"

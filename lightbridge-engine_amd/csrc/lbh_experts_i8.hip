@@ -1,0 +1,518 @@
+// lbh_experts_i8.hip — the feed-forward half of a mixture-of-experts layer for
+// few tokens, over int8 experts (lbh_i8.hip has the weights' layout).
+//
+//   h[p] = silu(g) * u          p = (token, slot): g, u the products of the slot's expert
+//   y[t] = residual[t] + sum over slots coef[p] * down(int8 row of h[p]) + down_shared(int8 row of h_shared[t])
+//
+// Integer sums are exact in any order; everything behind them is in 64 bits
+// (h is rounded to 32 bits once, y to 32 bits and its type), slots are added in their
+// order and the shared expert last, so a token's result hangs on its own row,
+// slots and weights alone, and the few roundings leave every int8 value of h where
+// the formula puts it but for one in millions.
+//
+// Bound: each used expert's weights once from HBM, 3 n ffn bytes; the products
+// themselves are a few percent of the matrix cores' rate.  So the launches go
+// by the weights: k_experts_up takes (expert, 16 channels of gate and up) per
+// workgroup with k split over its waves, k_experts_down takes 16 output channels
+// over every used expert, so that the sum over a token's slots ends in one
+// workgroup.  A matrix tile of 16 channels x 16 tokens costs the same for one
+// token as for sixteen, and weights stay in registers for all of an expert's
+// tokens.
+#include <hip/hip_runtime.h>
+
+#include "lbh_dev.h"
+#include "lbh_internal.h"
+#include "lbh_rows64.h"
+
+namespace lbh {
+
+namespace {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+
+constexpr int WAVES = 8;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *base, long long bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, (int)(uint32_t)bytes, 0x00020000);
+}
+// 16 bytes at a byte offset, zero past the resource's end.  ONCE: non-temporal.
+template <bool ONCE>
+__device__ __forceinline__ v4i load16(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+    return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, ONCE ? 2 : 0));
+}
+
+__device__ __forceinline__ int lane_rank(uint64_t mask) {   // set bits below this lane
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
+// The used experts, each with its (token, slot) pairs.  Up to 64 pairs each wave finds
+// them by itself, a pair a lane; more are sorted by k_experts_plan.  Slots whose id
+// is no expert are nobody's.
+struct Used {
+    int expert, count;   // wave-uniform
+    int pairs;           // up to 64 pairs: lane i holds the i-th
+    const int *list;     // more: the list
+};
+
+struct FewPairs {
+    int id;            // lane p: pair p's expert, or -1
+    uint64_t first;    // lanes with an expert's first pair
+    __device__ __forceinline__ FewPairs(const ExpertsArgs &a) {
+        const int lane = threadIdx.x & 63;
+        const uint32_t raw = lane < a.pairs ? a.ids[lane] : ~0u;
+        id = raw < (uint32_t)a.n_experts ? (int)raw : -1;
+        bool seen = id < 0;
+        for (int j = 0; j < a.pairs; ++j) {
+            const int other = __builtin_amdgcn_readlane(id, j);
+            seen |= j < lane && other == id;
+        }
+        first = __ballot(!seen);
+    }
+    __device__ __forceinline__ int used() const { return __builtin_popcountll(first); }
+    __device__ __forceinline__ Used at(int u) const {   // u < used()
+        const int lane = threadIdx.x & 63;
+        const uint64_t mine = __ballot(((first >> lane) & 1) && lane_rank(first) == u);
+        Used r;
+        r.expert = __builtin_amdgcn_readlane(id, (int)__builtin_ctzll(mine));
+        const uint64_t members = __ballot(id == r.expert);
+        r.count = __builtin_popcountll(members);
+        // member lanes to the front; the others to lanes behind them
+        const bool in = (members >> lane) & 1;
+        const int to = in ? lane_rank(members) : r.count + lane_rank(~members);
+        r.pairs = __builtin_amdgcn_ds_permute(4 * to, lane);
+        r.list = nullptr;
+        return r;
+    }
+};
+
+struct ManyPairs {
+    const ExpertsPlan *plan;
+    __device__ __forceinline__ ManyPairs(const ExpertsArgs &a) : plan(a.plan) {}
+    __device__ __forceinline__ int used() const { return __builtin_amdgcn_readfirstlane(plan->used); }
+    __device__ __forceinline__ Used at(int u) const {
+        const int from = __builtin_amdgcn_readfirstlane(plan->from[u]), to = __builtin_amdgcn_readfirstlane(plan->from[u + 1]);
+        return {__builtin_amdgcn_readfirstlane(plan->expert[u]), to - from, 0, plan->pair + from};
+    }
+};
+
+// The i-th pair of an expert (per lane; i < count).
+template <bool FEW>
+__device__ __forceinline__ int pair_at(const Used &u, int i) {
+    if constexpr (FEW) return __builtin_amdgcn_ds_bpermute(4 * i, u.pairs);
+    return u.list[i];
+}
+
+template <bool FEW>
+struct Pairs;
+template <>
+struct Pairs<true> : FewPairs {
+    using FewPairs::FewPairs;
+};
+template <>
+struct Pairs<false> : ManyPairs {
+    using ManyPairs::ManyPairs;
+};
+
+// Sorts more than 64 pairs by expert.  The order of an expert's pairs among
+// themselves hangs on the LDS atomics, and no result hangs on it: each pair has
+// a column of its own in the products.
+__global__ void __launch_bounds__(1024) k_experts_plan(ExpertsArgs a) {
+    __shared__ int count[1024], at[1024], wave_used[16], wave_pairs[16];
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    count[tid] = 0;
+    __syncthreads();
+    for (int p = tid; p < a.pairs; p += 1024)
+        if (a.ids[p] < (uint32_t)a.n_experts) atomicAdd(&count[a.ids[p]], 1);
+    __syncthreads();
+    const int mine = count[tid];
+    const uint64_t some = __ballot(mine != 0);
+    int sum = mine;   // inclusive within the wave
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const int below = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += below;
+    }
+    if (lane == 63) wave_pairs[wid] = sum, wave_used[wid] = __builtin_popcountll(some);
+    __syncthreads();
+    int u = lane_rank(some), from = sum - mine;
+    for (int w = 0; w < wid; ++w) u += wave_used[w], from += wave_pairs[w];
+    at[tid] = from;
+    if (mine) a.plan->expert[u] = tid, a.plan->from[u] = from;
+    if (tid == 1023) a.plan->used = u + (mine ? 1 : 0), a.plan->from[u + (mine ? 1 : 0)] = from + mine;
+    __syncthreads();
+    for (int p = tid; p < a.pairs; p += 1024)
+        if (a.ids[p] < (uint32_t)a.n_experts) a.plan->pair[atomicAdd(&at[a.ids[p]], 1)] = p;
+}
+
+// ------------------------------------------------------------ gate and up
+//
+// A workgroup has 16 channels of an expert's gate and up; wave w takes the k tiles
+// w, w + 8, ...  Tokens go straight to operand registers: 16 rows x 64 bytes an
+// instruction touch more lines than copies through LDS would, but at most 16 tokens
+// share a tile of weights that comes from HBM at a tenth of what the L1 moves.
+
+// Pairs base .. base + 16 NT - 1 of the expert against this wave's k tiles; D tiles a step.
+template <int NT, int D, bool FEW, bool SHARED, bool ONCE>
+__device__ __forceinline__ void up_tiles(const ExpertsArgs &a, const Used &u, int base, __amdgpu_buffer_rsrc_t rw,
+                                         __amdgpu_buffer_rsrc_t rx, int wid, v4i (&g)[NT], v4i (&up)[NT]) {
+    const int lane = threadIdx.x & 63;
+    uint32_t row[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int n = min(base + 16 * i + (lane & 15), u.count - 1);
+        const int t = SHARED ? n : pair_at<FEW>(u, n) / a.top_k;
+        row[i] = (uint32_t)t * (uint32_t)a.x_stride + 16 * (lane >> 4);
+    }
+    const int kt = a.kt_n;
+    v4i wg[2][D], wu[2][D], x[2][D][NT];
+    auto ask = [&](int b, int k0) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            const int k = k0 + d * WAVES;
+            // past the last tile: out of the resource's range, zero
+            wg[b][d] = load16<ONCE>(rw, lane * 16 + (k < kt ? k : 2 * kt) * 1024);
+            wu[b][d] = load16<ONCE>(rw, lane * 16 + (k < kt ? kt + k : 2 * kt) * 1024);
+        }
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) x[b][d][i] = load16<false>(rx, row[i] + (k0 + d * WAVES) * 64);
+    };
+    auto multiply = [&](int b) {
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                g[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wg[b][d], x[b][d][i], g[i], 0, 0, 0);
+                up[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wu[b][d], x[b][d][i], up[i], 0, 0, 0);
+            }
+    };
+    ask(0, wid);
+    for (int k = wid; k < kt; k += 2 * D * WAVES) {
+        ask(1, k + D * WAVES);
+        multiply(0);
+        ask(0, k + 2 * D * WAVES);
+        multiply(1);
+    }
+}
+
+template <int NT, int D, bool FEW, bool SHARED, bool ONCE>
+__device__ __forceinline__ void up_item(const ExpertsArgs &a, const Used &u, int base, int c0, __amdgpu_buffer_rsrc_t rw,
+                                        const float *gs, const float *us, v4i (*s_sum)[WAVES][64]) {
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const __amdgpu_buffer_rsrc_t rx = rsrc(a.x, (long long)(a.n_tokens - 1) * a.x_stride + a.x_bytes);
+    v4i g[NT] = {}, up[NT] = {};
+    up_tiles<NT, D, FEW, SHARED, ONCE>(a, u, base, rw, rx, wid, g, up);
+    // One value a thread: token tid / 16, channel tid % 16.
+    const int n0 = (tid >> 4) & 15, c = tid & 15, ffn = SHARED ? a.ffn_s : a.ffn;
+    const int from = n0 + 16 * (c >> 2);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        __syncthreads();   // what was there has been read
+        s_sum[0][wid][lane] = g[i], s_sum[1][wid][lane] = up[i];
+        __syncthreads();
+        const int n = base + 16 * i + n0;
+        int pair_of_row = 0;   // every lane takes part in the exchange
+        if constexpr (!SHARED) pair_of_row = pair_at<FEW>(u, min(n, u.count - 1));
+        if (tid < 256 && n < u.count && c0 + c < ffn) {
+            int sg = 0, su = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w)
+                sg += s_sum[0][w][from][c & 3], su += s_sum[1][w][from][c & 3];
+            const int p = SHARED ? n : pair_of_row, t = SHARED ? n : p / a.top_k;
+            const double xs = (double)a.x_scales[t];
+            const double vg = (double)sg * xs * (double)gs[c], vu = (double)su * xs * (double)us[c];
+            const float h = (float)(vg * sigmoid_f64(vg) * vu);
+            if constexpr (SHARED)
+                a.h_s[(long long)t * a.h_s_pitch + c0 + c] = h;
+            else
+                a.h[(long long)p * a.h_pitch + c0 + c] = h;
+        }
+    }
+}
+
+// Tiles of 16 tokens at once: as many as the call's tokens can fill.
+template <int NT, bool FEW, bool SHARED, bool ONCE>
+__device__ __forceinline__ void up_expert(const ExpertsArgs &a, const Used &u, int c0, __amdgpu_buffer_rsrc_t rw,
+                                          const float *gs, const float *us, v4i (*s_sum)[WAVES][64]) {
+    int base = 0;
+    if constexpr (NT == 4)
+        for (; u.count - base > 32; base += 64) up_item<4, 1, FEW, SHARED, ONCE>(a, u, base, c0, rw, gs, us, s_sum);
+    if constexpr (NT >= 2)
+        for (; u.count - base > 16; base += 32) up_item<2, 2, FEW, SHARED, ONCE>(a, u, base, c0, rw, gs, us, s_sum);
+    for (; base < u.count; base += 16) up_item<1, 4, FEW, SHARED, ONCE>(a, u, base, c0, rw, gs, us, s_sum);
+}
+
+// grid: (channel groups, used experts + shared)
+template <int NT, bool FEW, bool ONCE>
+__global__ void __launch_bounds__(64 * WAVES, 4) k_experts_up(ExpertsArgs a) {
+    __shared__ v4i s_sum[2][WAVES][64];
+    const int grp = blockIdx.x, c0 = grp * 16;
+    const long long bytes = 2ll * a.kt_n * 1024;
+    if (a.has_shared && blockIdx.y == 0) {
+        if (c0 >= a.ffn_s) return;
+        const float *s = a.shared.up_scales + grp * 32;
+        const Used all{0, a.n_tokens, 0, nullptr};
+        up_expert<NT, FEW, true, ONCE>(a, all, c0, rsrc(a.shared.up + grp * bytes, bytes), s, s + 16, s_sum);
+        return;
+    }
+    if (c0 >= a.ffn) return;
+    const Pairs<FEW> pairs(a);
+    const int i = blockIdx.y - a.has_shared;
+    if (i >= pairs.used()) return;
+    const Used u = pairs.at(i);
+    const ExpertI8 e = a.experts[u.expert];
+    const float *s = e.up_scales + grp * 32;
+    up_expert<NT, FEW, false, ONCE>(a, u, c0, rsrc(e.up + grp * bytes, bytes), s, s + 16, s_sum);
+}
+
+// ------------------------------------------------------ int8 rows of h
+//
+// One row a workgroup, as lbh_quantize_i8_rows does it.  Rows up to 4096 elements stay
+// in registers, longer ones are read twice.
+__global__ void __launch_bounds__(256) k_experts_quantize(ExpertsArgs a) {
+    const int row = blockIdx.x, tid = threadIdx.x;
+    const bool shared = row >= a.pairs;
+    if (!shared && a.ids[row] >= (uint32_t)a.n_experts) return;
+    const int n = shared ? a.ffn_s : a.ffn, kt = shared ? a.kt_fs : a.kt_f;
+    const float *h = shared ? a.h_s + (long long)(row - a.pairs) * a.h_s_pitch : a.h + (long long)row * a.h_pitch;
+    int8_t *q = shared ? a.hq_s + (long long)(row - a.pairs) * kt * 64 : a.hq + (long long)row * kt * 64;
+    constexpr int NV = 2;
+    auto take = [&](int i, float (&v)[8]) {   // rows are padded to 16 elements, what lies behind n is not read
+        const int e = (i * 256 + tid) * 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+        if (e + 8 <= n) {
+            const float4 lo = *reinterpret_cast<const float4 *>(h + e), hi = *reinterpret_cast<const float4 *>(h + e + 4);
+            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+        } else if (e < n) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (e + j < n) v[j] = h[e + j];
+        }
+    };
+    const int steps = (n + 2047) / 2048;
+    float v[NV][8], top = 0.0f, odd = 0.0f;
+    auto account = [&](const float (&x)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j])), odd = __builtin_fmaf(x[j], 0.0f, odd);
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) take(i, v[i]);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) account(v[i]);
+    for (int i = NV; i < steps; ++i) {
+        float x[8];
+        take(i, x);
+        account(x);
+    }
+    double t64 = (double)top, none = 0.0;
+    wave_sum_max(none, t64);
+    __shared__ double s_top[4];
+    __shared__ int s_odd[4];
+    const bool any = __ballot(odd != odd) != 0;
+    if ((tid & 63) == 0) s_top[tid >> 6] = t64, s_odd[tid >> 6] = any;
+    __syncthreads();
+    t64 = fmax(fmax(s_top[0], s_top[1]), fmax(s_top[2], s_top[3]));
+    float scale = (float)(t64 * (1.0 / 127.0));
+    double to_q = 0.0;
+    if (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3])
+        scale = __builtin_nanf("");
+    else if (scale < 0x1p-126f)
+        scale = 0.0f;
+    else
+        to_q = reciprocal_of(scale);
+    if (tid == 0) a.h_scales[row] = scale;
+    auto put = [&](int i, const float (&x)[8]) {
+        const int e = (i * 256 + tid) * 8;
+        if (e >= n) return;
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j >> 2] |= (uint32_t)(nearest_of_quotient((double)x[j], to_q) & 0xff) << (8 * (j & 3));
+        *reinterpret_cast<uint2 *>(q + e) = to_q == 0.0 ? make_uint2(0, 0) : make_uint2(w[0], w[1]);
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) put(i, v[i]);
+    for (int i = NV; i < steps; ++i) {
+        float x[8];
+        take(i, x);
+        put(i, x);
+    }
+}
+
+// ---------------------------------------------------------------- down
+//
+// A workgroup has 16 output channels.  Its waves take units of (expert, DOWN_TILES k
+// tiles) in turn, weights of the next unit on their way during the products of this
+// one; the integer sums of a pair meet in LDS, where their order does not
+// count, and the sum over a token's slots is made from there in the slots' order.
+constexpr int DOWN_TILES = 8;
+
+template <int OUT, bool FEW, bool ONCE>
+__global__ void __launch_bounds__(64 * WAVES, 2) k_experts_down(ExpertsArgs a) {
+    extern __shared__ int s_sum[];   // [pairs + shared rows][16]
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = blockIdx.x, rows = a.pairs + (a.has_shared ? a.n_tokens : 0);
+    for (int i = tid; i < rows * 4; i += 64 * WAVES) reinterpret_cast<v4i *>(s_sum)[i] = v4i{};
+    const Pairs<FEW> pairs(a);
+    const int used = pairs.used();
+    const int per = (a.kt_f + DOWN_TILES - 1) / DOWN_TILES;
+    const int first = a.has_shared ? (a.kt_fs + DOWN_TILES - 1) / DOWN_TILES : 0, units = first + used * per;
+    __syncthreads();
+
+    struct Unit {
+        Used u;
+        bool shared;
+        int kt, k0;
+        __amdgpu_buffer_rsrc_t rw, rh;
+    };
+    auto unit = [&](int j) {
+        Unit r;
+        r.shared = j < first;
+        const uint8_t *w;
+        if (r.shared) {
+            r.u = Used{0, a.n_tokens, 0, nullptr};
+            r.kt = a.kt_fs, r.k0 = j * DOWN_TILES, w = a.shared.down;
+            r.rh = rsrc(a.hq_s, (long long)a.n_tokens * a.kt_fs * 64);
+        } else {
+            const int i = (j - first) / per;
+            r.u = pairs.at(i);
+            r.kt = a.kt_f, r.k0 = ((j - first) - i * per) * DOWN_TILES, w = a.experts[r.u.expert].down;
+            r.rh = rsrc(a.hq, (long long)a.pairs * a.kt_f * 64);
+        }
+        r.rw = rsrc(w + (long long)grp * r.kt * 1024, (long long)r.kt * 1024);
+        return r;
+    };
+    auto row_of = [&](const Unit &r, int base) {
+        const int n = min(base + (lane & 15), r.u.count - 1);
+        return r.shared ? n : pair_at<FEW>(r.u, n);
+    };
+    auto ask = [&](const Unit &r, v4i (&w)[DOWN_TILES]) {
+#pragma unroll
+        for (int d = 0; d < DOWN_TILES; ++d)   // past the last tile: zero
+            w[d] = load16<ONCE>(r.rw, lane * 16 + (r.k0 + d) * 1024);
+    };
+    auto tokens = [&](const Unit &r, int row, v4i (&x)[DOWN_TILES]) {
+        const uint32_t at = (uint32_t)row * (uint32_t)(r.kt * 64) + 16 * (lane >> 4) + r.k0 * 64;
+#pragma unroll
+        for (int d = 0; d < DOWN_TILES; ++d) x[d] = load16<false>(r.rh, at + d * 64);
+    };
+    auto add = [&](const Unit &r, int base, int row, const v4i (&w)[DOWN_TILES], const v4i (&x)[DOWN_TILES]) {
+        v4i acc = {};
+#pragma unroll
+        for (int d = 0; d < DOWN_TILES; ++d) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d], x[d], acc, 0, 0, 0);
+        if (base + (lane & 15) < r.u.count) {
+            int *to = s_sum + ((r.shared ? a.pairs : 0) + row) * 16 + 4 * (lane >> 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) atomicAdd(to + e, acc[e]);
+        }
+    };
+    v4i w0[DOWN_TILES], w1[DOWN_TILES], x0[DOWN_TILES], x1[DOWN_TILES];
+    auto work = [&](const Unit &r, int row, const v4i (&w)[DOWN_TILES], const v4i (&x)[DOWN_TILES]) {
+        add(r, 0, row, w, x);
+        for (int base = 16; base < r.u.count; base += 16) {   // further tokens of the same weights
+            v4i more[DOWN_TILES];
+            const int other = row_of(r, base);
+            tokens(r, other, more);
+            add(r, base, other, w, more);
+        }
+    };
+    if (wid < units) {
+        Unit r0 = unit(wid), r1;
+        int row0 = row_of(r0, 0), row1 = 0;
+        ask(r0, w0), tokens(r0, row0, x0);
+        for (int j = wid; j < units; j += 2 * WAVES) {
+            const bool next = j + WAVES < units;
+            if (next) {
+                r1 = unit(j + WAVES);
+                row1 = row_of(r1, 0);
+                ask(r1, w1), tokens(r1, row1, x1);
+            }
+            work(r0, row0, w0, x0);
+            if (!next) break;
+            if (j + 2 * WAVES < units) {
+                r0 = unit(j + 2 * WAVES);
+                row0 = row_of(r0, 0);
+                ask(r0, w0), tokens(r0, row0, x0);
+            }
+            work(r1, row1, w1, x1);
+        }
+    }
+    __syncthreads();
+    using T = row_t<OUT>;
+    for (int i = tid; i < a.n_tokens * 16; i += 64 * WAVES) {
+        const int t = i >> 4, c = grp * 16 + (i & 15);
+        if (c >= a.n) continue;
+        double sum = 0.0;
+        for (int s = 0; s < a.top_k; ++s) {
+            const int p = t * a.top_k + s;
+            const uint32_t id = a.ids[p];
+            if (id >= (uint32_t)a.n_experts) continue;
+            const double scale = (double)a.coefs[p] * (double)a.h_scales[p];
+            sum += (double)s_sum[p * 16 + (i & 15)] * (double)a.down_scales[(long long)id * a.down_pitch + c] * scale;
+        }
+        if (a.has_shared)
+            sum += (double)s_sum[(a.pairs + t) * 16 + (i & 15)] * (double)a.shared.down_scales[c] * (double)a.h_scales[a.pairs + t];
+        if (a.residual) sum += (double)static_cast<const T *>(a.residual)[(long long)t * a.residual_stride + c];
+        static_cast<T *>(a.y)[(long long)t * a.y_stride + c] = (T)(float)sum;
+    }
+}
+
+template <bool FEW, bool ONCE>
+hipError_t launch_up(const ExpertsArgs &a, hipStream_t s) {
+    const int widest = a.has_shared && a.ffn_s > a.ffn ? a.ffn_s : a.ffn;
+    const int used = a.pairs < a.n_experts ? a.pairs : a.n_experts;
+    const dim3 grid((widest + 15) / 16, used + a.has_shared);
+    if (a.n_tokens <= 16)
+        hipLaunchKernelGGL((k_experts_up<1, FEW, ONCE>), grid, dim3(64 * WAVES), 0, s, a);
+    else if (a.n_tokens <= 32)
+        hipLaunchKernelGGL((k_experts_up<2, FEW, ONCE>), grid, dim3(64 * WAVES), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_experts_up<4, FEW, ONCE>), grid, dim3(64 * WAVES), 0, s, a);
+    return hipGetLastError();
+}
+
+template <int OUT, bool FEW, bool ONCE>
+hipError_t launch_down(const ExpertsArgs &a, hipStream_t s) {
+    const int lds = (a.pairs + (a.has_shared ? a.n_tokens : 0)) * 64;
+    auto kernel = k_experts_down<OUT, FEW, ONCE>;
+    if (lds > 64 * 1024) {
+        const hipError_t e =
+            hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(kernel, dim3((a.n + 15) / 16), dim3(64 * WAVES), lds, s, a);
+    return hipGetLastError();
+}
+
+template <bool FEW>
+hipError_t launch_layer(const ExpertsArgs &a, hipStream_t s) {
+    if constexpr (!FEW) {
+        hipLaunchKernelGGL(k_experts_plan, dim3(1), dim3(1024), 0, s, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    hipError_t e = launch_up<FEW, true>(a, s);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(k_experts_quantize, dim3(a.pairs + (a.has_shared ? a.n_tokens : 0)), dim3(256), 0, s, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    switch (a.y_type) {
+    case T_F32: return launch_down<T_F32, FEW, true>(a, s);
+    case T_F16: return launch_down<T_F16, FEW, true>(a, s);
+    case T_BF16: return launch_down<T_BF16, FEW, true>(a, s);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace
+
+hipError_t launch_experts_i8(const ExpertsArgs &a, hipStream_t s) {
+    if (a.n_tokens <= 0) return hipSuccess;
+    if (a.n_tokens > EXPERTS_MAX_TOKENS || a.pairs != a.n_tokens * a.top_k || a.pairs < 1 || a.pairs > EXPERTS_MAX_PAIRS ||
+        a.n_experts < 1 || a.n_experts > EXPERTS_MAX)
+        return hipErrorInvalidValue;
+    return a.pairs <= 64 ? launch_layer<true>(a, s) : launch_layer<false>(a, s);
+}
+
+}  // namespace lbh

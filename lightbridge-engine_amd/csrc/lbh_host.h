@@ -31,6 +31,33 @@ struct lbh_matrix {
     uint8_t *gemm_a;     // MFMA-ready copy for token batches (lbh_matrix_prepare_gemm), or NULL
 };
 
+// 8-bit integer channels in the product's tiles (lbh_i8.hip); gated: the gate's
+// and the up's channel groups alternate.
+struct lbh_i8_matrix {
+    int device;
+    size_t rows, k, kt, groups;   // groups: channel groups of one matrix
+    int gated;
+    uint8_t *tiles;
+    float *scales;
+    size_t bytes;
+};
+
+struct lbh_router {
+    int device;
+    size_t n_experts, hidden;
+    float *w;            // transposed, interleaved by four (RouterArgs::w)
+    float *bias;         // [n_experts] or NULL
+    float *logits;
+    lbh::MoeRoute *route;     // device
+    lbh::MoeRoute *route_host;
+    // [0] first invalid selection input of route_into, [1] ring give-up of the
+    // block decodes (sticky until lbh_router_take_status), [2..4] their
+    // rejected selections (RouterArgs::reject), [5] ring give-up of route_into.
+    unsigned long long *status;
+    unsigned long long *status_host;
+    long long spin_limit;              // RouterArgs::spin_limit (0: default)
+};
+
 namespace {
 
 lbh_status fail(lbh_error *err, lbh_status st, int ty = 0, uint64_t index = 0, uint64_t expected = 0,

@@ -241,6 +241,26 @@ struct NormArgs {
 };
 constexpr int NORM_MAX_Q8K = 16384;   // a row of Q8_K input waits in LDS
 
+// A block's output into the residual stream, and the next norm (lbh_block_norm.hip).
+// Strides are in elements.
+enum : int { GATE_AS_IS = 0, GATE_SIGMOID = 1, GATE_SILU = 2 };
+struct BlockNormArgs {
+    const void *block, *hidden;   // [rows][n] of `type`
+    const void *gate;             // optional, [rows][n] of `type`; stride 0: one row for all
+    void *hidden_out;             // [rows][n] of `type`
+    const float *post_weight;     // [n]; NULL: no norm behind the block
+    const float *weight;          // [n]; NULL: no norm in front of the next one, and no output but hidden_out
+    void *y;                      // [rows][n] of y_type
+    uint8_t *q8k;                 // as NormArgs::q8k
+    int8_t *q;                    // [rows][n]
+    float *scales;                // [rows]
+    long long block_stride, hidden_stride, gate_stride, hidden_out_stride, y_stride, q_stride;
+    long long rows;
+    int32_t n, type, y_type, gate_act;
+    double post_eps, eps, inv_n, scale;
+};
+constexpr int BLOCK_NORM_MAX = 16384;   // a row stays in registers
+
 // 8-bit integer product (lbh_i8.hip).  Strides are in elements; x rows start
 // at multiples of 16 bytes.
 struct I8Args {
@@ -256,8 +276,72 @@ struct I8Args {
     int32_t vec_out;         // y and residual rows start at multiples of 16 bytes
     int32_t cu_count;
     int32_t form;            // 0: the rule's; else the form's number (LBH_TUNE_I8_FORM)
+    // epilogue != 0: y = residual + scale * act(product + bias), a pair act(gate + bias) *
+    // (up + up_bias) (* scale); else the product, a pair's SwiGLU
+    int32_t epilogue, act;
+    const float *bias, *up_bias;   // [rows], optional
+    float scale;
 };
 constexpr int I8_FORMS = 11;
+// Activations (enum lbh_activation of the C ABI).
+enum : int { ACT_NONE = 0, ACT_RELU = 1, ACT_RELU2 = 2, ACT_SILU = 3, ACT_GELU = 4, ACT_GELU_TANH = 5 };
+
+// ------------------------------------------------ int8 experts (lbh_experts_i8.hip)
+constexpr int EXPERTS_MAX = 1024;           // routed experts of a layer
+constexpr int EXPERTS_MAX_TOKENS = 256;     // of a call
+constexpr int EXPERTS_MAX_PAIRS = 2048;     // tokens * top_k; with the shared rows their sums fit the LDS
+struct ExpertI8 {
+    const uint8_t *up, *down;               // tiles of the gated pair and of the down matrix
+    const float *up_scales, *down_scales;   // gate and up alternate by 16
+};
+struct ExpertsPlan {
+    int32_t used;
+    int32_t expert[EXPERTS_MAX], from[EXPERTS_MAX + 1];
+    int32_t pair[EXPERTS_MAX_PAIRS];
+};
+struct ExpertsArgs {
+    const ExpertI8 *experts;    // device table [n_experts]
+    const float *down_scales;   // [n_experts][down_pitch]: the down matrices' scales side by side
+    ExpertI8 shared;
+    int32_t has_shared, n_experts;
+    int32_t n, ffn, ffn_s, kt_n, kt_f, kt_fs;   // widths and their k tiles of 64
+    int32_t down_pitch;
+    const int8_t *x;            // rows at multiples of 16 bytes
+    const float *x_scales;
+    long long x_stride;
+    int32_t x_bytes;            // of a row that may be read
+    int32_t n_tokens, top_k, pairs;
+    const uint32_t *ids;        // [n_tokens][top_k]
+    const float *coefs;
+    void *y;
+    const void *residual;
+    long long y_stride, residual_stride;
+    int32_t y_type;
+    // workspace
+    ExpertsPlan *plan;
+    float *h, *h_s;             // rows of h_pitch, h_s_pitch (multiples of 16)
+    long long h_pitch, h_s_pitch;
+    int8_t *hq, *hq_s;          // rows of kt_f * 64, kt_fs * 64
+    float *h_scales;            // [pairs + n_tokens]
+};
+hipError_t launch_experts_i8(const ExpertsArgs &a, hipStream_t s);
+
+// Routing of rows (lbh_route_rows.hip).
+struct RouteRowsArgs {
+    const float *w;             // RouterArgs::w
+    const float *bias;          // mode 1
+    const void *x;              // [n_tokens][hidden] of x_type
+    long long x_stride;
+    double *part;               // workspace: [parts][n_tokens][n_experts]
+    uint32_t *ids;              // [n_tokens][top_k]
+    float *coefs, *logits;      // logits optional, [n_tokens][n_experts]
+    double weight_scale;
+    int32_t n_tokens, n_experts, hidden, top_k, mode, x_type;
+};
+constexpr int ROUTE_SLICES = 8;
+// Slices whose sums wait in the workspace.
+constexpr int route_parts(long long n_tokens) { return n_tokens <= 64 ? ROUTE_SLICES : 1; }
+hipError_t launch_route_rows(const RouteRowsArgs &a, hipStream_t s);
 
 // Batch selection: top-k of each token's finished logits (select_route).
 struct RouteBatchArgs {
@@ -271,6 +355,7 @@ struct RouteBatchArgs {
 };
 
 hipError_t launch_norm_rows(const NormArgs &a, hipStream_t s);
+hipError_t launch_block_norm(const BlockNormArgs &a, hipStream_t s);
 // Weight rows [rows][k] and scales [rows] into or out of the product's tiles:
 // channel group g of this matrix is group g * step + part of the tiles.
 hipError_t launch_i8_layout(const int8_t *rowmajor, uint8_t *tiles, const float *scales, float *tile_scales,
@@ -278,6 +363,9 @@ hipError_t launch_i8_layout(const int8_t *rowmajor, uint8_t *tiles, const float 
 hipError_t launch_i8_align_rows(const int8_t *x, long long stride, int k, int pitch, long long n, uint8_t *out,
                                 hipStream_t s);
 hipError_t launch_i8_product(const I8Args &a, hipStream_t s);
+// Its forms with an epilogue (form from 0): every activation but ACT_GELU, and that.
+hipError_t launch_i8_sigmoid(const I8Args &a, int form, hipStream_t s);
+hipError_t launch_i8_normal(const I8Args &a, int form, hipStream_t s);
 // out[i][c] = the exact f32 decode of element c of row r0 + i (quantized types).
 hipError_t launch_dequant_rows(const MatView &m, long long r0, long long n, float *out, hipStream_t s);
 

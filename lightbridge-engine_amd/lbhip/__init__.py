@@ -22,6 +22,8 @@ LIB_PATH = PKG_DIR / "liblightbridge_hip.so"
 F32, Q4_K, Q5_K, Q8_K, IQ3_S, IQ2_S = 0, 12, 13, 15, 21, 22
 F16, BF16 = 1, 30   # row operands of the norm and the int8 products
 Q8_K_BLOCK_ELEMENTS, Q8_K_BLOCK_BYTES = 256, 292
+ACTIVATIONS = {"none": 0, "relu": 1, "relu2": 2, "silu": 3, "gelu": 4, "gelu_tanh": 5}   # gemm_i8_act
+GATE_ACTS = {"none": 0, "sigmoid": 1, "silu": 2}                                          # block_norm_rows
 BLOCK_BYTES = {Q4_K: 144, Q5_K: 176, IQ2_S: 82, IQ3_S: 110}
 
 STATUS = {
@@ -167,6 +169,15 @@ def lib() -> C.CDLL:
             "lbh_gemm_i8_workspace_bytes": ([p, sz], sz),
             "lbh_gemm_i8": ([p, p, p, sz, p, sz, i32, p, sz, p, sz, p, sz, E], i32),
             "lbh_gemm_i8_swiglu": ([p, p, p, sz, p, sz, i32, p, sz, p, sz, E], i32),
+            "lbh_gemm_i8_act": ([p, p, p, sz, p, sz, i32, p, p, C.c_double, i32, p, sz, p, sz, p, sz, E], i32),
+            "lbh_block_norm_rows": ([p, i32, p, sz, p, C.c_double, p, sz, i32, C.c_double, p, sz, p, sz, p, C.c_double,
+                                     sz, sz, i32, p, sz, p, sz, p, p, E], i32),
+            "lbh_router_route_rows": ([p, p, i32, p, sz, sz, sz, i32, C.c_double, p, p, p, p, sz, E], i32),
+            "lbh_router_route_rows_workspace_bytes": ([p, sz], sz),
+            "lbh_moe_i8_create": ([p, p, p, sz, p, p, C.POINTER(p), E], i32),
+            "lbh_moe_i8_destroy": ([p], i32),
+            "lbh_moe_i8_workspace_bytes": ([p, sz, sz], sz),
+            "lbh_moe_i8_forward": ([p, p, p, sz, p, p, p, sz, sz, i32, p, sz, p, sz, p, sz, E], i32),
             "lbh_matrix_create_streamed": ([p, i32, sz, sz, p, p, C.POINTER(p), E], i32),
         }
         for name, (args, res) in sig.items():
@@ -245,7 +256,7 @@ class HipBackend:
         if not torch.cuda.is_available():
             raise RuntimeError("HipBackend needs a ROCm GPU")
         self.device = device
-        self._f32, self._i8 = torch.float32, torch.int8
+        self._f32, self._i8, self._i32 = torch.float32, torch.int8, torch.int32
         _ROW_TYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
         torch.cuda.set_device(device)
         self._stream = stream if stream is not None else torch.cuda.current_stream(device)
@@ -475,6 +486,86 @@ class HipBackend:
         """h [tokens, rows] = silu(gate) * up of int8 rows q times a gated pair (asynchronous)."""
         _call(lib().lbh_gemm_i8_swiglu, *self._product_args(m, q, scales, h),
               *_space(self.device, workspace))
+
+    def gemm_i8_act(self, m: "DeviceI8Matrix", q, scales, y, activation: str = "none", workspace=None, bias=None,
+                    up_bias=None, residual=None, scale: float = 1.0) -> None:
+        """y = (residual +) scale * act(int8 rows q times the matrix + bias), of a gated pair
+        scale * act(gate + bias) * (up + up_bias); activation: a name of ACTIVATIONS (asynchronous)."""
+        dev, f32, rows = self.device, self._f32, m.rows
+        n = q.shape[0]
+        _call(lib().lbh_gemm_i8_act, self.ctx, m.handle, *_rows(dev, q, (n, m.k), self._i8),
+              _vector(dev, scales, n, f32, "scales"), n, ACTIVATIONS[activation],
+              None if bias is None else _vector(dev, bias, rows, f32, "bias"),
+              None if up_bias is None else _vector(dev, up_bias, rows, f32, "up_bias"), scale, _row_type(y),
+              *_rows(dev, y, (n, rows)), *_rows(dev, residual, y.shape, y.dtype), *_space(dev, workspace))
+
+    # -- a layer's experts in 8-bit integers ------------------------------------------------
+    def block_norm_rows(self, block, hidden, hidden_out, post_weight=None, post_eps: float = 0.0, gate=None,
+                        gate_act: str = "none", scale: float = 1.0, weight=None, eps: float = 0.0, y=None, q=None,
+                        scales=None, encoded=None) -> None:
+        """hidden_out = h = hidden + scale * a(gate) * norm(block) [rows, n], and with `weight` the norm of h into any of
+        y, int8 rows (q, scales) and Q8_K blocks (encoded).  post_weight None: block as it is; gate [rows, n], or
+        [1, n] for every row; gate_act: "none", "sigmoid" or "silu" (asynchronous).  hidden_out may be hidden or block."""
+        dev, f32, shape, dt = self.device, self._f32, hidden.shape, hidden.dtype
+        rows, n = shape
+        ty = _row_type(hidden)
+        if gate is None:
+            gp, gs = None, 0
+        else:
+            one = gate.shape[0] == 1 and rows != 1
+            gp, gs = _rows(dev, gate, (1, n) if one else shape, dt)
+            gs = 0 if one else gs
+        if encoded is not None:
+            assert encoded.get_device() == dev and encoded.is_contiguous(), f"expected a contiguous tensor on GPU {dev}"
+            assert n % 256 or encoded.nbytes == rows * (n // 256) * Q8_K_BLOCK_BYTES, "encoded"
+        _call(lib().lbh_block_norm_rows, self.ctx, ty, *_rows(dev, block, shape, dt),
+              None if post_weight is None else _vector(dev, post_weight, n, f32, "post_weight"), post_eps, gp, gs,
+              GATE_ACTS[gate_act], scale, *_rows(dev, hidden, shape), *_rows(dev, hidden_out, shape, dt),
+              None if weight is None else _vector(dev, weight, n, f32, "weight"), eps, rows, n,
+              ty if y is None else _row_type(y), *_rows(dev, y, shape), *_rows(dev, q, shape, self._i8),
+              None if scales is None else _vector(dev, scales, rows, f32, "scales"),
+              None if encoded is None else encoded.data_ptr())
+
+    def router(self, weights, bias=None) -> "Router":
+        """The router of weights [n_experts, hidden] and an optional selection bias (numpy arrays)."""
+        return Router(self, weights, bias)
+
+    @staticmethod
+    def route_rows_workspace_bytes(router: "Router", n_tokens: int) -> int:
+        return lib().lbh_router_route_rows_workspace_bytes(router.handle, n_tokens)
+
+    def route_rows(self, router: "Router", x, ids, coefs, workspace, mode: int = 0, weight_scale: float = 1.0,
+                   logits=None) -> None:
+        """The best experts of rows x [tokens, hidden]: ids (int32) and coefs (float32) [tokens, top_k], ids ascending,
+        and the logits [tokens, n_experts] when given (asynchronous, in 64 bits)."""
+        dev, f32 = self.device, self._f32
+        n, top_k = ids.shape
+        assert coefs.shape == ids.shape, "ids and coefs of one shape"
+        _call(lib().lbh_router_route_rows, self.ctx, router.handle, _row_type(x), *_rows(dev, x, (n, router.hidden)), n,
+              top_k, mode, weight_scale, _vector(dev, ids, n * top_k, self._i32, "ids"),
+              _vector(dev, coefs, n * top_k, f32, "coefs"),
+              None if logits is None else _vector(dev, logits, n * router.n_experts, f32, "logits"),
+              *_space(dev, workspace))
+
+    def moe_i8_create(self, experts, shared=None) -> "MoeI8Layer":
+        """experts: (gated pair, down matrix) of each routed expert; shared: those of the shared one."""
+        return MoeI8Layer(self, experts, shared)
+
+    @staticmethod
+    def moe_i8_workspace_bytes(moe: "MoeI8Layer", n_tokens: int, top_k: int) -> int:
+        return lib().lbh_moe_i8_workspace_bytes(moe.handle, n_tokens, top_k)
+
+    def moe_i8_forward(self, moe: "MoeI8Layer", q, scales, ids, coefs, y, workspace, residual=None) -> None:
+        """y [tokens, n] = (residual +) the routed experts of int8 rows q [tokens, n], each token's by ids (int32) and coefs
+        [tokens, top_k], + the shared expert (asynchronous).  An id that is no expert is an empty slot."""
+        dev, f32 = self.device, self._f32
+        n, top_k = ids.shape
+        shape = (n, moe.n)
+        assert coefs.shape == ids.shape, "ids and coefs of one shape"
+        _call(lib().lbh_moe_i8_forward, self.ctx, moe.handle, *_rows(dev, q, shape, self._i8),
+              _vector(dev, scales, n, f32, "scales"), _vector(dev, ids, n * top_k, self._i32, "ids"),
+              _vector(dev, coefs, n * top_k, f32, "coefs"), n, top_k, _row_type(y), *_rows(dev, y, shape),
+              *_rows(dev, residual, shape, y.dtype), *_space(dev, workspace))
 
     def f16_to_f32(self, src, dst) -> None:
         _call(lib().lbh_debug_f16_to_f32, self.ctx, _dev_ptr(src), _dev_ptr(dst), src.numel())
@@ -812,6 +903,33 @@ class DeviceI8Matrix:
     def close(self) -> None:
         if self.handle:
             lib().lbh_i8_matrix_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class MoeI8Layer:
+    """The experts of a layer over int8 matrices: (gated pair, down matrix) of each routed expert and of an optional
+    shared one.  The matrices are kept alive with the layer."""
+
+    def __init__(self, be: HipBackend, experts, shared=None):
+        self.handle = None
+        self.be, self._keep, self.n_experts = be, (list(experts), shared), len(experts)
+        pairs = (C.c_void_p * len(experts))(*(e[0].handle for e in experts))
+        downs = (C.c_void_p * len(experts))(*(e[1].handle for e in experts))
+        h = C.c_void_p()
+        _call(lib().lbh_moe_i8_create, be.ctx, pairs, downs, len(experts), shared[0].handle if shared else None,
+              shared[1].handle if shared else None, C.byref(h))
+        self.handle = h
+        self.n, self.ffn = experts[0][0].k, experts[0][0].rows
+
+    def close(self) -> None:
+        if self.handle:
+            lib().lbh_moe_i8_destroy(self.handle)
             self.handle = None
 
     def __del__(self):
