@@ -22,139 +22,151 @@ namespace lbh {
 
 namespace {
 
-// The block-wide sum, and the second reduction's sum, maximum and oddness.
-template <int NW>
-struct RowScratch {
-    double first[NW], sum[NW], top[NW];
-    int odd[NW];
-};
+enum : int { NO_GATE, AS_IS, ACTIVATED };
+
+// Eight consecutive elements of a row as they are in memory.
+template <int TY>
+using raw8 = rvec<row_t<TY>, 8>;
 
 // One row by TPR threads, 8 * NV elements of each operand in a thread's registers
-// (n <= 8 * NV * TPR).  VEC: a thread's eight elements of a step are consecutive (n a
-// multiple of 8); otherwise they lie TPR apart.
-template <int TY, int TPR, int NV, bool VEC>
+// (n <= 8 * NV * TPR), 16-bit ones packed as they came until they are used.  A thread's
+// eight elements of a step are consecutive and moved as words of 16 bytes at any
+// address.  Where they reach past the row's end, the words are the row's last eight
+// elements, shifted into place once everything is on its way: no load waits behind a
+// branch (elements one by one, TPR apart, took twice as long: 333 x 4095 fp16 with
+// gates 17.2 us).
+// GATE: no gate, one as it is, one through an activation.
+template <int TY, int TPR, int NV, int GATE>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(BlockNormArgs p) {
     using T = row_t<TY>;
     constexpr int RPW = TPR < 256 ? 256 / TPR : 1;   // rows per workgroup
     constexpr int NW = TPR / 64;                     // waves per row
     const int tid = threadIdx.x % TPR;
-    const long long row = (long long)blockIdx.x * RPW + threadIdx.x / TPR;
-    const bool live = RPW == 1 || row < p.rows;
-    const long long rr = live ? row : 0;
     const int n = p.n;
-    const T *blk = static_cast<const T *>(p.block) + rr * p.block_stride;
-    const T *hid = static_cast<const T *>(p.hidden) + rr * p.hidden_stride;
-    const T *gat = p.gate ? static_cast<const T *>(p.gate) + rr * p.gate_stride : nullptr;
-    T *ho = static_cast<T *>(p.hidden_out) + rr * p.hidden_out_stride;
 
-    auto at = [&](int i, int j) { return VEC ? (i * TPR + tid) * 8 + j : (i * 8 + j) * TPR + tid; };
-    // Elements of step i of a row, zeros (or `fill`) behind its end.
-    auto take = [&](auto ty, const auto *src, int i, float (&v)[8], float fill) {
-        if constexpr (VEC) {
-            if (at(i, 0) < n) {
-                load8<decltype(ty)::value>(src + at(i, 0), v);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = fill;
-            }
+    auto at = [&](int i) { return (i * TPR + tid) * 8; };
+    auto take = [&](const auto *src, int i, auto &v) {
+        if (n >= 8) {
+            __builtin_memcpy(&v, src + min(at(i), n - 8), sizeof v);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = at(i, j) < n ? (float)src[at(i, j)] : fill;
+            for (int j = 0; j < 8; ++j) v[j] = at(i) + j < n ? src[at(i) + j] : 0;
         }
     };
-    using Row = std::integral_constant<int, TY>;
-    using F32 = std::integral_constant<int, T_F32>;
-    float o[NV][8], h[NV][8], g[NV][8], w1[NV][8], w2[NV][8];
+    // The words of a step that reaches past the end: shifted, zeros behind it.
+    auto settle = [&](int i, auto &v) {
+        const int over = at(i) + 8 - n;
+        if (over <= 0 || n < 8) return;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) take(Row{}, blk, i, o[i], 0.0f);
+        for (int s = 4; s; s /= 2)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (over & s) v[j] = v[j + s < 8 ? j + s : 7];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j + over >= 8) v[j] = 0;
+    };
+    const long long row = (long long)blockIdx.x * RPW + (RPW == 1 ? 0 : threadIdx.x / TPR);
+    if (RPW > 1 && row >= p.rows) return;   // a wave with a row of its own, without a barrier
+    const T *blk = static_cast<const T *>(p.block) + row * p.block_stride;
+    const T *hid = static_cast<const T *>(p.hidden) + row * p.hidden_stride;
+    T *ho = static_cast<T *>(p.hidden_out) + row * p.hidden_out_stride;
+    raw8<TY> o[NV], x[NV], g[NV];
+    raw8<T_F32> w1[NV], w2[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) take(blk, i, o[i]);
     if (p.post_weight) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) take(F32{}, p.post_weight, i, w1[i], 0.0f);
+        for (int i = 0; i < NV; ++i) take(p.post_weight, i, w1[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) w1[i] = 1.0f;
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) take(Row{}, hid, i, h[i], 0.0f);
-    if (gat) {
+    for (int i = 0; i < NV; ++i) take(hid, i, x[i]);
+    if constexpr (GATE != NO_GATE) {
+        const T *gat = static_cast<const T *>(p.gate) + row * p.gate_stride;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) take(Row{}, gat, i, g[i], 0.0f);
+        for (int i = 0; i < NV; ++i) take(gat, i, g[i]);
     }
     if (p.weight) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) take(F32{}, p.weight, i, w2[i], 0.0f);
+        for (int i = 0; i < NV; ++i) take(p.weight, i, w2[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) w2[i] = 1.0f;
     }
+    __shared__ double s_first[NW], s_sum[NW], s_top[NW];
+    __shared__ int s_odd[NW];
+    extern __shared__ __align__(16) float s_v[];
 
-    __shared__ RowScratch<NW> s_row[RPW];
-    RowScratch<NW> &sc = s_row[RPW == 1 ? 0 : threadIdx.x / TPR];
-    double r1 = 1.0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) settle(i, o[i]);
+    double r1 = p.scale;
     if (p.post_weight) {
-        double ssq = 0.0, none = 0.0;
+        double ssq = 0.0;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) ssq = __builtin_fma((double)o[i][j], (double)o[i][j], ssq);
-        wave_sum_max(ssq, none);
+            for (int j = 0; j < 8; ++j) ssq = __builtin_fma((double)(float)o[i][j], (double)(float)o[i][j], ssq);
+        ssq = wave_sum(ssq);
         if constexpr (NW > 1) {
-            if ((tid & 63) == 0) sc.first[tid >> 6] = ssq;
+            if ((tid & 63) == 0) s_first[tid >> 6] = ssq;
             __syncthreads();
             ssq = 0.0;
 #pragma unroll
-            for (int i = 0; i < NW; ++i) ssq += sc.first[i];
+            for (int i = 0; i < NW; ++i) ssq += s_first[i];
         }
-        r1 = rsqrt_f64(__builtin_fma(ssq, p.inv_n, p.post_eps));
+        r1 *= rsqrt_f64(__builtin_fma(ssq, p.inv_n, p.post_eps));
     }
 
-    // The stream after the block, and the products of the next norm.
-    double hw[NV][8], ssq = 0.0, top = 0.0;
+    // The stream after the block, and the next norm's sums.
+    double ssq = 0.0, top = 0.0;
     float odd = 0.0f;
+    const Exp64 ex;
+    const bool silu = p.gate_act == GATE_SILU;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+        settle(i, x[i]);
+        settle(i, w1[i]);
+        settle(i, w2[i]);
+        if constexpr (GATE != NO_GATE) settle(i, g[i]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            double v = (double)o[i][j];
-            if (p.post_weight) v = v * r1 * (double)w1[i][j];
-            if (gat) {
-                const double x = (double)g[i][j];
-                double a = x;
-                if (p.gate_act) {
-                    a = sigmoid_f64(x);
-                    if (p.gate_act == GATE_SILU) a *= x;
-                }
-                v *= a;
+            double v = (double)(float)o[i][j] * (double)w1[i][j];   // exact
+            if constexpr (GATE == AS_IS) v *= (double)(float)g[i][j];
+            if constexpr (GATE == ACTIVATED) {
+                const float z = (float)g[i][j];
+                v *= ex.sigmoid(z) * (double)(silu ? z : 1.0f);
             }
-            const float sum = (float)__builtin_fma(p.scale, v, (double)h[i][j]);
-            h[i][j] = (float)(T)sum;
+            x[i][j] = (T)(float)__builtin_fma(v, r1, (double)(float)x[i][j]);
+            const double h = (double)(float)x[i][j];
+            ssq = __builtin_fma(h, h, ssq);
+            top = max_abs(top, h * (double)w2[i][j]);
+            odd = __builtin_fmaf(w2[i][j], 0.0f, odd);
         }
-        if (!live) continue;
-        if constexpr (VEC) {
-            if (at(i, 0) < n) store8<TY>(ho + at(i, 0), h[i]);
+        const int e = at(i), over = e + 8 - n;
+        if (e >= n) continue;
+        if (over <= 0) {
+            __builtin_memcpy(ho + e, &x[i], sizeof x[i]);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (at(i, j) < n) ho[at(i, j)] = (T)h[i][j];
+                if (j + over < 8) ho[e + j] = x[i][j];
         }
     }
     if (!p.weight) return;   // the same for every thread
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const double x = VEC ? (double)h[i][j] : at(i, j) < n ? (double)h[i][j] : 0.0;
-            hw[i][j] = x * (double)w2[i][j];
-            ssq = __builtin_fma(x, x, ssq);
-            odd = __builtin_fmaf(w2[i][j], 0.0f, odd);
-            top = fmax(top, fabs(hw[i][j]));
-        }
-    }
     wave_sum_max(ssq, top);
     bool any_odd = __ballot(odd != odd) != 0;
     if constexpr (NW > 1) {
-        if ((tid & 63) == 0) sc.sum[tid >> 6] = ssq, sc.top[tid >> 6] = top, sc.odd[tid >> 6] = any_odd;
+        if ((tid & 63) == 0) s_sum[tid >> 6] = ssq, s_top[tid >> 6] = top, s_odd[tid >> 6] = any_odd;
         __syncthreads();
         ssq = 0.0, top = 0.0, any_odd = false;
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
-            ssq += sc.sum[i];
-            top = fmax(top, sc.top[i]);
-            any_odd |= sc.odd[i] != 0;
+            ssq += s_sum[i];
+            top = fmax(top, s_top[i]);
+            any_odd |= s_odd[i] != 0;
         }
     }
     const double r = rsqrt_f64(__builtin_fma(ssq, p.inv_n, p.eps));
@@ -168,82 +180,92 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(BlockNormA
             scale = 0.0f;
         else
             to_q = r * reciprocal_of(scale);
-        if (tid == 0 && live) p.scales[rr] = scale;
+        if (tid == 0) p.scales[row] = scale;
     }
     const bool blank = to_q == 0.0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        extern __shared__ __align__(16) float s_v[];
-        if (!live) continue;
-        if constexpr (VEC) {
-            const int e = at(i, 0);
-            if (e >= n) continue;
-            if (p.q) {
-                uint32_t q[2] = {0, 0};
+        const int e = at(i), over = e + 8 - n;
+        if (e >= n) continue;
+        double hw[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) q[j >> 2] |= (uint32_t)(nearest_of_product(hw[i][j], to_q) & 0xff) << (8 * (j & 3));
-                const uint2 word = blank ? make_uint2(0, 0) : make_uint2(q[0], q[1]);
-                __builtin_memcpy(p.q + rr * p.q_stride + e, &word, sizeof word);
+        for (int j = 0; j < 8; ++j) hw[j] = (double)(float)x[i][j] * (double)w2[i][j];
+        if (p.q) {
+            uint32_t q[2] = {0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[j >> 2] |= (uint32_t)(nearest_of_product(hw[j], to_q) & 0xff) << (8 * (j & 3));
+            const uint2 word = blank ? make_uint2(0, 0) : make_uint2(q[0], q[1]);
+            int8_t *to = p.q + row * p.q_stride + e;
+            if (over <= 0) {
+                __builtin_memcpy(to, &word, sizeof word);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j + over < 8) to[j] = (int8_t)((j < 4 ? word.x : word.y) >> (8 * (j & 3)));
             }
-            if (p.y || p.q8k) {
-                float v[8];
+        }
+        if (p.y || p.q8k) {
+            float v[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = (float)(hw[i][j] * r);
-                if (p.y && p.y_type == T_F32)
-                    store8<T_F32>(static_cast<float *>(p.y) + rr * p.y_stride + e, v);
-                else if (p.y && p.y_type == T_F16)
-                    store8<T_F16>(static_cast<_Float16 *>(p.y) + rr * p.y_stride + e, v);
-                else if (p.y)
-                    store8<T_BF16>(static_cast<__bf16 *>(p.y) + rr * p.y_stride + e, v);
-                if (TPR > 64 && p.q8k) {
-                    *reinterpret_cast<float4 *>(s_v + e) = make_float4(v[0], v[1], v[2], v[3]);
-                    *reinterpret_cast<float4 *>(s_v + e + 4) = make_float4(v[4], v[5], v[6], v[7]);
-                }
-            }
-        } else {
+            for (int j = 0; j < 8; ++j) v[j] = (float)(hw[j] * r);
+            auto put = [&](auto ty) {
+                using Y = row_t<decltype(ty)::value>;
+                Y *to = static_cast<Y *>(p.y) + row * p.y_stride + e;
+                if (over <= 0) {
+                    store8<decltype(ty)::value>(to, v);
+                } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int e = at(i, j);
-                if (e >= n) continue;
-                if (p.q) p.q[rr * p.q_stride + e] = (int8_t)(blank ? 0 : nearest_of_product(hw[i][j], to_q));
-                if (p.y) {
-                    const float v = (float)(hw[i][j] * r);
-                    if (p.y_type == T_F32)
-                        static_cast<float *>(p.y)[rr * p.y_stride + e] = v;
-                    else if (p.y_type == T_F16)
-                        static_cast<_Float16 *>(p.y)[rr * p.y_stride + e] = (_Float16)v;
-                    else
-                        static_cast<__bf16 *>(p.y)[rr * p.y_stride + e] = (__bf16)v;
+                    for (int j = 0; j < 8; ++j)
+                        if (j + over < 8) to[j] = (Y)v[j];
                 }
+            };
+            if (p.y && p.y_type == T_F32)
+                put(std::integral_constant<int, T_F32>());
+            else if (p.y && p.y_type == T_F16)
+                put(std::integral_constant<int, T_F16>());
+            else if (p.y)
+                put(std::integral_constant<int, T_BF16>());
+            if (TPR > 64 && p.q8k) {   // n is a multiple of 256
+                *reinterpret_cast<float4 *>(s_v + e) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4 *>(s_v + e + 4) = make_float4(v[4], v[5], v[6], v[7]);
             }
         }
     }
-    if constexpr (VEC && TPR > 64) {   // Q8_K rows are multiples of 256
+    if constexpr (TPR > 64) {
         if (p.q8k) {
-            extern __shared__ __align__(16) float s_v[];
             __syncthreads();
             const int nb = n / 256;
             for (int b0 = (tid >> 6) * 4; b0 < nb; b0 += NW * 4)
-                quantize_blocks_wave(s_v, p.q8k + rr * (long long)nb * 292, b0, nb);
+                quantize_blocks_wave(s_v, p.q8k + row * (long long)nb * 292, b0, nb);
         }
     }
 }
 
-template <int TY, bool VEC>
-hipError_t launch_form(const BlockNormArgs &a, hipStream_t s) {
-    // Forms by the row's length, as the norm's.
-    const size_t lds = a.q8k ? (size_t)a.n * 4 : 0;
-    if (a.n <= 512 && !a.q8k)
-        hipLaunchKernelGGL((k_block_norm<TY, 64, 1, VEC>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a);
-    else if (a.n <= 2048)
-        hipLaunchKernelGGL((k_block_norm<TY, 256, 1, VEC>), dim3((unsigned)a.rows), dim3(256), lds, s, a);
-    else if (a.n <= 4096)
-        hipLaunchKernelGGL((k_block_norm<TY, 256, 2, VEC>), dim3((unsigned)a.rows), dim3(256), lds, s, a);
-    else if (a.n <= 8192)
-        hipLaunchKernelGGL((k_block_norm<TY, 512, 2, VEC>), dim3((unsigned)a.rows), dim3(512), lds, s, a);
-    else
-        hipLaunchKernelGGL((k_block_norm<TY, 1024, 2, VEC>), dim3((unsigned)a.rows), dim3(1024), lds, s, a);
+template <int TY, int GATE, int TPR, int NV>
+hipError_t launch_rows(const BlockNormArgs &a, hipStream_t s) {
+    constexpr int RPW = TPR < 256 ? 256 / TPR : 1;
+    hipLaunchKernelGGL((k_block_norm<TY, TPR, NV, GATE>), dim3((unsigned)((a.rows + RPW - 1) / RPW)), dim3(TPR * RPW),
+                       a.q8k ? (size_t)a.n * 4 : 0, s, a);
     return hipGetLastError();
+}
+
+// Two steps a thread keep more of a row's loads in flight than one step of twice as many
+// threads (4096 x 4096 bf16: 27.6 against 32.4 us).  Workgroups that went through rows
+// with the next row on its way and the weights kept had half the waves in the
+// registers that took, and were slower (32.0; with gates 52 against 46).
+template <int TY, int GATE>
+hipError_t launch_form(const BlockNormArgs &a, hipStream_t s) {
+    if (a.n <= 512 && !a.q8k) return launch_rows<TY, GATE, 64, 1>(a, s);
+    if (a.n <= 2048) return launch_rows<TY, GATE, 256, 1>(a, s);
+    if (a.n <= 4096) return launch_rows<TY, GATE, 256, 2>(a, s);
+    if (a.n <= 8192) return launch_rows<TY, GATE, 512, 2>(a, s);
+    return launch_rows<TY, GATE, 1024, 2>(a, s);
+}
+
+template <int TY>
+hipError_t launch_gate(const BlockNormArgs &a, hipStream_t s) {
+    if (!a.gate) return launch_form<TY, NO_GATE>(a, s);
+    return a.gate_act == GATE_AS_IS ? launch_form<TY, AS_IS>(a, s) : launch_form<TY, ACTIVATED>(a, s);
 }
 
 }  // namespace
@@ -251,11 +273,10 @@ hipError_t launch_form(const BlockNormArgs &a, hipStream_t s) {
 hipError_t launch_block_norm(const BlockNormArgs &a, hipStream_t s) {
     if (a.rows <= 0) return hipSuccess;
     if (a.n < 1 || a.n > BLOCK_NORM_MAX || a.rows > 0x7fffffff) return hipErrorInvalidValue;
-    const bool vec = a.n % 8 == 0;
     switch (a.type) {
-    case T_F32: return vec ? launch_form<T_F32, true>(a, s) : launch_form<T_F32, false>(a, s);
-    case T_F16: return vec ? launch_form<T_F16, true>(a, s) : launch_form<T_F16, false>(a, s);
-    case T_BF16: return vec ? launch_form<T_BF16, true>(a, s) : launch_form<T_BF16, false>(a, s);
+    case T_F32: return launch_gate<T_F32>(a, s);
+    case T_F16: return launch_gate<T_F16>(a, s);
+    case T_BF16: return launch_gate<T_BF16>(a, s);
     default: return hipErrorInvalidValue;
     }
 }

@@ -20,6 +20,8 @@
 // tokens.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "lbh_dev.h"
 #include "lbh_internal.h"
 #include "lbh_rows64.h"
@@ -30,7 +32,7 @@ namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 
-constexpr int WAVES = 8;
+constexpr int UP_WAVES = 4, WAVES = 8;   // of k_experts_up and k_experts_down
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *base, long long bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, (int)(uint32_t)bytes, 0x00020000);
@@ -56,32 +58,49 @@ struct Used {
 
 struct FewPairs {
     int id;            // lane p: pair p's expert, or -1
-    uint64_t first;    // lanes with an expert's first pair
     __device__ __forceinline__ FewPairs(const ExpertsArgs &a) {
         const int lane = threadIdx.x & 63;
         const uint32_t raw = lane < a.pairs ? a.ids[lane] : ~0u;
         id = raw < (uint32_t)a.n_experts ? (int)raw : -1;
-        bool seen = id < 0;
-        for (int j = 0; j < a.pairs; ++j) {
-            const int other = __builtin_amdgcn_readlane(id, j);
-            seen |= j < lane && other == id;
+    }
+    __device__ __forceinline__ Used of(int expert, uint64_t members) const {
+        const int lane = threadIdx.x & 63;
+        Used r;
+        r.expert = expert;
+        r.count = __builtin_popcountll(members);
+        // member lanes to the front; the others to lanes behind them
+        const int to = (members >> lane) & 1 ? lane_rank(members) : r.count + lane_rank(~members);
+        r.pairs = __builtin_amdgcn_ds_permute(4 * to, lane);
+        r.list = nullptr;
+        return r;
+    }
+    // The expert whose first pair is pair p; count 0: pair p is no expert's first.
+    __device__ __forceinline__ Used starting_at(int p) const {
+        const int expert = __builtin_amdgcn_readlane(id, p);
+        const uint64_t members = __ballot(id == expert);
+        if (expert < 0 || (int)__builtin_ctzll(members) != p) return {};
+        return of(expert, members);
+    }
+};
+
+// Every used expert in turn, by the place of its first pair.
+struct FewExperts : FewPairs {
+    uint64_t first;
+    __device__ __forceinline__ FewExperts(const ExpertsArgs &a) : FewPairs(a) {
+        uint64_t left = __ballot(id >= 0);
+        first = 0;
+        while (left) {
+            const int p = (int)__builtin_ctzll(left);
+            first |= 1ull << p;
+            left &= ~__ballot(id == __builtin_amdgcn_readlane(id, p));
         }
-        first = __ballot(!seen);
     }
     __device__ __forceinline__ int used() const { return __builtin_popcountll(first); }
     __device__ __forceinline__ Used at(int u) const {   // u < used()
         const int lane = threadIdx.x & 63;
         const uint64_t mine = __ballot(((first >> lane) & 1) && lane_rank(first) == u);
-        Used r;
-        r.expert = __builtin_amdgcn_readlane(id, (int)__builtin_ctzll(mine));
-        const uint64_t members = __ballot(id == r.expert);
-        r.count = __builtin_popcountll(members);
-        // member lanes to the front; the others to lanes behind them
-        const bool in = (members >> lane) & 1;
-        const int to = in ? lane_rank(members) : r.count + lane_rank(~members);
-        r.pairs = __builtin_amdgcn_ds_permute(4 * to, lane);
-        r.list = nullptr;
-        return r;
+        const int expert = __builtin_amdgcn_readlane(id, (int)__builtin_ctzll(mine));
+        return of(expert, __ballot(id == expert));
     }
 };
 
@@ -103,15 +122,7 @@ __device__ __forceinline__ int pair_at(const Used &u, int i) {
 }
 
 template <bool FEW>
-struct Pairs;
-template <>
-struct Pairs<true> : FewPairs {
-    using FewPairs::FewPairs;
-};
-template <>
-struct Pairs<false> : ManyPairs {
-    using ManyPairs::ManyPairs;
-};
+using Experts = std::conditional_t<FEW, FewExperts, ManyPairs>;
 
 // Sorts more than 64 pairs by expert.  The order of an expert's pairs among
 // themselves hangs on the LDS atomics, and no result hangs on it: each pair has
@@ -168,7 +179,7 @@ __device__ __forceinline__ void up_tiles(const ExpertsArgs &a, const Used &u, in
     auto ask = [&](int b, int k0) {
 #pragma unroll
         for (int d = 0; d < D; ++d) {
-            const int k = k0 + d * WAVES;
+            const int k = k0 + d * UP_WAVES;
             // past the last tile: out of the resource's range, zero
             wg[b][d] = load16<ONCE>(rw, lane * 16 + (k < kt ? k : 2 * kt) * 1024);
             wu[b][d] = load16<ONCE>(rw, lane * 16 + (k < kt ? kt + k : 2 * kt) * 1024);
@@ -176,7 +187,7 @@ __device__ __forceinline__ void up_tiles(const ExpertsArgs &a, const Used &u, in
 #pragma unroll
         for (int d = 0; d < D; ++d)
 #pragma unroll
-            for (int i = 0; i < NT; ++i) x[b][d][i] = load16<false>(rx, row[i] + (k0 + d * WAVES) * 64);
+            for (int i = 0; i < NT; ++i) x[b][d][i] = load16<false>(rx, row[i] + (k0 + d * UP_WAVES) * 64);
     };
     auto multiply = [&](int b) {
 #pragma unroll
@@ -188,21 +199,22 @@ __device__ __forceinline__ void up_tiles(const ExpertsArgs &a, const Used &u, in
             }
     };
     ask(0, wid);
-    for (int k = wid; k < kt; k += 2 * D * WAVES) {
-        ask(1, k + D * WAVES);
+    for (int k = wid; k < kt; k += 2 * D * UP_WAVES) {
+        ask(1, k + D * UP_WAVES);
         multiply(0);
-        ask(0, k + 2 * D * WAVES);
+        ask(0, k + 2 * D * UP_WAVES);
         multiply(1);
     }
 }
 
 template <int NT, int D, bool FEW, bool SHARED, bool ONCE>
 __device__ __forceinline__ void up_item(const ExpertsArgs &a, const Used &u, int base, int c0, __amdgpu_buffer_rsrc_t rw,
-                                        const float *gs, const float *us, v4i (*s_sum)[WAVES][64]) {
+                                        const float *gs, const float *us, v4i (*s_sum)[UP_WAVES][64]) {
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const __amdgpu_buffer_rsrc_t rx = rsrc(a.x, (long long)(a.n_tokens - 1) * a.x_stride + a.x_bytes);
     v4i g[NT] = {}, up[NT] = {};
     up_tiles<NT, D, FEW, SHARED, ONCE>(a, u, base, rw, rx, wid, g, up);
+    const Exp64 ex;
     // One value a thread: token tid / 16, channel tid % 16.
     const int n0 = (tid >> 4) & 15, c = tid & 15, ffn = SHARED ? a.ffn_s : a.ffn;
     const int from = n0 + 16 * (c >> 2);
@@ -214,15 +226,15 @@ __device__ __forceinline__ void up_item(const ExpertsArgs &a, const Used &u, int
         const int n = base + 16 * i + n0;
         int pair_of_row = 0;   // every lane takes part in the exchange
         if constexpr (!SHARED) pair_of_row = pair_at<FEW>(u, min(n, u.count - 1));
-        if (tid < 256 && n < u.count && c0 + c < ffn) {
+        if (n < u.count && c0 + c < ffn && tid < 256) {
             int sg = 0, su = 0;
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w)
+            for (int w = 0; w < UP_WAVES; ++w)
                 sg += s_sum[0][w][from][c & 3], su += s_sum[1][w][from][c & 3];
             const int p = SHARED ? n : pair_of_row, t = SHARED ? n : p / a.top_k;
             const double xs = (double)a.x_scales[t];
             const double vg = (double)sg * xs * (double)gs[c], vu = (double)su * xs * (double)us[c];
-            const float h = (float)(vg * sigmoid_f64(vg) * vu);
+            const float h = (float)(vg * ex.sigmoid(vg) * vu);
             if constexpr (SHARED)
                 a.h_s[(long long)t * a.h_s_pitch + c0 + c] = h;
             else
@@ -234,7 +246,7 @@ __device__ __forceinline__ void up_item(const ExpertsArgs &a, const Used &u, int
 // Tiles of 16 tokens at once: as many as the call's tokens can fill.
 template <int NT, bool FEW, bool SHARED, bool ONCE>
 __device__ __forceinline__ void up_expert(const ExpertsArgs &a, const Used &u, int c0, __amdgpu_buffer_rsrc_t rw,
-                                          const float *gs, const float *us, v4i (*s_sum)[WAVES][64]) {
+                                          const float *gs, const float *us, v4i (*s_sum)[UP_WAVES][64]) {
     int base = 0;
     if constexpr (NT == 4)
         for (; u.count - base > 32; base += 64) up_item<4, 1, FEW, SHARED, ONCE>(a, u, base, c0, rw, gs, us, s_sum);
@@ -243,10 +255,10 @@ __device__ __forceinline__ void up_expert(const ExpertsArgs &a, const Used &u, i
     for (; base < u.count; base += 16) up_item<1, 4, FEW, SHARED, ONCE>(a, u, base, c0, rw, gs, us, s_sum);
 }
 
-// grid: (channel groups, used experts + shared)
+// grid: (channel groups, the shared expert and one for each used expert or pair)
 template <int NT, bool FEW, bool ONCE>
-__global__ void __launch_bounds__(64 * WAVES, 4) k_experts_up(ExpertsArgs a) {
-    __shared__ v4i s_sum[2][WAVES][64];
+__global__ void __launch_bounds__(64 * UP_WAVES, 4) k_experts_up(ExpertsArgs a) {
+    __shared__ v4i s_sum[2][UP_WAVES][64];
     const int grp = blockIdx.x, c0 = grp * 16;
     const long long bytes = 2ll * a.kt_n * 1024;
     if (a.has_shared && blockIdx.y == 0) {
@@ -257,10 +269,16 @@ __global__ void __launch_bounds__(64 * WAVES, 4) k_experts_up(ExpertsArgs a) {
         return;
     }
     if (c0 >= a.ffn) return;
-    const Pairs<FEW> pairs(a);
     const int i = blockIdx.y - a.has_shared;
-    if (i >= pairs.used()) return;
-    const Used u = pairs.at(i);
+    Used u;
+    if constexpr (FEW) {   // a pair a row of the grid
+        u = FewPairs(a).starting_at(i);
+        if (!u.count) return;
+    } else {
+        const ManyPairs pairs(a);
+        if (i >= pairs.used()) return;
+        u = pairs.at(i);
+    }
     const ExpertI8 e = a.experts[u.expert];
     const float *s = e.up_scales + grp * 32;
     up_expert<NT, FEW, false, ONCE>(a, u, c0, rsrc(e.up + grp * bytes, bytes), s, s + 16, s_sum);
@@ -268,7 +286,50 @@ __global__ void __launch_bounds__(64 * WAVES, 4) k_experts_up(ExpertsArgs a) {
 
 // ------------------------------------------------------ int8 rows of h
 //
-// One row a workgroup, as lbh_quantize_i8_rows does it.  Rows up to 4096 elements stay
+// The scale of a row and its values, as lbh_quantize_i8_rows makes them.
+struct RowScale {
+    float scale;
+    double to_q;   // zero: a row of zeros, or one that is not finite
+    // top: the row's largest |value|, or not finite if any value is not
+    __device__ __forceinline__ explicit RowScale(float top) : to_q(0.0) {
+        scale = (float)((double)top * (1.0 / 127.0));
+        if (!(top < __builtin_inff()))
+            scale = __builtin_nanf("");
+        else if (scale < 0x1p-126f)
+            scale = 0.0f;
+        else
+            to_q = reciprocal_of(scale);
+    }
+    __device__ __forceinline__ uint2 values(const float (&x)[8]) const {
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j >> 2] |= (uint32_t)(nearest_of_quotient((double)x[j], to_q) & 0xff) << (8 * (j & 3));
+        return to_q == 0.0 ? make_uint2(0, 0) : make_uint2(w[0], w[1]);
+    }
+};
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = row16_max(v);
+#pragma unroll
+    for (int o = 16; o < 64; o *= 2) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+    return v;
+}
+// The bits of |v|, which are ordered as the values are, those that are not finite above the rest.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+// Elements e .. e + 7 of a row of n, zeros behind its end (rows start at multiples of 16 bytes).
+__device__ __forceinline__ void eight_of(const float *h, int e, int n, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    if (e + 8 <= n) {
+        const float4 lo = *reinterpret_cast<const float4 *>(h + e), hi = *reinterpret_cast<const float4 *>(h + e + 4);
+        v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+    } else if (e < n) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (e + j < n) v[j] = h[e + j];
+    }
+}
+
+// One row a workgroup.  Rows up to 4096 elements stay
 // in registers, longer ones are read twice.
 __global__ void __launch_bounds__(256) k_experts_quantize(ExpertsArgs a) {
     const int row = blockIdx.x, tid = threadIdx.x;
@@ -278,24 +339,13 @@ __global__ void __launch_bounds__(256) k_experts_quantize(ExpertsArgs a) {
     const float *h = shared ? a.h_s + (long long)(row - a.pairs) * a.h_s_pitch : a.h + (long long)row * a.h_pitch;
     int8_t *q = shared ? a.hq_s + (long long)(row - a.pairs) * kt * 64 : a.hq + (long long)row * kt * 64;
     constexpr int NV = 2;
-    auto take = [&](int i, float (&v)[8]) {   // rows are padded to 16 elements, what lies behind n is not read
-        const int e = (i * 256 + tid) * 8;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-        if (e + 8 <= n) {
-            const float4 lo = *reinterpret_cast<const float4 *>(h + e), hi = *reinterpret_cast<const float4 *>(h + e + 4);
-            v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
-        } else if (e < n) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (e + j < n) v[j] = h[e + j];
-        }
-    };
+    auto take = [&](int i, float (&v)[8]) { eight_of(h, (i * 256 + tid) * 8, n, v); };
     const int steps = (n + 2047) / 2048;
-    float v[NV][8], top = 0.0f, odd = 0.0f;
+    float v[NV][8];
+    uint32_t top = 0;
     auto account = [&](const float (&x)[8]) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j])), odd = __builtin_fmaf(x[j], 0.0f, odd);
+        for (int j = 0; j < 8; ++j) top = max(top, magnitude(x[j]));
     };
 #pragma unroll
     for (int i = 0; i < NV; ++i) take(i, v[i]);
@@ -306,30 +356,15 @@ __global__ void __launch_bounds__(256) k_experts_quantize(ExpertsArgs a) {
         take(i, x);
         account(x);
     }
-    double t64 = (double)top, none = 0.0;
-    wave_sum_max(none, t64);
-    __shared__ double s_top[4];
-    __shared__ int s_odd[4];
-    const bool any = __ballot(odd != odd) != 0;
-    if ((tid & 63) == 0) s_top[tid >> 6] = t64, s_odd[tid >> 6] = any;
+    __shared__ uint32_t s_top[4];
+    top = wave_max(top);
+    if ((tid & 63) == 0) s_top[tid >> 6] = top;
     __syncthreads();
-    t64 = fmax(fmax(s_top[0], s_top[1]), fmax(s_top[2], s_top[3]));
-    float scale = (float)(t64 * (1.0 / 127.0));
-    double to_q = 0.0;
-    if (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3])
-        scale = __builtin_nanf("");
-    else if (scale < 0x1p-126f)
-        scale = 0.0f;
-    else
-        to_q = reciprocal_of(scale);
-    if (tid == 0) a.h_scales[row] = scale;
+    const RowScale sc(__builtin_bit_cast(float, max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]))));
+    if (tid == 0) a.h_scales[row] = sc.scale;
     auto put = [&](int i, const float (&x)[8]) {
         const int e = (i * 256 + tid) * 8;
-        if (e >= n) return;
-        uint32_t w[2] = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j >> 2] |= (uint32_t)(nearest_of_quotient((double)x[j], to_q) & 0xff) << (8 * (j & 3));
-        *reinterpret_cast<uint2 *>(q + e) = to_q == 0.0 ? make_uint2(0, 0) : make_uint2(w[0], w[1]);
+        if (e < n) *reinterpret_cast<uint2 *>(q + e) = sc.values(x);
     };
 #pragma unroll
     for (int i = 0; i < NV; ++i) put(i, v[i]);
@@ -347,18 +382,22 @@ __global__ void __launch_bounds__(256) k_experts_quantize(ExpertsArgs a) {
 // one; the integer sums of a pair meet in LDS, where their order does not
 // count, and the sum over a token's slots is made from there in the slots' order.
 constexpr int DOWN_TILES = 8;
+constexpr int FUSED_STEPS = 2;   // of 512 elements a wave
 
-template <int OUT, bool FEW, bool ONCE>
+// FUSED (few pairs): the int8 rows are made here, by every workgroup for itself, in
+// place of a launch of k_experts_quantize; the first weights are on their way meanwhile.
+template <int OUT, bool FEW, bool ONCE, bool FUSED>
 __global__ void __launch_bounds__(64 * WAVES, 2) k_experts_down(ExpertsArgs a) {
-    extern __shared__ int s_sum[];   // [pairs + shared rows][16]
+    extern __shared__ __align__(16) int s_sum[];   // [rows][16]; FUSED: int8 rows (shared, then routed), scales
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = blockIdx.x, rows = a.pairs + (a.has_shared ? a.n_tokens : 0);
     for (int i = tid; i < rows * 4; i += 64 * WAVES) reinterpret_cast<v4i *>(s_sum)[i] = v4i{};
-    const Pairs<FEW> pairs(a);
-    const int used = pairs.used();
-    const int per = (a.kt_f + DOWN_TILES - 1) / DOWN_TILES;
-    const int first = a.has_shared ? (a.kt_fs + DOWN_TILES - 1) / DOWN_TILES : 0, units = first + used * per;
-    __syncthreads();
+    uint8_t *s_hq = reinterpret_cast<uint8_t *>(s_sum + rows * 16), *s_hq_r = s_hq + (a.has_shared ? a.n_tokens * a.kt_fs * 64 : 0);
+    float *s_scale = reinterpret_cast<float *>(s_hq_r + a.pairs * a.kt_f * 64);
+    (void)s_scale;
+    if constexpr (FUSED)
+        for (int i = tid; i < rows; i += 64 * WAVES) s_scale[i] = 0.0f;   // the rows' maxima
+    __syncthreads();   // the sums are zero
 
     struct Unit {
         Used u;
@@ -366,21 +405,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_experts_down(ExpertsArgs a) {
         int kt, k0;
         __amdgpu_buffer_rsrc_t rw, rh;
     };
-    auto unit = [&](int j) {
+    auto shared_unit = [&](int j) {
         Unit r;
-        r.shared = j < first;
-        const uint8_t *w;
-        if (r.shared) {
-            r.u = Used{0, a.n_tokens, 0, nullptr};
-            r.kt = a.kt_fs, r.k0 = j * DOWN_TILES, w = a.shared.down;
-            r.rh = rsrc(a.hq_s, (long long)a.n_tokens * a.kt_fs * 64);
-        } else {
-            const int i = (j - first) / per;
-            r.u = pairs.at(i);
-            r.kt = a.kt_f, r.k0 = ((j - first) - i * per) * DOWN_TILES, w = a.experts[r.u.expert].down;
-            r.rh = rsrc(a.hq, (long long)a.pairs * a.kt_f * 64);
-        }
-        r.rw = rsrc(w + (long long)grp * r.kt * 1024, (long long)r.kt * 1024);
+        r.u = Used{0, a.n_tokens, 0, nullptr};
+        r.shared = true, r.kt = a.kt_fs, r.k0 = j * DOWN_TILES;
+        r.rh = rsrc(a.hq_s, (long long)a.n_tokens * a.kt_fs * 64);
+        r.rw = rsrc(a.shared.down + (long long)grp * r.kt * 1024, (long long)r.kt * 1024);
         return r;
     };
     auto row_of = [&](const Unit &r, int base) {
@@ -393,6 +423,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_experts_down(ExpertsArgs a) {
             w[d] = load16<ONCE>(r.rw, lane * 16 + (r.k0 + d) * 1024);
     };
     auto tokens = [&](const Unit &r, int row, v4i (&x)[DOWN_TILES]) {
+        if constexpr (FUSED) {   // rows end at k tiles: the tiles behind, whose weights are zero, repeat the last
+            const uint8_t *from = (r.shared ? s_hq : s_hq_r) + row * (r.kt * 64) + 16 * (lane >> 4);
+#pragma unroll
+            for (int d = 0; d < DOWN_TILES; ++d) x[d] = *reinterpret_cast<const v4i *>(from + min(r.k0 + d, r.kt - 1) * 64);
+            return;
+        }
         const uint32_t at = (uint32_t)row * (uint32_t)(r.kt * 64) + 16 * (lane >> 4) + r.k0 * 64;
 #pragma unroll
         for (int d = 0; d < DOWN_TILES; ++d) x[d] = load16<false>(r.rh, at + d * 64);
@@ -408,6 +444,25 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_experts_down(ExpertsArgs a) {
         }
     };
     v4i w0[DOWN_TILES], w1[DOWN_TILES], x0[DOWN_TILES], x1[DOWN_TILES];
+    Unit r0, r1;
+    // The shared expert's units come first: their weights can be asked for before the ids are there.
+    const int per = (a.kt_f + DOWN_TILES - 1) / DOWN_TILES, first = a.has_shared ? (a.kt_fs + DOWN_TILES - 1) / DOWN_TILES : 0;
+    if (wid < first) {
+        r0 = shared_unit(wid);
+        ask(r0, w0);
+    }
+    const Experts<FEW> pairs(a);
+    const int units = first + pairs.used() * per;
+    auto unit = [&](int j) {
+        if (j < first) return shared_unit(j);
+        Unit r;
+        const int i = (j - first) / per;
+        r.u = pairs.at(i);
+        r.shared = false, r.kt = a.kt_f, r.k0 = ((j - first) - i * per) * DOWN_TILES;
+        r.rh = rsrc(a.hq, (long long)a.pairs * a.kt_f * 64);
+        r.rw = rsrc(a.experts[r.u.expert].down + (long long)grp * r.kt * 1024, (long long)r.kt * 1024);
+        return r;
+    };
     auto work = [&](const Unit &r, int row, const v4i (&w)[DOWN_TILES], const v4i (&x)[DOWN_TILES]) {
         add(r, 0, row, w, x);
         for (int base = 16; base < r.u.count; base += 16) {   // further tokens of the same weights
@@ -417,10 +472,59 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_experts_down(ExpertsArgs a) {
             add(r, base, other, w, more);
         }
     };
+    int row0 = 0, row1 = 0;
     if (wid < units) {
-        Unit r0 = unit(wid), r1;
-        int row0 = row_of(r0, 0), row1 = 0;
-        ask(r0, w0), tokens(r0, row0, x0);
+        if (wid >= first) {
+            r0 = unit(wid);
+            ask(r0, w0);
+        }
+        row0 = row_of(r0, 0);
+    }
+    if constexpr (FUSED) {
+        // 512 elements of a row a wave at once, all of them in registers between the maximum and the values.
+        const int per_s = a.has_shared ? (a.ffn_s + 511) / 512 : 0, per_r = (a.ffn + 511) / 512;
+        const int all_s = per_s * a.n_tokens, all = all_s + per_r * a.pairs;
+        float v[FUSED_STEPS][8];
+        auto place = [&](int i, int &row, int &e) {   // row: of the sums
+            const int j = wid + i * WAVES;
+            const bool sh = j < all_s;
+            const int per = sh ? per_s : per_r, k = sh ? j : j - all_s;
+            row = k / per + (sh ? a.pairs : 0), e = (k % per) * 512 + lane * 8;
+            return j < all && (sh || a.ids[row] < (uint32_t)a.n_experts);
+        };
+#pragma unroll
+        for (int i = 0; i < FUSED_STEPS; ++i) {
+            int row, e;
+            if (!place(i, row, e)) continue;
+            if (row >= a.pairs)
+                eight_of(a.h_s + (long long)(row - a.pairs) * a.h_s_pitch, e, a.ffn_s, v[i]);
+            else
+                eight_of(a.h + (long long)row * a.h_pitch, e, a.ffn, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < FUSED_STEPS; ++i) {
+            int row, e;
+            if (!place(i, row, e)) continue;
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max(top, magnitude(v[i][j]));
+            top = wave_max(top);
+            if (lane == 0) atomicMax(reinterpret_cast<uint32_t *>(s_scale) + row, top);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < FUSED_STEPS; ++i) {
+            int row, e;
+            if (!place(i, row, e)) continue;
+            const bool sh = row >= a.pairs;
+            if (e < (sh ? a.ffn_s : a.ffn))
+                *reinterpret_cast<uint2 *>((sh ? s_hq + (row - a.pairs) * (a.kt_fs * 64) : s_hq_r + row * (a.kt_f * 64)) + e) =
+                    RowScale(s_scale[row]).values(v[i]);
+        }
+        __syncthreads();
+    }
+    if (wid < units) {
+        tokens(r0, row0, x0);
         for (int j = wid; j < units; j += 2 * WAVES) {
             const bool next = j + WAVES < units;
             if (next) {
@@ -440,6 +544,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_experts_down(ExpertsArgs a) {
     }
     __syncthreads();
     using T = row_t<OUT>;
+    auto scale_of = [&](int row) { return FUSED ? (double)RowScale(s_scale[row]).scale : (double)a.h_scales[row]; };
     for (int i = tid; i < a.n_tokens * 16; i += 64 * WAVES) {
         const int t = i >> 4, c = grp * 16 + (i & 15);
         if (c >= a.n) continue;
@@ -448,11 +553,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_experts_down(ExpertsArgs a) {
             const int p = t * a.top_k + s;
             const uint32_t id = a.ids[p];
             if (id >= (uint32_t)a.n_experts) continue;
-            const double scale = (double)a.coefs[p] * (double)a.h_scales[p];
+            const double scale = (double)a.coefs[p] * scale_of(p);
             sum += (double)s_sum[p * 16 + (i & 15)] * (double)a.down_scales[(long long)id * a.down_pitch + c] * scale;
         }
         if (a.has_shared)
-            sum += (double)s_sum[(a.pairs + t) * 16 + (i & 15)] * (double)a.shared.down_scales[c] * (double)a.h_scales[a.pairs + t];
+            sum += (double)s_sum[(a.pairs + t) * 16 + (i & 15)] * (double)a.shared.down_scales[c] * scale_of(a.pairs + t);
         if (a.residual) sum += (double)static_cast<const T *>(a.residual)[(long long)t * a.residual_stride + c];
         static_cast<T *>(a.y)[(long long)t * a.y_stride + c] = (T)(float)sum;
     }
@@ -461,21 +566,20 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_experts_down(ExpertsArgs a) {
 template <bool FEW, bool ONCE>
 hipError_t launch_up(const ExpertsArgs &a, hipStream_t s) {
     const int widest = a.has_shared && a.ffn_s > a.ffn ? a.ffn_s : a.ffn;
-    const int used = a.pairs < a.n_experts ? a.pairs : a.n_experts;
+    const int used = FEW || a.pairs < a.n_experts ? a.pairs : a.n_experts;
     const dim3 grid((widest + 15) / 16, used + a.has_shared);
     if (a.n_tokens <= 16)
-        hipLaunchKernelGGL((k_experts_up<1, FEW, ONCE>), grid, dim3(64 * WAVES), 0, s, a);
+        hipLaunchKernelGGL((k_experts_up<1, FEW, ONCE>), grid, dim3(64 * UP_WAVES), 0, s, a);
     else if (a.n_tokens <= 32)
-        hipLaunchKernelGGL((k_experts_up<2, FEW, ONCE>), grid, dim3(64 * WAVES), 0, s, a);
+        hipLaunchKernelGGL((k_experts_up<2, FEW, ONCE>), grid, dim3(64 * UP_WAVES), 0, s, a);
     else
-        hipLaunchKernelGGL((k_experts_up<4, FEW, ONCE>), grid, dim3(64 * WAVES), 0, s, a);
+        hipLaunchKernelGGL((k_experts_up<4, FEW, ONCE>), grid, dim3(64 * UP_WAVES), 0, s, a);
     return hipGetLastError();
 }
 
-template <int OUT, bool FEW, bool ONCE>
-hipError_t launch_down(const ExpertsArgs &a, hipStream_t s) {
-    const int lds = (a.pairs + (a.has_shared ? a.n_tokens : 0)) * 64;
-    auto kernel = k_experts_down<OUT, FEW, ONCE>;
+template <int OUT, bool FEW, bool ONCE, bool FUSED>
+hipError_t launch_down(const ExpertsArgs &a, int lds, hipStream_t s) {
+    auto kernel = k_experts_down<OUT, FEW, ONCE, FUSED>;
     if (lds > 64 * 1024) {
         const hipError_t e =
             hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -485,22 +589,22 @@ hipError_t launch_down(const ExpertsArgs &a, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <bool FEW>
-hipError_t launch_layer(const ExpertsArgs &a, hipStream_t s) {
+template <bool FEW, bool FUSED>
+hipError_t launch_layer(const ExpertsArgs &a, int lds, hipStream_t s) {
+    hipError_t e;
     if constexpr (!FEW) {
         hipLaunchKernelGGL(k_experts_plan, dim3(1), dim3(1024), 0, s, a);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
+        if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    hipError_t e = launch_up<FEW, true>(a, s);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_experts_quantize, dim3(a.pairs + (a.has_shared ? a.n_tokens : 0)), dim3(256), 0, s, a);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    if ((e = launch_up<FEW, true>(a, s)) != hipSuccess) return e;
+    if constexpr (!FUSED) {
+        hipLaunchKernelGGL(k_experts_quantize, dim3(a.pairs + (a.has_shared ? a.n_tokens : 0)), dim3(256), 0, s, a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
     switch (a.y_type) {
-    case T_F32: return launch_down<T_F32, FEW, true>(a, s);
-    case T_F16: return launch_down<T_F16, FEW, true>(a, s);
-    case T_BF16: return launch_down<T_BF16, FEW, true>(a, s);
+    case T_F32: return launch_down<T_F32, FEW, true, FUSED>(a, lds, s);
+    case T_F16: return launch_down<T_F16, FEW, true, FUSED>(a, lds, s);
+    case T_BF16: return launch_down<T_BF16, FEW, true, FUSED>(a, lds, s);
     default: return hipErrorInvalidValue;
     }
 }
@@ -512,7 +616,14 @@ hipError_t launch_experts_i8(const ExpertsArgs &a, hipStream_t s) {
     if (a.n_tokens > EXPERTS_MAX_TOKENS || a.pairs != a.n_tokens * a.top_k || a.pairs < 1 || a.pairs > EXPERTS_MAX_PAIRS ||
         a.n_experts < 1 || a.n_experts > EXPERTS_MAX)
         return hipErrorInvalidValue;
-    return a.pairs <= 64 ? launch_layer<true>(a, s) : launch_layer<false>(a, s);
+    const int rows = a.pairs + (a.has_shared ? a.n_tokens : 0), sums = rows * 64;
+    if (a.pairs > 64) return launch_layer<false, false>(a, sums, s);
+    const long long steps = (long long)a.pairs * ((a.ffn + 511) / 512) + (long long)a.n_tokens * ((a.ffn_s + 511) / 512);
+    if (steps <= FUSED_STEPS * WAVES) {
+        const int values = 64 * (a.pairs * a.kt_f + (a.has_shared ? a.n_tokens * a.kt_fs : 0));
+        return launch_layer<true, true>(a, sums + values + rows * 4, s);
+    }
+    return launch_layer<true, false>(a, sums, s);
 }
 
 }  // namespace lbh

@@ -500,7 +500,10 @@ __global__ void __launch_bounds__(256, CW * TW > 8 ? 1 : 2) k_i8_tile(I8Args p) 
                         make_float4((float)acc[i][n][4 * q] * xs[n], (float)acc[i][n][4 * q + 1] * xs[n],
                                     (float)acc[i][n][4 * q + 2] * xs[n], (float)acc[i][n][4 * q + 3] * xs[n]);
             wave_sync();
-#pragma unroll
+            // With an activation the passes stay a loop: unrolled they outgrow the instruction cache, and
+            // the largest tile's sums went to memory for it (2048 x 13312 x 4096: 2380 us).
+            constexpr int UNROLL = EPI != EPI_NONE && !RES ? 1 : PASSES;
+#pragma unroll UNROLL
             for (int r = 0; r < 32; r += AT_ONCE) {
                 const int tl = r + lane / PER, t = (wt * TW + n) * 32 + tl;
                 const int tr = min(tl, 31);

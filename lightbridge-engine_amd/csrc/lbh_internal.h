@@ -332,15 +332,15 @@ struct RouteRowsArgs {
     const float *bias;          // mode 1
     const void *x;              // [n_tokens][hidden] of x_type
     long long x_stride;
-    double *part;               // workspace: [parts][n_tokens][n_experts]
+    double *part;               // workspace: [route_parts()][n_tokens][n_experts]
     uint32_t *ids;              // [n_tokens][top_k]
     float *coefs, *logits;      // logits optional, [n_tokens][n_experts]
     double weight_scale;
     int32_t n_tokens, n_experts, hidden, top_k, mode, x_type;
 };
-constexpr int ROUTE_SLICES = 8;
-// Slices whose sums wait in the workspace.
-constexpr int route_parts(long long n_tokens) { return n_tokens <= 64 ? ROUTE_SLICES : 1; }
+constexpr int ROUTE_SUMS = 4, ROUTE_PARTS = 8;
+// Sums of a logit that wait in the workspace.
+constexpr int route_parts(long long n_tokens) { return n_tokens <= 256 ? ROUTE_SUMS : 1; }
 hipError_t launch_route_rows(const RouteRowsArgs &a, hipStream_t s);
 
 // Batch selection: top-k of each token's finished logits (select_route).

@@ -11,16 +11,17 @@
 // number of rows.  (The router of lbh_router.hip reproduces a sequential 32-bit
 // sum instead, one token at a time, at 4096 dependent additions.)
 //
-// Products run on v_mfma_f64_16x16x4_f64, 16 experts x 16 rows.  The inner
-// dimension is cut into 8 slices, each over a workgroup's four waves; few rows
-// give every slice a workgroup of its own (its sums wait in the workspace), many
-// rows let a workgroup go through all eight, with the sums added in the same
-// order.  Bound: many rows by the matrix instruction (64 cycles for 1024 products), few by
+// Products run on v_mfma_f64_16x16x4_f64, 16 experts x 16 rows.  The inner dimension
+// is cut into 32 parts; the sums of eight parts are added in turn to one of four
+// sums, and these in turn to the logit, whoever does it: few rows spread the parts
+// over four workgroups of eight waves (their sums wait in the workspace), many rows
+// over the four waves of one.  Bound: many rows by the matrix instruction (64 cycles for 1024 products), few by
 // latency.
 #include <type_traits>
 
 #include "lbh_dev.h"
 #include "lbh_internal.h"
+#include "lbh_router.h"
 #include "lbh_rows64.h"
 
 namespace lbh {
@@ -29,61 +30,76 @@ namespace {
 
 typedef double v4d __attribute__((ext_vector_type(4)));
 
-template <int TY>
-__device__ __forceinline__ void load4(const row_t<TY> *p, float (&v)[4]) {
-    rvec<row_t<TY>, 4> a;
-    __builtin_memcpy(&a, p, sizeof a);   // at any address of its type
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = (float)a[j];
-}
-
-// grid: (16 experts, 16 rows, slices or 1)
-template <int TY>
-__global__ void __launch_bounds__(256) k_route_logits(RouteRowsArgs a) {
-    __shared__ double s_part[4][16][17];
+// The inner dimension's steps of 16 in 32 parts, eight for each of four sums.  MANY: a
+// wave makes a sum, part after part; else a workgroup does, a part a wave.  grid: (16
+// experts, 16 rows, 1 or the four sums)
+template <int TY, bool MANY>
+__global__ void __launch_bounds__(MANY ? 256 : 512) k_route_logits(RouteRowsArgs a) {
+    constexpr int WAVES = MANY ? ROUTE_SUMS : ROUTE_PARTS;
+    __shared__ double s_sum[WAVES][16][17];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int e = min((int)blockIdx.x * 16 + (lane & 15), a.n_experts - 1);
     const int t = min((int)blockIdx.y * 16 + (lane & 15), a.n_tokens - 1);
     const float4 *w = reinterpret_cast<const float4 *>(a.w) + e;
     const row_t<TY> *x = static_cast<const row_t<TY> *>(a.x) + (long long)t * a.x_stride;
     const int steps = a.hidden / 16, q = lane >> 4;
-    const int s0 = gridDim.z == 1 ? 0 : blockIdx.z, s1 = gridDim.z == 1 ? ROUTE_SLICES : s0 + 1;
-    double total = 0.0;
-    for (int s = s0; s < s1; ++s) {
-        const int part = s * 4 + wid;
-        int k = part * steps / (4 * ROUTE_SLICES);
-        const int end = (part + 1) * steps / (4 * ROUTE_SLICES);
-        v4d acc = {};
-        // 16 of the inner dimension a step: the lane's four are those of 4 q .. 4 q + 3, product m takes the m-th of each
-        auto ask = [&](int i, float4 &wv, float (&xv)[4]) {
-            i = min(i, steps - 1);
-            wv = w[(long long)(4 * i + q) * a.n_experts];
-            load4<TY>(x + 16 * i + 4 * q, xv);
-        };
-        auto multiply = [&](const float4 &wv, const float (&xv)[4]) {
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)wv.x, (double)xv[0], acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)wv.y, (double)xv[1], acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)wv.z, (double)xv[2], acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)wv.w, (double)xv[3], acc, 0, 0, 0);
-        };
-        constexpr int AHEAD = 8;   // a slice of 4096 in flight at once
-        float4 wv[AHEAD];
-        float xv[AHEAD][4];
-        for (; k < end; k += AHEAD) {
+    auto edge = [&](int part) { return part * steps / (ROUTE_SUMS * ROUTE_PARTS); };
+    int part = MANY ? wid * ROUTE_PARTS : blockIdx.z * ROUTE_PARTS + wid;
+    const int first = edge(part), last = edge(part + (MANY ? ROUTE_PARTS : 1));
+    v4d sum = {}, acc = {};
+    // 16 of the inner dimension a step: the lane's four are those of 4 q .. 4 q + 3, product m takes the m-th of each
+    constexpr int AHEAD = 4;
+    struct Step {
+        float4 w;
+        rvec<row_t<TY>, 4> x;
+    };
+    auto ask = [&](int k, Step (&v)[AHEAD]) {
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) ask(k + i, wv[i], xv[i]);
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i)
-                if (k + i < end) multiply(wv[i], xv[i]);
+        for (int i = 0; i < AHEAD; ++i) {
+            const int at = min(k + i, steps - 1);
+            v[i].w = w[(long long)(4 * at + q) * a.n_experts];
+            __builtin_memcpy(&v[i].x, x + 16 * at + 4 * q, sizeof v[i].x);   // at any address of its type
         }
-        // D: lane l holds row l % 16 and experts 4 i + l / 16
-        if (s > s0) __syncthreads();
+    };
+    // The end of the part that position `at` lies in (of narrow rows some parts are empty).
+    auto end_of = [&](int at) {
+        while (edge(part) <= at && edge(part) < last) ++part;
+        return edge(part);
+    };
+    int next = end_of(first);
+    auto multiply = [&](int k, const Step (&v)[AHEAD]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s_part[wid][lane & 15][4 * i + q] = acc[i];
-        __syncthreads();
-        const int r = tid >> 4, c = tid & 15;
-        total += s_part[0][r][c] + s_part[1][r][c] + s_part[2][r][c] + s_part[3][r][c];
+        for (int i = 0; i < AHEAD; ++i) {
+            if (k + i >= last) continue;
+            const float4 f = v[i].w;
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f.x, (double)(float)v[i].x[0], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f.y, (double)(float)v[i].x[1], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f.z, (double)(float)v[i].x[2], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f.w, (double)(float)v[i].x[3], acc, 0, 0, 0);
+            if (MANY && k + i + 1 == next) {   // the part is done
+                sum += acc;
+                acc = v4d{};
+                next = end_of(k + i + 1);
+            }
+        }
+    };
+    Step v0[AHEAD], v1[AHEAD];
+    ask(first, v0);
+    for (int k = first; k < last; k += 2 * AHEAD) {
+        ask(k + AHEAD, v1);
+        multiply(k, v0);
+        ask(k + 2 * AHEAD, v0);
+        multiply(k + AHEAD, v1);
     }
+    if (!MANY) sum = acc;
+    // D: lane l holds row l % 16 and experts 4 i + l / 16
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_sum[wid][lane & 15][4 * i + q] = sum[i];
+    __syncthreads();
+    if (tid >= 256) return;
+    double total = 0.0;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) total += s_sum[i][tid >> 4][tid & 15];
     const int to = blockIdx.y * 16 + (tid >> 4), te = blockIdx.x * 16 + (tid & 15);
     if (to < a.n_tokens && te < a.n_experts)
         a.part[((long long)blockIdx.z * a.n_tokens + to) * a.n_experts + te] = total;
@@ -94,47 +110,27 @@ __device__ __forceinline__ unsigned long long key_of(double v) {
     const unsigned long long b = __builtin_bit_cast(unsigned long long, v + 0.0);   // -0 is 0
     return b >> 63 ? ~b : b | 1ull << 63;
 }
-__device__ __forceinline__ unsigned long long wave_max_key(unsigned long long v) {
-    auto take = [&](unsigned long long o) { v = o > v ? o : v; };
-    auto dpp = [&](auto ctrl) {
-        constexpr int C = decltype(ctrl)::value;
-        return (unsigned long long)dpp_row<C>((uint32_t)(v >> 32)) << 32 | dpp_row<C>((uint32_t)v);
-    };
-    take(dpp(std::integral_constant<int, 0xB1>()));    // quad_perm [1, 0, 3, 2]
-    take(dpp(std::integral_constant<int, 0x4E>()));    // quad_perm [2, 3, 0, 1]
-    take(dpp(std::integral_constant<int, 0x141>()));   // row_half_mirror
-    take(dpp(std::integral_constant<int, 0x140>()));   // row_mirror
-    // one value a row of 16 lanes: four scalars
-    unsigned long long m = 0;
-#pragma unroll
-    for (int i = 0; i < 64; i += 16) {
-        const unsigned long long o = (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32 |
-                                     (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, i);
-        m = o > m ? o : m;
-    }
-    return m;
-}
-
 // A wave a row; lane l has experts l, l + 64, ...
 __global__ void __launch_bounds__(256) k_route_select(RouteRowsArgs a, int parts) {
     constexpr int SLOTS = 4;   // up to 256 experts
     const int lane = threadIdx.x & 63;
     const long long t = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t >= a.n_tokens) return;
-    double logit[SLOTS], weight[SLOTS];
+    const Exp64 ex;
+    double logit[SLOTS];
     unsigned long long key[SLOTS];
     float bias[SLOTS];
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k) {
         const int e = min(lane + 64 * k, a.n_experts - 1);
         bias[k] = a.mode ? a.bias[e] : 0.0f;
-        logit[k] = 0.0;
-        if (parts == 1) {
-            logit[k] += a.part[t * a.n_experts + e];
-        } else {
+        const double *part = a.part + t * a.n_experts + e;
+        double v[ROUTE_SUMS];   // one sum: the others are not added
 #pragma unroll
-            for (int s = 0; s < ROUTE_SLICES; ++s) logit[k] += a.part[(s * (long long)a.n_tokens + t) * a.n_experts + e];
-        }
+        for (int s = 0; s < ROUTE_SUMS; ++s) v[s] = part[s < parts ? s * (long long)a.n_tokens * a.n_experts : 0];
+        logit[k] = v[0];
+#pragma unroll
+        for (int s = 1; s < ROUTE_SUMS; ++s) logit[k] = s < parts ? logit[k] + v[s] : logit[k];
     }
     bool bad = false;
 #pragma unroll
@@ -142,8 +138,7 @@ __global__ void __launch_bounds__(256) k_route_select(RouteRowsArgs a, int parts
         const int e = lane + 64 * k;
         const bool some = e < a.n_experts;
         if (some && a.logits) a.logits[t * a.n_experts + e] = (float)logit[k];
-        weight[k] = a.mode ? 1.0 / (1.0 + exp(-logit[k])) : logit[k];
-        const double score = a.mode ? weight[k] + (double)bias[k] : logit[k];
+        const double score = a.mode ? ex.sigmoid(logit[k]) + (double)bias[k] : logit[k];
         bad |= some && !(fabs(score) < __builtin_inf() && fabs(logit[k]) < __builtin_inf());
         key[k] = some ? key_of(score) : 0;
     }
@@ -153,48 +148,62 @@ __global__ void __launch_bounds__(256) k_route_select(RouteRowsArgs a, int parts
         if (lane < a.top_k) ids[lane] = (uint32_t)lane, coefs[lane] = __builtin_nanf("");
         return;
     }
-    bool taken[SLOTS] = {};
-    double best = 0.0;   // the largest logit of a selection by logits
+    // Rounds of a maximum over the keys' upper words; where several have it, over their
+    // lower words, and the lowest id among equals.  Lane r keeps what round r chose.
+    int id = 0x7fffffff;
+    double chosen = 0.0;
     for (int r = 0; r < a.top_k; ++r) {
-        unsigned long long top = key[0];
+        uint32_t high = 0, low = 0;
 #pragma unroll
-        for (int k = 1; k < SLOTS; ++k) top = key[k] > top ? key[k] : top;
-        const unsigned long long m = wave_max_key(top);
-        if (r == 0) best = __builtin_bit_cast(double, m >> 63 ? m & ~(1ull << 63) : ~m);
+        for (int k = 0; k < SLOTS; ++k) high = max(high, (uint32_t)(key[k] >> 32));
+        high = wave_max_u32(high);
+        int many = 0;
+#pragma unroll
+        for (int k = 0; k < SLOTS; ++k) many += __builtin_popcountll(__ballot((uint32_t)(key[k] >> 32) == high));
+        if (many > 1) {
+#pragma unroll
+            for (int k = 0; k < SLOTS; ++k)
+                if ((uint32_t)(key[k] >> 32) == high) low = max(low, (uint32_t)key[k]);
+            low = wave_max_u32(low);
+        }
         bool found = false;
 #pragma unroll
-        for (int k = 0; k < SLOTS; ++k) {   // the lowest id among equals
-            const uint64_t equal = __ballot(key[k] == m);
-            if (!found && equal) {
-                found = true;
-                if (lane == (int)__builtin_ctzll(equal)) taken[k] = true, key[k] = 0;
-            }
+        for (int k = 0; k < SLOTS; ++k) {
+            const uint64_t equal = __ballot((uint32_t)(key[k] >> 32) == high && (many == 1 || (uint32_t)key[k] == low));
+            if (found || !equal) continue;   // the same for every lane
+            found = true;
+            const int from = (int)__builtin_ctzll(equal);
+            const uint64_t bits = __builtin_bit_cast(uint64_t, logit[k]);
+            const uint64_t l = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(bits >> 32), from) << 32 |
+                               (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bits, from);
+            if (lane == r) id = from + 64 * k, chosen = __builtin_bit_cast(double, l);
+            if (lane == from) key[k] = 0;
         }
     }
-    double sum = 0.0, none = 0.0;
-#pragma unroll
-    for (int k = 0; k < SLOTS; ++k) {
-        if (!a.mode) weight[k] = taken[k] ? exp(logit[k] - best) : 0.0;
-        if (taken[k]) sum += weight[k];
+    const bool mine = lane < a.top_k;
+    double weight;
+    if (a.mode) {
+        weight = ex.sigmoid(chosen);
+    } else {
+        double best = mine ? chosen : -__builtin_inf(), none = 0.0;
+        wave_sum_max(none, best);
+        const double x = fmax(chosen - best, -708.0);   // from there on its share of the sum is 0
+        weight = ex.exp(x, (float)x);
     }
-    wave_sum_max(sum, none);
+    double sum = wave_sum(mine ? weight : 0.0);
     if (a.mode) sum = fmax(sum, 0x1p-14);
     int at = 0;
-#pragma unroll
-    for (int k = 0; k < SLOTS; ++k) {
-        const uint64_t mask = __ballot(taken[k]);
-        const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-        if (taken[k]) {
-            ids[at + rank] = (uint32_t)(lane + 64 * k);
-            coefs[at + rank] = (float)(weight[k] / sum * a.weight_scale);
-        }
-        at += __builtin_popcountll(mask);
-    }
+    for (int r = 0; r < a.top_k; ++r) at += __builtin_amdgcn_readlane(id, r) < id;
+    if (mine) ids[at] = (uint32_t)id, coefs[at] = (float)(weight / sum * a.weight_scale);
 }
 
 template <int TY>
 hipError_t launch_logits(const RouteRowsArgs &a, int parts, hipStream_t s) {
-    hipLaunchKernelGGL((k_route_logits<TY>), dim3((a.n_experts + 15) / 16, (a.n_tokens + 15) / 16, parts), dim3(256), 0, s, a);
+    const dim3 grid((a.n_experts + 15) / 16, (a.n_tokens + 15) / 16, parts);
+    if (parts == 1)
+        hipLaunchKernelGGL((k_route_logits<TY, true>), grid, dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((k_route_logits<TY, false>), grid, dim3(512), 0, s, a);
     return hipGetLastError();
 }
 

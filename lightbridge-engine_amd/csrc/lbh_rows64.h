@@ -90,26 +90,68 @@ __device__ __forceinline__ void store8(row_t<TY> *p, const float (&v)[8]) {
     }
 }
 
-// 1 / (1 + exp(-g)) to some 2^-46 of itself: exp(x) = 2^n exp(f), |f| <= ln 2 / 2, by
-// the series up to f^11 (what is cut off is below 0.3466^12 / 12! = 2^-47), n ln 2 in two
-// parts.  The library's exp and division are exact to the last bit or so at more
-// than twice the instructions, which a row of gates would wait for.  Below g = -708
-// it is 0, as 1 / (1 + exp(-g)) is soon after.
-__device__ __forceinline__ double sigmoid_f64(double g) {
-    constexpr double LOG2E = 0x1.71547652b82fep+0, LN2_HI = 0x1.62e42fefa0000p-1, LN2_LO = 0x1.cf79abc9e3b3ap-40;
-    const double x = fmin(fmax(-g, -708.0), 708.0);
-    const double n = __builtin_rint(x * LOG2E);
-    const double f = __builtin_fma(n, -LN2_LO, __builtin_fma(n, -LN2_HI, x));
-    double e = 1.0 / 39916800.0;
-    constexpr double C[] = {1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0, 1.0 / 120.0,
-                            1.0 / 24.0,      1.0 / 6.0,      0.5,           1.0,          1.0};
+__device__ __forceinline__ double wave_sum(double v) {
+    v += dpp_f64<0xB1>(v);    // quad_perm [1, 0, 3, 2]
+    v += dpp_f64<0x4E>(v);    // quad_perm [2, 3, 0, 1]
+    v += dpp_f64<0x141>(v);   // row_half_mirror
+    v += dpp_f64<0x140>(v);   // row_mirror
 #pragma unroll
-    for (int i = 0; i < 11; ++i) e = __builtin_fma(e, f, C[i]);
-    const double d = 1.0 + __builtin_ldexp(e, (int)n);
-    double r = __builtin_amdgcn_rcp(d);
+    for (int o = 16; o < 64; o *= 2) v += shfl_xor_f64(v, o);
+    return v;
+}
+
+// The exponential and the sigmoid to some 2^-39 of themselves.  exp(x) = 2^n 2^f with
+// |f| <= 1/2 (n by a 32-bit rounding; the product with log2(e) in 64 bits), 2^f by a
+// polynomial of degree eight through the Chebyshev nodes (off by 2^-38.8 at most), the
+// reciprocal by the hardware's estimate and one step of third order.  The library's
+// exp and division cost more than twice the instructions, and a kernel of gated
+// rows is bound by instructions.  Below g = -708 the sigmoid is 0, as its formula in
+// 64 bits is from -745.
+struct Exp64 {
+    double c[8];
+    // The coefficients in scalar registers, where an instruction takes them as they are
+    // (as literals each costs two moves a use).
+    __device__ __forceinline__ Exp64()
+        : c{0x1.63b2d7971923fp-20, 0x1.00c0e4e15189cp-16, 0x1.4308c7183d6a2p-13, 0x1.5d877598350dep-10, 0x1.3b2ab70ad2565p-7, 0x1.c6b08da70cce3p-5, 0x1.ebfbdff82a734p-3, 0x1.62e42fef9cc69p-1} {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) r = __builtin_fma(r, __builtin_fma(-d, r, 1.0), r);
-    return g < -708.0 ? 0.0 : g != g ? g : r;
+        for (int i = 0; i < 8; ++i) asm("" : "+s"(c[i]));
+    }
+    __device__ __forceinline__ double sigmoid(float g) const {
+        const float x = __builtin_amdgcn_fmed3f(-g, -708.0f, 708.0f);
+        const double s = of((double)x, x);
+        return g < -708.0f ? 0.0 : g != g ? (double)g : s;
+    }
+    __device__ __forceinline__ double sigmoid(double g) const {
+        const double x = fmin(fmax(-g, -708.0), 708.0);
+        const double s = of(x, (float)x);
+        return g < -708.0 ? 0.0 : g != g ? g : s;
+    }
+
+    // exp(x), |x| <= 708; x32 is x to 32 bits.
+    __device__ __forceinline__ double exp(double x, float x32) const {
+        constexpr double LOG2E = 0x1.71547652b82fep+0;
+        const float n = __builtin_rintf(x32 * (float)LOG2E);
+        const double f = __builtin_fma(x, LOG2E, -(double)n);
+        double e = c[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) e = __builtin_fma(e, f, c[i]);
+        return __builtin_ldexp(__builtin_fma(e, f, 1.0), (int)n);
+    }
+
+private:
+    // 1 / (1 + exp(x)), |x| <= 708.
+    __device__ __forceinline__ double of(double x, float x32) const {
+        const double d = 1.0 + exp(x, x32);
+        const double r = __builtin_amdgcn_rcp(d), miss = __builtin_fma(-d, r, 1.0);
+        return __builtin_fma(r, __builtin_fma(miss, miss, miss), r);
+    }
+};
+
+// The larger of a and |b|: one instruction (fmax makes two, the first to quiet a NaN that
+// cannot be there).  NaN in b leaves a.
+__device__ __forceinline__ double max_abs(double a, double b) {
+    asm("v_max_f64 %0, %0, |%1|" : "+v"(a) : "v"(b));
+    return a;
 }
 
 }  // namespace
