@@ -94,7 +94,13 @@ float estimate(const I8Args &a, const Form &f) {
         float weights = bytes / 5.2e6f;
         if (a.n_tokens <= 64 * f.tw)
             weights = rounds * k * (float)f.cw * 4096 / (f.cw == 1 && rounds == 1 ? 17.5e3f : 25.5e3f);
-        return 2.0f + wait + fmaxf(rounds * (f.fixed + f.step * k), weights);
+        // An activation's work behind the products, which the largest tile, alone on its CU,
+        // shows twice as much of.  Measured over the product alone: 2048 x 13312 T44 111 us, none
+        // 116, silu 130, gelu 135, T22 124, 128, 132, 133; gated 1024 x 13312 T44 117, silu 122, T22 128, 130.
+        const float each = a.act == ACT_GELU ? 0.8e-4f : a.act >= ACT_SILU ? 0.6e-4f : 0.3e-4f;
+        const float outputs = (float)(f.cw * f.tw) * 4096 / (a.gated ? 2 : 1);
+        const float after = a.epilogue ? rounds * outputs * (f.cw == 4 ? 2 * each : each) : 0.0f;
+        return 2.0f + wait + after + fmaxf(rounds * (f.fixed + f.step * k), weights);
     }
     // Two to four workgroups share a CU and its L1, which takes 19.5 ns for a KiB.
     // Tokens come from L2 beside the weights, each workgroup's its own: 17 TB/s

@@ -57,20 +57,27 @@ __device__ __forceinline__ void store_row(row_t<OUT> *p, const float (&v)[V]) {
 
 // The scales of channels c .. c + V - 1 (c % V == 0, V <= 16; channels past the last
 // one have the zeros that fill its group, or those of the last group).
-template <bool GATED, int EPI, int V>
+template <bool GATED, int V>
 struct ChannelScales {
     float g[V], u[GATED ? V : 1];
-    float bias[EPI ? V : 1], up_bias[EPI && GATED ? V : 1];   // the caller's, any address: one at a time
     __device__ __forceinline__ ChannelScales(const I8Args &p, int c) {
         const int grp = min(c >> 4, (p.rows - 1) >> 4);
         const float *s = p.ws + (GATED ? 32 : 16) * grp + (c & 15);
         load_row<T_F32, V>(s, g);
         if constexpr (GATED) load_row<T_F32, V>(s + 16, u);
+    }
+};
+
+// Their biases (the caller's, at any address: one at a time), where the epilogue has them.
+template <bool GATED, int EPI, int V>
+struct ChannelBiases {
+    float g[EPI ? V : 1], u[EPI && GATED ? V : 1];
+    __device__ __forceinline__ ChannelBiases(const I8Args &p, int c) {
         if constexpr (EPI != EPI_NONE) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                bias[j] = p.bias ? p.bias[min(c + j, p.rows - 1)] : 0.0f;
-                if constexpr (GATED) up_bias[j] = p.up_bias ? p.up_bias[min(c + j, p.rows - 1)] : 0.0f;
+                g[j] = p.bias ? p.bias[min(c + j, p.rows - 1)] : 0.0f;
+                if constexpr (GATED) u[j] = p.up_bias ? p.up_bias[min(c + j, p.rows - 1)] : 0.0f;
             }
         }
     }
@@ -106,38 +113,65 @@ __device__ __forceinline__ float sigmoid_of(float g) {
 }
 __device__ __forceinline__ float swiglu(float g, float u) { return g * sigmoid_of(g) * u; }
 
+// The same for outputs of 16 bits, without the steps that matter to 32: off by some 8 *
+// 2^-24 and 2 * 2^-24 |g|, where the output's rounding is 2^-12 or 2^-9.  (With them the
+// activations of 2048 x 13312 took 5 us more.)
+__device__ __forceinline__ float sigmoid_of_16(float g) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(-g, -104.0f, 88.0f) * 0x1.715476p+0f));
+}
+
 // x times the normal distribution's function of x.  Its lower tail is exp(-a^2 / 2)
 // times a smooth function of a = |x|, here t P(t) with t = 1 / (1 + 0.35 a) and P of degree
 // eight, fitted for the least relative error over 0 <= a <= 14 (3.2e-8); a^2 goes into
-// the exponential in two parts.  Past a = 13.2 the tail is 0 (what is right is below
-// 2^-126 there, and up to 2^-122 |x| is given up).
+// the exponential in two parts (WIDE: an output of 32 bits).  Past a = 13.2 the tail is 0
+// (what is right is below 2^-126 there, and up to 2^-122 |x| is given up).
+template <bool WIDE>
 __device__ __forceinline__ float normal_gate(float x) {
     const float a = fminf(fabsf(x), 14.0f);
-    const float t = reciprocal_step(__builtin_fmaf(0.35f, a, 1.0f));
+    const float d = __builtin_fmaf(0.35f, a, 1.0f);
+    const float t = WIDE ? reciprocal_step(d) : __builtin_amdgcn_rcpf(d);
     float p = -0x1.dd86ep-6f;
     constexpr float C[] = {0x1.26daap-3f, -0x1.05d9f4p-2f, 0x1.45fd1ap-3f, -0x1.7aa1a6p-6f, 0x1.b02928p-4f, 0x1.ead5dep-4f, 0x1.1e6fe6p-3f, 0x1.1df1d4p-3f};
 #pragma unroll
     for (int i = 0; i < 8; ++i) p = __builtin_fmaf(p, t, C[i]);
-    const float s = a * a, s_lo = __builtin_fmaf(a, a, -s);
-    float e = exp_of(-0.5f * s);
-    e = __builtin_fmaf(e, -0.5f * s_lo, e);
+    const float s = a * a;
+    float e;
+    if constexpr (WIDE) {
+        e = exp_of(-0.5f * s);
+        e = __builtin_fmaf(e, -0.5f * __builtin_fmaf(a, a, -s), e);
+    } else {
+        e = __builtin_amdgcn_exp2f(s * -0x1.715476p-1f);
+    }
     const float tail = p * t * e;
     return x * (x > 0.0f ? 1.0f - tail : tail);
 }
 
-// The activation of a product's epilogue (I8Args::act).
-template <int EPI>
-__device__ __forceinline__ float activate(const I8Args &p, float x) {
-    if constexpr (EPI == EPI_NORMAL) return normal_gate(x);
-    if (p.act <= ACT_RELU2) {
-        // a comparison, not fmaxf: NaN stays NaN
-        const float pos = x < 0.0f ? 0.0f : x;
-        return p.act == ACT_NONE ? x : p.act == ACT_RELU ? pos : pos * pos;
+// The activation of a product's epilogue (I8Args::act) on V values.
+template <int EPI, bool WIDE, int V>
+__device__ __forceinline__ void activate(const I8Args &p, float (&v)[V]) {
+    if constexpr (EPI == EPI_NORMAL) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = normal_gate<WIDE>(v[j]);
+        return;
     }
-    // x / (1 + exp(-z)): z = x, or sqrt(8 / pi) (x + 0.044715 x^3), whose x / 2 (1 + tanh(z / 2)) this is
-    float z = x;
-    if (p.act == ACT_GELU_TANH) z = x * __builtin_fmaf(x * x, 0x1.2444f2p-4f, 0x1.988454p+0f);
-    return x * sigmoid_of(z);
+    if (p.act == ACT_NONE) return;
+    if (p.act <= ACT_RELU2) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float pos = v[j] < 0.0f ? 0.0f : v[j];   // a comparison, not fmaxf: NaN stays NaN
+            v[j] = p.act == ACT_RELU ? pos : pos * pos;
+        }
+        return;
+    }
+    // v / (1 + exp(-z)): z = v, or sqrt(8 / pi) (v + 0.044715 v^3), whose v / 2 (1 + tanh(z / 2)) this is
+    const bool tanh = p.act == ACT_GELU_TANH;
+    constexpr float C1 = 0x1.988454p+0f, C3 = 0x1.2444f2p-4f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        float z = v[j];
+        if (tanh) z *= __builtin_fmaf(v[j] * v[j], C3, C1);
+        v[j] *= WIDE ? sigmoid_of(z) : sigmoid_of_16(z);
+    }
 }
 
 // Channels c .. c + V - 1 of token t from their sums times the token's scale
@@ -145,21 +179,26 @@ __device__ __forceinline__ float activate(const I8Args &p, float x) {
 // are aligned to 16 bytes, and the residual's values (if any) are at hand.
 template <int OUT, bool GATED, int EPI, bool INSIDE, int V>
 __device__ __forceinline__ void finish(const I8Args &p, int t, int c, const float (&sum)[V], const float (&up)[V],
-                                       const ChannelScales<GATED, EPI, V> &ws,
+                                       const ChannelScales<GATED, V> &ws, const ChannelBiases<GATED, EPI, V> &bias,
                                        const rvec<row_t<OUT>, V> *residual = nullptr) {
     if (!INSIDE && c >= p.rows) return;
     float v[V];
+    if constexpr (EPI != EPI_NONE) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        v[j] = sum[j] * ws.g[j];
-        if constexpr (EPI != EPI_NONE) {
-            v[j] = activate<EPI>(p, v[j] + ws.bias[j]);
-            if constexpr (GATED) v[j] *= up[j] * ws.u[j] + ws.up_bias[j];
-            v[j] *= p.scale;
-        } else if constexpr (GATED) {
-            v[j] = swiglu(v[j], up[j] * ws.u[j]);
+        for (int j = 0; j < V; ++j) v[j] = sum[j] * ws.g[j] + bias.g[j];
+        activate<EPI, OUT == T_F32, V>(p, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if constexpr (GATED) v[j] *= up[j] * ws.u[j] + bias.u[j];
+            v[j] = rounded(v[j] * p.scale);
         }
-        v[j] = rounded(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            v[j] = sum[j] * ws.g[j];
+            if constexpr (GATED) v[j] = swiglu(v[j], up[j] * ws.u[j]);
+            v[j] = rounded(v[j]);
+        }
     }
     row_t<OUT> *y = static_cast<row_t<OUT> *>(p.y) + (long long)t * p.y_stride + c;
     if constexpr (INSIDE) {
@@ -299,12 +338,13 @@ __global__ void __launch_bounds__(64 * ST_WAVES, 4) k_i8_stream(I8Args p) {
             if constexpr (GATED) up += sums(w)[((2 * r + 1) * TT + i) * 64 + lane];
         }
         const int t = 16 * i + (lane & 15), c = (bx * R + r) * 16 + 4 * (lane >> 4);
-        const ChannelScales<GATED, EPI, 4> ws(p, c);
+        const ChannelScales<GATED, 4> ws(p, c);
+        const ChannelBiases<GATED, EPI, 4> bias(p, c);
         const float xs = p.xs[t0 + min(t, nt - 1)];
         float u[4], v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = (float)sum[e] * xs, u[e] = (float)up[e] * xs;
-        if (t < nt) finish<OUT, GATED, EPI, false, 4>(p, t0 + t, c, v, u, ws);
+        if (t < nt) finish<OUT, GATED, EPI, false, 4>(p, t0 + t, c, v, u, ws, bias);
     }
 }
 
@@ -354,7 +394,7 @@ __global__ void __launch_bounds__(256, CW * TW > 8 ? 1 : 2) k_i8_tile(I8Args p) 
     constexpr int PER = WIDE / V, AT_ONCE = 64 / PER;             // lanes a token, tokens a pass
     const int lc = (lane % PER) * V;
     const int c = (GATED ? g0 / 2 : g0) * 16 + wc * WIDE + lc;
-    const ChannelScales<GATED, EPI, V> ws(p, c);
+    const ChannelScales<GATED, V> ws(p, c);
     float xs[TW];
 #pragma unroll
     for (int n = 0; n < TW; ++n) xs[n] = p.xs[t0 + min((wt * TW + n) * 32 + (lane & 31), nt - 1)];
@@ -471,6 +511,7 @@ __global__ void __launch_bounds__(256, CW * TW > 8 ? 1 : 2) k_i8_tile(I8Args p) 
     // straight from D, 16 bytes a token and line, the stores took a quarter of the
     // kernel).
     static_assert(32 * ROW * 4 == W, "a wave's part is a buffer of weights");
+    const ChannelBiases<GATED, EPI, V> bias(p, c);   // (not before the products, whose registers they would take)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -502,7 +543,7 @@ __global__ void __launch_bounds__(256, CW * TW > 8 ? 1 : 2) k_i8_tile(I8Args p) 
             wave_sync();
             // With an activation the passes stay a loop: unrolled they outgrow the instruction cache, and
             // the largest tile's sums went to memory for it (2048 x 13312 x 4096: 2380 us).
-            constexpr int UNROLL = EPI != EPI_NONE && !RES ? 1 : PASSES;
+            constexpr int UNROLL = EPI != EPI_NONE && !RES && CW == 4 ? 1 : PASSES;
 #pragma unroll UNROLL
             for (int r = 0; r < 32; r += AT_ONCE) {
                 const int tl = r + lane / PER, t = (wt * TW + n) * 32 + tl;
@@ -519,7 +560,7 @@ __global__ void __launch_bounds__(256, CW * TW > 8 ? 1 : 2) k_i8_tile(I8Args p) 
                 }
                 const bool mine = (64 % PER == 0 || lane < PER * AT_ONCE) && (32 % AT_ONCE == 0 || tl < 32);
                 if (mine && (INSIDE || t < nt))
-                    finish<OUT, GATED, EPI, INSIDE, V>(p, t0 + t, c, g, u, ws, RES ? &res[r / AT_ONCE] : nullptr);
+                    finish<OUT, GATED, EPI, INSIDE, V>(p, t0 + t, c, g, u, ws, bias, RES ? &res[r / AT_ONCE] : nullptr);
             }
             wave_sync();
             __builtin_amdgcn_sched_barrier(0);   // the next tokens' residuals do not need registers yet
