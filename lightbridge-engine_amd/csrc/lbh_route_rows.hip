@@ -30,7 +30,7 @@ namespace {
 
 typedef double v4d __attribute__((ext_vector_type(4)));
 
-// The inner dimension's steps of 16 in 32 parts, eight for each of four sums.  MANY: a
+// The inner dimension's units of 64 in 32 parts, eight for each of four sums.  MANY: a
 // wave makes a sum, part after part; else a workgroup does, a part a wave.  grid: (16
 // experts, 16 rows, 1 or the four sums)
 template <int TY, bool MANY>
@@ -42,24 +42,23 @@ __global__ void __launch_bounds__(MANY ? 256 : 512) k_route_logits(RouteRowsArgs
     const int t = min((int)blockIdx.y * 16 + (lane & 15), a.n_tokens - 1);
     const float4 *w = reinterpret_cast<const float4 *>(a.w) + e;
     const row_t<TY> *x = static_cast<const row_t<TY> *>(a.x) + (long long)t * a.x_stride;
-    const int steps = a.hidden / 16, q = lane >> 4;
-    auto edge = [&](int part) { return part * steps / (ROUTE_SUMS * ROUTE_PARTS); };
+    const int units = a.hidden / 64, q = lane >> 4;
+    auto edge = [&](int part) { return part * units / (ROUTE_SUMS * ROUTE_PARTS); };
     int part = MANY ? wid * ROUTE_PARTS : blockIdx.z * ROUTE_PARTS + wid;
     const int first = edge(part), last = edge(part + (MANY ? ROUTE_PARTS : 1));
     v4d sum = {}, acc = {};
-    // 16 of the inner dimension a step: the lane's four are those of 4 q .. 4 q + 3, product m takes the m-th of each
-    constexpr int AHEAD = 4;
-    struct Step {
-        float4 w;
-        rvec<row_t<TY>, 4> x;
+    // A unit is 64 of the inner dimension.  The lane's sixteen are those of 16 q .. 16 q + 15, so that a row's bytes are
+    // read a whole line at a time; product i takes the i-th of each.  (Four of each 16, a quarter of the line, had the
+    // lines come from L2 four times: 1000 rows 44 us.)
+    struct Unit {
+        float4 w[4];
+        rvec<row_t<TY>, 16> x;
     };
-    auto ask = [&](int k, Step (&v)[AHEAD]) {
+    auto ask = [&](int k, Unit &v) {
+        const int at = min(k, units - 1);
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const int at = min(k + i, steps - 1);
-            v[i].w = w[(long long)(4 * at + q) * a.n_experts];
-            __builtin_memcpy(&v[i].x, x + 16 * at + 4 * q, sizeof v[i].x);   // at any address of its type
-        }
+        for (int i = 0; i < 4; ++i) v.w[i] = w[(long long)(16 * at + 4 * q + i) * a.n_experts];
+        __builtin_memcpy(&v.x, x + 64 * at + 16 * q, sizeof v.x);   // at any address of its type
     };
     // The end of the part that position `at` lies in (of narrow rows some parts are empty).
     auto end_of = [&](int at) {
@@ -67,29 +66,29 @@ __global__ void __launch_bounds__(MANY ? 256 : 512) k_route_logits(RouteRowsArgs
         return edge(part);
     };
     int next = end_of(first);
-    auto multiply = [&](int k, const Step (&v)[AHEAD]) {
+    auto multiply = [&](int k, const Unit &v) {
+        if (k >= last) return;
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            if (k + i >= last) continue;
-            const float4 f = v[i].w;
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f.x, (double)(float)v[i].x[0], acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f.y, (double)(float)v[i].x[1], acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f.z, (double)(float)v[i].x[2], acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f.w, (double)(float)v[i].x[3], acc, 0, 0, 0);
-            if (MANY && k + i + 1 == next) {   // the part is done
-                sum += acc;
-                acc = v4d{};
-                next = end_of(k + i + 1);
-            }
+        for (int i = 0; i < 4; ++i) {
+            const float4 f = v.w[i];
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f.x, (double)(float)v.x[4 * i], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f.y, (double)(float)v.x[4 * i + 1], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f.z, (double)(float)v.x[4 * i + 2], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f.w, (double)(float)v.x[4 * i + 3], acc, 0, 0, 0);
+        }
+        if (MANY && k + 1 == next) {   // the part is done
+            sum += acc;
+            acc = v4d{};
+            next = end_of(k + 1);
         }
     };
-    Step v0[AHEAD], v1[AHEAD];
+    Unit v0, v1;
     ask(first, v0);
-    for (int k = first; k < last; k += 2 * AHEAD) {
-        ask(k + AHEAD, v1);
+    for (int k = first; k < last; k += 2) {
+        ask(k + 1, v1);
         multiply(k, v0);
-        ask(k + 2 * AHEAD, v0);
-        multiply(k + AHEAD, v1);
+        ask(k + 2, v0);
+        multiply(k + 1, v1);
     }
     if (!MANY) sum = acc;
     // D: lane l holds row l % 16 and experts 4 i + l / 16
