@@ -16,8 +16,8 @@
 // workgroup with k split over its waves, k_experts_down takes 16 output channels
 // over every used expert, so that the sum over a token's slots ends in one
 // workgroup.  A matrix tile of 16 channels x 16 tokens costs the same for one
-// token as for sixteen, and weights stay in registers for all of an expert's
-// tokens.
+// token as for sixteen, and up to 64 tokens of an expert (in k_experts_down all of
+// them) share one read of its weights.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -32,12 +32,20 @@ namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 
-constexpr int UP_WAVES = 4, WAVES = 8;   // of k_experts_up and k_experts_down
+// Waves of k_experts_up: four, so that a workgroup's start (ids, first weights) and end (the
+// join, silu) are spread over four times as many bytes a wave as with sixteen; eight took
+// 5 to 30% longer (8 tokens, 192 experts of 4096 x 1536: 182 against 160 us), two and one 5 to
+// 20%.  Of k_experts_down, which has one workgroup a CU at n = 4096: sixteen (eight waves of
+// units twice as long took 1 to 4% longer, twelve 1%).
+constexpr int UP_WAVES = 4, WAVES = 16;
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *base, long long bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, (int)(uint32_t)bytes, 0x00020000);
 }
-// 16 bytes at a byte offset, zero past the resource's end.  ONCE: non-temporal.
+// 16 bytes at a byte offset, zero past the resource's end.  Weights are read non-temporally:
+// a layer's used experts do not stay in the last cache until the model comes back to the
+// layer, and pushing nothing out for them is faster in any case (5 tokens 112 against 139 us,
+// 64 tokens 516 against 612).
 template <bool ONCE>
 __device__ __forceinline__ v4i load16(__amdgpu_buffer_rsrc_t r, uint32_t at) {
     return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, ONCE ? 2 : 0));
@@ -158,12 +166,12 @@ __global__ void __launch_bounds__(1024) k_experts_plan(ExpertsArgs a) {
 // ------------------------------------------------------------ gate and up
 //
 // A workgroup has 16 channels of an expert's gate and up; wave w takes the k tiles
-// w, w + 8, ...  Tokens go straight to operand registers: 16 rows x 64 bytes an
+// w, w + 4, ...  Tokens go straight to operand registers: 16 rows x 64 bytes an
 // instruction touch more lines than copies through LDS would, but at most 16 tokens
 // share a tile of weights that comes from HBM at a tenth of what the L1 moves.
 
 // Pairs base .. base + 16 NT - 1 of the expert against this wave's k tiles; D tiles a step.
-template <int NT, int D, bool FEW, bool SHARED, bool ONCE>
+template <int NT, int D, bool FEW, bool SHARED>
 __device__ __forceinline__ void up_tiles(const ExpertsArgs &a, const Used &u, int base, __amdgpu_buffer_rsrc_t rw,
                                          __amdgpu_buffer_rsrc_t rx, int wid, v4i (&g)[NT], v4i (&up)[NT]) {
     const int lane = threadIdx.x & 63;
@@ -181,8 +189,8 @@ __device__ __forceinline__ void up_tiles(const ExpertsArgs &a, const Used &u, in
         for (int d = 0; d < D; ++d) {
             const int k = k0 + d * UP_WAVES;
             // past the last tile: out of the resource's range, zero
-            wg[b][d] = load16<ONCE>(rw, lane * 16 + (k < kt ? k : 2 * kt) * 1024);
-            wu[b][d] = load16<ONCE>(rw, lane * 16 + (k < kt ? kt + k : 2 * kt) * 1024);
+            wg[b][d] = load16<true>(rw, lane * 16 + (k < kt ? k : 2 * kt) * 1024);
+            wu[b][d] = load16<true>(rw, lane * 16 + (k < kt ? kt + k : 2 * kt) * 1024);
         }
 #pragma unroll
         for (int d = 0; d < D; ++d)
@@ -207,13 +215,13 @@ __device__ __forceinline__ void up_tiles(const ExpertsArgs &a, const Used &u, in
     }
 }
 
-template <int NT, int D, bool FEW, bool SHARED, bool ONCE>
+template <int NT, int D, bool FEW, bool SHARED>
 __device__ __forceinline__ void up_item(const ExpertsArgs &a, const Used &u, int base, int c0, __amdgpu_buffer_rsrc_t rw,
                                         const float *gs, const float *us, v4i (*s_sum)[UP_WAVES][64]) {
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const __amdgpu_buffer_rsrc_t rx = rsrc(a.x, (long long)(a.n_tokens - 1) * a.x_stride + a.x_bytes);
     v4i g[NT] = {}, up[NT] = {};
-    up_tiles<NT, D, FEW, SHARED, ONCE>(a, u, base, rw, rx, wid, g, up);
+    up_tiles<NT, D, FEW, SHARED>(a, u, base, rw, rx, wid, g, up);
     const Exp64 ex;
     // One value a thread: token tid / 16, channel tid % 16.
     const int n0 = (tid >> 4) & 15, c = tid & 15, ffn = SHARED ? a.ffn_s : a.ffn;
@@ -244,19 +252,19 @@ __device__ __forceinline__ void up_item(const ExpertsArgs &a, const Used &u, int
 }
 
 // Tiles of 16 tokens at once: as many as the call's tokens can fill.
-template <int NT, bool FEW, bool SHARED, bool ONCE>
+template <int NT, bool FEW, bool SHARED>
 __device__ __forceinline__ void up_expert(const ExpertsArgs &a, const Used &u, int c0, __amdgpu_buffer_rsrc_t rw,
                                           const float *gs, const float *us, v4i (*s_sum)[UP_WAVES][64]) {
     int base = 0;
     if constexpr (NT == 4)
-        for (; u.count - base > 32; base += 64) up_item<4, 1, FEW, SHARED, ONCE>(a, u, base, c0, rw, gs, us, s_sum);
+        for (; u.count - base > 32; base += 64) up_item<4, 1, FEW, SHARED>(a, u, base, c0, rw, gs, us, s_sum);
     if constexpr (NT >= 2)
-        for (; u.count - base > 16; base += 32) up_item<2, 2, FEW, SHARED, ONCE>(a, u, base, c0, rw, gs, us, s_sum);
-    for (; base < u.count; base += 16) up_item<1, 4, FEW, SHARED, ONCE>(a, u, base, c0, rw, gs, us, s_sum);
+        for (; u.count - base > 16; base += 32) up_item<2, 2, FEW, SHARED>(a, u, base, c0, rw, gs, us, s_sum);
+    for (; base < u.count; base += 16) up_item<1, 4, FEW, SHARED>(a, u, base, c0, rw, gs, us, s_sum);
 }
 
 // grid: (channel groups, the shared expert and one for each used expert or pair)
-template <int NT, bool FEW, bool ONCE>
+template <int NT, bool FEW>
 __global__ void __launch_bounds__(64 * UP_WAVES, 4) k_experts_up(ExpertsArgs a) {
     __shared__ v4i s_sum[2][UP_WAVES][64];
     const int grp = blockIdx.x, c0 = grp * 16;
@@ -265,7 +273,7 @@ __global__ void __launch_bounds__(64 * UP_WAVES, 4) k_experts_up(ExpertsArgs a) 
         if (c0 >= a.ffn_s) return;
         const float *s = a.shared.up_scales + grp * 32;
         const Used all{0, a.n_tokens, 0, nullptr};
-        up_expert<NT, FEW, true, ONCE>(a, all, c0, rsrc(a.shared.up + grp * bytes, bytes), s, s + 16, s_sum);
+        up_expert<NT, FEW, true>(a, all, c0, rsrc(a.shared.up + grp * bytes, bytes), s, s + 16, s_sum);
         return;
     }
     if (c0 >= a.ffn) return;
@@ -281,7 +289,7 @@ __global__ void __launch_bounds__(64 * UP_WAVES, 4) k_experts_up(ExpertsArgs a) 
     }
     const ExpertI8 e = a.experts[u.expert];
     const float *s = e.up_scales + grp * 32;
-    up_expert<NT, FEW, false, ONCE>(a, u, c0, rsrc(e.up + grp * bytes, bytes), s, s + 16, s_sum);
+    up_expert<NT, FEW, false>(a, u, c0, rsrc(e.up + grp * bytes, bytes), s, s + 16, s_sum);
 }
 
 // ------------------------------------------------------ int8 rows of h
@@ -381,13 +389,13 @@ __global__ void __launch_bounds__(256) k_experts_quantize(ExpertsArgs a) {
 // tiles) in turn, weights of the next unit on their way during the products of this
 // one; the integer sums of a pair meet in LDS, where their order does not
 // count, and the sum over a token's slots is made from there in the slots' order.
-constexpr int DOWN_TILES = 8;
-constexpr int FUSED_STEPS = 2;   // of 512 elements a wave
+constexpr int DOWN_TILES = 4;
+constexpr int FUSED_STEPS = 1;   // of 512 elements a wave
 
 // FUSED (few pairs): the int8 rows are made here, by every workgroup for itself, in
 // place of a launch of k_experts_quantize; the first weights are on their way meanwhile.
-template <int OUT, bool FEW, bool ONCE, bool FUSED>
-__global__ void __launch_bounds__(64 * WAVES, 2) k_experts_down(ExpertsArgs a) {
+template <int OUT, bool FEW, bool FUSED>
+__global__ void __launch_bounds__(64 * WAVES, 4) k_experts_down(ExpertsArgs a) {
     extern __shared__ __align__(16) int s_sum[];   // [rows][16]; FUSED: int8 rows (shared, then routed), scales
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = blockIdx.x, rows = a.pairs + (a.has_shared ? a.n_tokens : 0);
@@ -420,7 +428,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_experts_down(ExpertsArgs a) {
     auto ask = [&](const Unit &r, v4i (&w)[DOWN_TILES]) {
 #pragma unroll
         for (int d = 0; d < DOWN_TILES; ++d)   // past the last tile: zero
-            w[d] = load16<ONCE>(r.rw, lane * 16 + (r.k0 + d) * 1024);
+            w[d] = load16<true>(r.rw, lane * 16 + (r.k0 + d) * 1024);
     };
     auto tokens = [&](const Unit &r, int row, v4i (&x)[DOWN_TILES]) {
         if constexpr (FUSED) {   // rows end at k tiles: the tiles behind, whose weights are zero, repeat the last
@@ -563,23 +571,23 @@ __global__ void __launch_bounds__(64 * WAVES, 2) k_experts_down(ExpertsArgs a) {
     }
 }
 
-template <bool FEW, bool ONCE>
+template <bool FEW>
 hipError_t launch_up(const ExpertsArgs &a, hipStream_t s) {
     const int widest = a.has_shared && a.ffn_s > a.ffn ? a.ffn_s : a.ffn;
     const int used = FEW || a.pairs < a.n_experts ? a.pairs : a.n_experts;
     const dim3 grid((widest + 15) / 16, used + a.has_shared);
     if (a.n_tokens <= 16)
-        hipLaunchKernelGGL((k_experts_up<1, FEW, ONCE>), grid, dim3(64 * UP_WAVES), 0, s, a);
+        hipLaunchKernelGGL((k_experts_up<1, FEW>), grid, dim3(64 * UP_WAVES), 0, s, a);
     else if (a.n_tokens <= 32)
-        hipLaunchKernelGGL((k_experts_up<2, FEW, ONCE>), grid, dim3(64 * UP_WAVES), 0, s, a);
+        hipLaunchKernelGGL((k_experts_up<2, FEW>), grid, dim3(64 * UP_WAVES), 0, s, a);
     else
-        hipLaunchKernelGGL((k_experts_up<4, FEW, ONCE>), grid, dim3(64 * UP_WAVES), 0, s, a);
+        hipLaunchKernelGGL((k_experts_up<4, FEW>), grid, dim3(64 * UP_WAVES), 0, s, a);
     return hipGetLastError();
 }
 
-template <int OUT, bool FEW, bool ONCE, bool FUSED>
+template <int OUT, bool FEW, bool FUSED>
 hipError_t launch_down(const ExpertsArgs &a, int lds, hipStream_t s) {
-    auto kernel = k_experts_down<OUT, FEW, ONCE, FUSED>;
+    auto kernel = k_experts_down<OUT, FEW, FUSED>;
     if (lds > 64 * 1024) {
         const hipError_t e =
             hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -596,15 +604,15 @@ hipError_t launch_layer(const ExpertsArgs &a, int lds, hipStream_t s) {
         hipLaunchKernelGGL(k_experts_plan, dim3(1), dim3(1024), 0, s, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    if ((e = launch_up<FEW, true>(a, s)) != hipSuccess) return e;
+    if ((e = launch_up<FEW>(a, s)) != hipSuccess) return e;
     if constexpr (!FUSED) {
         hipLaunchKernelGGL(k_experts_quantize, dim3(a.pairs + (a.has_shared ? a.n_tokens : 0)), dim3(256), 0, s, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     switch (a.y_type) {
-    case T_F32: return launch_down<T_F32, FEW, true, FUSED>(a, lds, s);
-    case T_F16: return launch_down<T_F16, FEW, true, FUSED>(a, lds, s);
-    case T_BF16: return launch_down<T_BF16, FEW, true, FUSED>(a, lds, s);
+    case T_F32: return launch_down<T_F32, FEW, FUSED>(a, lds, s);
+    case T_F16: return launch_down<T_F16, FEW, FUSED>(a, lds, s);
+    case T_BF16: return launch_down<T_BF16, FEW, FUSED>(a, lds, s);
     default: return hipErrorInvalidValue;
     }
 }
@@ -617,7 +625,12 @@ hipError_t launch_experts_i8(const ExpertsArgs &a, hipStream_t s) {
         a.n_experts < 1 || a.n_experts > EXPERTS_MAX)
         return hipErrorInvalidValue;
     const int rows = a.pairs + (a.has_shared ? a.n_tokens : 0), sums = rows * 64;
+    // Up to 64 pairs every wave finds its expert's pairs with a few ballots; a launch that sorts
+    // them takes longer (64 pairs, 8 tokens of 4096 x 1536: 154 against 159 us).
     if (a.pairs > 64) return launch_layer<false, false>(a, sums, s);
+    // Rows that fit the waves' registers once are quantized inside k_experts_down: one token
+    // of four experts of 2048 x 1024 11.9 us, with a launch for it 13.0; twice or four times as many
+    // steps gain nothing (one token, eight of 4096 x 1536 and a shared one of 4096: 40.4 and 39.5).
     const long long steps = (long long)a.pairs * ((a.ffn + 511) / 512) + (long long)a.n_tokens * ((a.ffn_s + 511) / 512);
     if (steps <= FUSED_STEPS * WAVES) {
         const int values = 64 * (a.pairs * a.kt_f + (a.has_shared ? a.n_tokens * a.kt_fs : 0));

@@ -918,7 +918,8 @@ class MoeI8Layer:
 
     def __init__(self, be: HipBackend, experts, shared=None):
         self.handle = None
-        self.be, self._keep, self.n_experts = be, (list(experts), shared), len(experts)
+        experts = list(experts)
+        self.be, self._keep, self.n_experts = be, (experts, shared), len(experts)
         pairs = (C.c_void_p * len(experts))(*(e[0].handle for e in experts))
         downs = (C.c_void_p * len(experts))(*(e[1].handle for e in experts))
         h = C.c_void_p()
