@@ -734,8 +734,8 @@ enum lbh_activation {
  *   y = scale * act(gate + bias) * (up + up_bias)         a gated pair, without a residual
  * bias and up_bias (optional, up_bias a pair's only) are float32 [rows].  In float32
  * between the sum and y_type, to which it is rounded once; the activations are good to
- * a few roundings of their value and their argument, and 0 where that is below
- * 2^-119 |v|.  y may be the residual itself, in place.  The same bits for any number
+ * 2^-20 of their value and 2^-22 of it for each unit of their exponent (with float32
+ * outputs mostly to a few roundings), and 0 where they are below 2^-118 |v|.  y may be the residual itself, in place.  The same bits for any number
  * of tokens in the call.  Workspace as for lbh_gemm_i8. */
 lbh_status lbh_gemm_i8_act(lbh_ctx *ctx, const lbh_i8_matrix *m, const int8_t *x_dev, size_t x_stride,
                            const float *x_scales_dev, size_t n_tokens, int32_t activation, const float *bias_dev,
@@ -765,8 +765,8 @@ enum lbh_gate_act {
  * themselves, in place.  v goes to any of y (in y_type), int8 rows with scales (q and
  * scales together) and Q8_K blocks (encoded; n % 256 == 0), each as in
  * lbh_rms_norm_rows and its siblings; without weight there is no v and no such
- * output.  Everything between the loads and the roundings is in 64 bits.  A row gets
- * the same bits among any number of rows, at any addresses and strides (Q8_K: as
+ * output.  Everything between the loads and the roundings is in 64 bits, the gates'
+ * exponentials good to 2^-39.  A row gets the same bits among any number of rows, at any addresses and strides (Q8_K: as
  * lbh_rms_norm_q8_k_rows). */
 lbh_status lbh_block_norm_rows(lbh_ctx *ctx, int32_t type, const void *block_dev, size_t block_stride,
                                const float *post_weight_dev, double post_eps, const void *gate_dev, size_t gate_stride,
@@ -780,7 +780,7 @@ lbh_status lbh_block_norm_rows(lbh_ctx *ctx, int32_t type, const void *block_dev
  * ids ascending, in device memory:
  *   mode 0: by logit, coefs = weight_scale * softmax over the chosen logits
  *   mode 1: by sigmoid(logit) + bias, coefs = weight_scale * sigmoid / max(their sum, 2^-14)
- * in 64 bits, ties to the lower id, coefs and logits (optional, [n_tokens][n_experts])
+ * in 64 bits (exponentials good to 2^-39), ties to the lower id, coefs and logits (optional, [n_tokens][n_experts])
  * rounded to float32.  A row with a logit (or score) that is not finite gets the ids
  * 0 .. top_k - 1 with NaN coefficients.  The same bits for any number of rows, at most
  * 2^19.  Unlike lbh_router_route_into and lbh_route_experts_batch it does not reproduce
@@ -805,7 +805,7 @@ lbh_status lbh_moe_i8_destroy(lbh_moe_i8 *moe);
 /* Workspace bytes of a call (16-byte aligned); calls that may run at once need one each. */
 size_t lbh_moe_i8_workspace_bytes(const lbh_moe_i8 *moe, size_t n_tokens, size_t top_k);
 /* [async] The layer's experts for int8 rows x [n_tokens][n] with a scale each:
- *   h = silu(gate) * up                      of each slot's expert, in 64 bits, rounded to float32
+ *   h = silu(gate) * up     of each slot's expert, in 64 bits (the exponential good to 2^-39), rounded to float32
  *   y[t] = residual[t] + sum over slots coefs[t][slot] * down(int8 row of h) + shared expert of x[t]
  * int8 rows as lbh_quantize_i8_rows makes them, the sums over an expert's products
  * exact, the sum over slots in 64 bits in their order, y rounded to float32 and to
