@@ -735,8 +735,9 @@ enum lbh_activation {
  * bias and up_bias (optional, up_bias a pair's only) are float32 [rows].  In float32
  * between the sum and y_type, to which it is rounded once; the activations are good to
  * 2^-20 of their value and 2^-22 of it for each unit of their exponent (with float32
- * outputs mostly to a few roundings), and 0 where they are below 2^-118 |v|.  y may be the residual itself, in place.  The same bits for any number
- * of tokens in the call.  Workspace as for lbh_gemm_i8. */
+ * outputs mostly to a few roundings), and 0 where they are below 2^-118 |v|.  y may be
+ * the residual itself, in place.  The same bits for any number of tokens in the call.
+ * Workspace as for lbh_gemm_i8. */
 lbh_status lbh_gemm_i8_act(lbh_ctx *ctx, const lbh_i8_matrix *m, const int8_t *x_dev, size_t x_stride,
                            const float *x_scales_dev, size_t n_tokens, int32_t activation, const float *bias_dev,
                            const float *up_bias_dev, double scale, int32_t y_type, void *y_dev, size_t y_stride,

@@ -12,6 +12,9 @@
 // Two norm launches in its place read the sum again and store the normed block
 // between them.  Everything between the loads and the roundings is in 64 bits,
 // for the reasons lbh_norm.hip gives; the order of the sums hangs on n alone.
+// 4096 x 4096 bf16 to int8 rows: 28.6 us without a gate (4.1 TB/s), 46 through a sigmoid or
+// silu, whose 64-bit exponentials bind it then (70 vector instructions for 64 elements); float32
+// rows with the norm behind the block 44.7 us (4.9 TB/s); a single row 3.7 us.
 #include <type_traits>
 
 #include "lbh_dev.h"

@@ -18,6 +18,8 @@
 // workgroup.  A matrix tile of 16 channels x 16 tokens costs the same for one
 // token as for sixteen, and up to 64 tokens of an expert (in k_experts_down all of
 // them) share one read of its weights.
+// 192 experts of 4096 x 1536, top 8, a shared one of 4096: 1 token 39.6 us (5.1 TB/s), 5 111
+// (6.1), 64 516 (6.6).
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
