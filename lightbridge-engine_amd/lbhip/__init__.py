@@ -532,6 +532,7 @@ class HipBackend:
 
     @staticmethod
     def route_rows_workspace_bytes(router: "Router", n_tokens: int) -> int:
+        """For calls of exactly n_tokens; of any number up to it, the larger of this and that of min(n_tokens, 256)."""
         return lib().lbh_router_route_rows_workspace_bytes(router.handle, n_tokens)
 
     def route_rows(self, router: "Router", x, ids, coefs, workspace, mode: int = 0, weight_scale: float = 1.0,
