@@ -13,7 +13,7 @@
 // Bound: each used expert's weights once from HBM, 3 n ffn bytes; the products
 // themselves are a few percent of the matrix cores' rate.  So the launches go
 // by the weights: k_experts_up takes (expert, 16 channels of gate and up) per
-// workgroup with k split over its waves, k_experts_down takes 16 output channels
+// workgroup with k split over its waves, k_experts_down takes 8 or 16 output channels
 // over every used expert, so that the sum over a token's slots ends in one
 // workgroup.  A matrix tile of 16 channels x 16 tokens costs the same for one
 // token as for sixteen, and up to 64 tokens of an expert (in k_experts_down all of
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(256) k_experts_quantize(ExpertsArgs a) {
 
 // ---------------------------------------------------------------- down
 //
-// A workgroup has 16 output channels.  Its waves take units of (expert, DOWN_TILES k
+// A workgroup has CH output channels.  Its waves take units of (expert, DOWN_TILES k
 // tiles) in turn, weights of the next unit on their way during the products of this
 // one; the integer sums of a pair meet in LDS, where their order does not
 // count, and the sum over a token's slots is made from there in the slots' order.
@@ -396,13 +396,14 @@ constexpr int FUSED_STEPS = 1;   // of 512 elements a wave
 
 // FUSED (few pairs): the int8 rows are made here, by every workgroup for itself, in
 // place of a launch of k_experts_quantize; the first weights are on their way meanwhile.
-template <int OUT, bool FEW, bool FUSED>
+template <int OUT, bool FEW, bool FUSED, int CH>
 __global__ void __launch_bounds__(64 * WAVES, 4) k_experts_down(ExpertsArgs a) {
-    extern __shared__ __align__(16) int s_sum[];   // [rows][16]; FUSED: int8 rows (shared, then routed), scales
+    constexpr int PER_LOAD = 16 / CH, LOADS = DOWN_TILES / PER_LOAD;
+    extern __shared__ __align__(16) int s_sum[];   // [rows][CH]; FUSED: int8 rows (shared, then routed), scales
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int grp = blockIdx.x, rows = a.pairs + (a.has_shared ? a.n_tokens : 0);
-    for (int i = tid; i < rows * 4; i += 64 * WAVES) reinterpret_cast<v4i *>(s_sum)[i] = v4i{};
-    uint8_t *s_hq = reinterpret_cast<uint8_t *>(s_sum + rows * 16), *s_hq_r = s_hq + (a.has_shared ? a.n_tokens * a.kt_fs * 64 : 0);
+    const int c0 = blockIdx.x * CH, grp = c0 / 16, rows = a.pairs + (a.has_shared ? a.n_tokens : 0);
+    for (int i = tid; i < rows * CH / 4; i += 64 * WAVES) reinterpret_cast<v4i *>(s_sum)[i] = v4i{};
+    uint8_t *s_hq = reinterpret_cast<uint8_t *>(s_sum + rows * CH), *s_hq_r = s_hq + (a.has_shared ? a.n_tokens * a.kt_fs * 64 : 0);
     float *s_scale = reinterpret_cast<float *>(s_hq_r + a.pairs * a.kt_f * 64);
     (void)s_scale;
     if constexpr (FUSED)
@@ -427,10 +428,13 @@ __global__ void __launch_bounds__(64 * WAVES, 4) k_experts_down(ExpertsArgs a) {
         const int n = min(base + (lane & 15), r.u.count - 1);
         return r.shared ? n : pair_at<FEW>(r.u, n);
     };
-    auto ask = [&](const Unit &r, v4i (&w)[DOWN_TILES]) {
+    // Of the 16 rows a load has for the matrix instruction, CH are channels of one k tile, the next CH those
+    // channels of the next.
+    const int lane_at = ((lane & 48) + c0 % 16 + lane % CH) * 16 + lane % 16 / CH * 1024;
+    auto ask = [&](const Unit &r, v4i (&w)[LOADS]) {
 #pragma unroll
-        for (int d = 0; d < DOWN_TILES; ++d)   // past the last tile: zero
-            w[d] = load16<true>(r.rw, lane * 16 + (r.k0 + d) * 1024);
+        for (int d = 0; d < LOADS; ++d)   // past the last tile: zero
+            w[d] = load16<true>(r.rw, lane_at + (r.k0 + d * PER_LOAD) * 1024);
     };
     auto tokens = [&](const Unit &r, int row, v4i (&x)[DOWN_TILES]) {
         if constexpr (FUSED) {   // rows end at k tiles: the tiles behind, whose weights are zero, repeat the last
@@ -443,17 +447,22 @@ __global__ void __launch_bounds__(64 * WAVES, 4) k_experts_down(ExpertsArgs a) {
 #pragma unroll
         for (int d = 0; d < DOWN_TILES; ++d) x[d] = load16<false>(r.rh, at + d * 64);
     };
-    auto add = [&](const Unit &r, int base, int row, const v4i (&w)[DOWN_TILES], const v4i (&x)[DOWN_TILES]) {
-        v4i acc = {};
+    auto add = [&](const Unit &r, int base, int row, const v4i (&w)[LOADS], const v4i (&x)[DOWN_TILES]) {
+        v4i sums[PER_LOAD] = {};   // the i-th: of every PER_LOAD-th k tile, in rows CH i .. CH i + CH - 1
 #pragma unroll
-        for (int d = 0; d < DOWN_TILES; ++d) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d], x[d], acc, 0, 0, 0);
+        for (int d = 0; d < DOWN_TILES; ++d)
+            sums[d % PER_LOAD] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d / PER_LOAD], x[d], sums[d % PER_LOAD], 0, 0, 0);
+        v4i acc = sums[0];
+#pragma unroll
+        for (int i = 1; i < PER_LOAD; ++i)
+            if ((lane >> 4) * 4 / CH == i) acc = sums[i];
         if (base + (lane & 15) < r.u.count) {
-            int *to = s_sum + ((r.shared ? a.pairs : 0) + row) * 16 + 4 * (lane >> 4);
+            int *to = s_sum + ((r.shared ? a.pairs : 0) + row) * CH + 4 * (lane >> 4) % CH;
 #pragma unroll
             for (int e = 0; e < 4; ++e) atomicAdd(to + e, acc[e]);
         }
     };
-    v4i w0[DOWN_TILES], w1[DOWN_TILES], x0[DOWN_TILES], x1[DOWN_TILES];
+    v4i w0[LOADS], w1[LOADS], x0[DOWN_TILES], x1[DOWN_TILES];
     Unit r0, r1;
     // The shared expert's units come first: their weights can be asked for before the ids are there.
     const int per = (a.kt_f + DOWN_TILES - 1) / DOWN_TILES, first = a.has_shared ? (a.kt_fs + DOWN_TILES - 1) / DOWN_TILES : 0;
@@ -473,7 +482,7 @@ __global__ void __launch_bounds__(64 * WAVES, 4) k_experts_down(ExpertsArgs a) {
         r.rw = rsrc(a.experts[r.u.expert].down + (long long)grp * r.kt * 1024, (long long)r.kt * 1024);
         return r;
     };
-    auto work = [&](const Unit &r, int row, const v4i (&w)[DOWN_TILES], const v4i (&x)[DOWN_TILES]) {
+    auto work = [&](const Unit &r, int row, const v4i (&w)[LOADS], const v4i (&x)[DOWN_TILES]) {
         add(r, 0, row, w, x);
         for (int base = 16; base < r.u.count; base += 16) {   // further tokens of the same weights
             v4i more[DOWN_TILES];
@@ -555,8 +564,8 @@ __global__ void __launch_bounds__(64 * WAVES, 4) k_experts_down(ExpertsArgs a) {
     __syncthreads();
     using T = row_t<OUT>;
     auto scale_of = [&](int row) { return FUSED ? (double)RowScale(s_scale[row]).scale : (double)a.h_scales[row]; };
-    for (int i = tid; i < a.n_tokens * 16; i += 64 * WAVES) {
-        const int t = i >> 4, c = grp * 16 + (i & 15);
+    for (int i = tid; i < a.n_tokens * CH; i += 64 * WAVES) {
+        const int t = i / CH, c = c0 + i % CH;
         if (c >= a.n) continue;
         double sum = 0.0;
         for (int s = 0; s < a.top_k; ++s) {
@@ -564,10 +573,10 @@ __global__ void __launch_bounds__(64 * WAVES, 4) k_experts_down(ExpertsArgs a) {
             const uint32_t id = a.ids[p];
             if (id >= (uint32_t)a.n_experts) continue;
             const double scale = (double)a.coefs[p] * scale_of(p);
-            sum += (double)s_sum[p * 16 + (i & 15)] * (double)a.down_scales[(long long)id * a.down_pitch + c] * scale;
+            sum += (double)s_sum[p * CH + i % CH] * (double)a.down_scales[(long long)id * a.down_pitch + c] * scale;
         }
         if (a.has_shared)
-            sum += (double)s_sum[(a.pairs + t) * 16 + (i & 15)] * (double)a.shared.down_scales[c] * scale_of(a.pairs + t);
+            sum += (double)s_sum[(a.pairs + t) * CH + i % CH] * (double)a.shared.down_scales[c] * scale_of(a.pairs + t);
         if (a.residual) sum += (double)static_cast<const T *>(a.residual)[(long long)t * a.residual_stride + c];
         static_cast<T *>(a.y)[(long long)t * a.y_stride + c] = (T)(float)sum;
     }
@@ -587,20 +596,32 @@ hipError_t launch_up(const ExpertsArgs &a, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <int OUT, bool FEW, bool FUSED>
-hipError_t launch_down(const ExpertsArgs &a, int lds, hipStream_t s) {
-    auto kernel = k_experts_down<OUT, FEW, FUSED>;
+template <int OUT, bool FEW, bool FUSED, int CH>
+hipError_t launch_down(const ExpertsArgs &a, hipStream_t s) {
+    auto kernel = k_experts_down<OUT, FEW, FUSED, CH>;
+    const int rows = a.pairs + (a.has_shared ? a.n_tokens : 0);
+    int lds = rows * CH * 4;
+    if constexpr (FUSED) lds += 64 * (a.pairs * a.kt_f + (a.has_shared ? a.n_tokens * a.kt_fs : 0)) + rows * 4;
     if (lds > 64 * 1024) {
         const hipError_t e =
             hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(kernel, dim3((a.n + 15) / 16), dim3(64 * WAVES), lds, s, a);
+    hipLaunchKernelGGL(kernel, dim3((a.n + CH - 1) / CH), dim3(64 * WAVES), lds, s, a);
     return hipGetLastError();
 }
 
+// Up to 2048 channels sixteen a workgroup leave half the CUs without one, eight (whole 128-byte lines of the
+// tiles) give each of them one: 64 experts of 2048 x 1024, 64 tokens 85.9 -> 80.2 us, 128 of 2048 x 1536 222.6 -> 204.8,
+// 4 tokens 63.0 -> 57.6; one token of the former 11.6 -> 11.8.  Four (half lines) for up to 1024 channels took
+// as long or longer than eight (64 experts of 1024 x 512, 64 tokens 48.8 against 46.2).
+template <int OUT, bool FEW, bool FUSED>
+hipError_t launch_down(const ExpertsArgs &a, hipStream_t s) {
+    return a.n <= 2048 ? launch_down<OUT, FEW, FUSED, 8>(a, s) : launch_down<OUT, FEW, FUSED, 16>(a, s);
+}
+
 template <bool FEW, bool FUSED>
-hipError_t launch_layer(const ExpertsArgs &a, int lds, hipStream_t s) {
+hipError_t launch_layer(const ExpertsArgs &a, hipStream_t s) {
     hipError_t e;
     if constexpr (!FEW) {
         hipLaunchKernelGGL(k_experts_plan, dim3(1), dim3(1024), 0, s, a);
@@ -612,9 +633,9 @@ hipError_t launch_layer(const ExpertsArgs &a, int lds, hipStream_t s) {
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     switch (a.y_type) {
-    case T_F32: return launch_down<T_F32, FEW, FUSED>(a, lds, s);
-    case T_F16: return launch_down<T_F16, FEW, FUSED>(a, lds, s);
-    case T_BF16: return launch_down<T_BF16, FEW, FUSED>(a, lds, s);
+    case T_F32: return launch_down<T_F32, FEW, FUSED>(a, s);
+    case T_F16: return launch_down<T_F16, FEW, FUSED>(a, s);
+    case T_BF16: return launch_down<T_BF16, FEW, FUSED>(a, s);
     default: return hipErrorInvalidValue;
     }
 }
@@ -626,19 +647,15 @@ hipError_t launch_experts_i8(const ExpertsArgs &a, hipStream_t s) {
     if (a.n_tokens > EXPERTS_MAX_TOKENS || a.pairs != a.n_tokens * a.top_k || a.pairs < 1 || a.pairs > EXPERTS_MAX_PAIRS ||
         a.n_experts < 1 || a.n_experts > EXPERTS_MAX)
         return hipErrorInvalidValue;
-    const int rows = a.pairs + (a.has_shared ? a.n_tokens : 0), sums = rows * 64;
     // Up to 64 pairs every wave finds its expert's pairs with a few ballots; a launch that sorts
     // them takes longer (64 pairs, 8 tokens of 4096 x 1536: 154 against 159 us).
-    if (a.pairs > 64) return launch_layer<false, false>(a, sums, s);
+    if (a.pairs > 64) return launch_layer<false, false>(a, s);
     // Rows that fit the waves' registers once are quantized inside k_experts_down: one token
     // of four experts of 2048 x 1024 11.9 us, with a launch for it 13.0; twice or four times as many
     // steps gain nothing (one token, eight of 4096 x 1536 and a shared one of 4096: 40.4 and 39.5).
     const long long steps = (long long)a.pairs * ((a.ffn + 511) / 512) + (long long)a.n_tokens * ((a.ffn_s + 511) / 512);
-    if (steps <= FUSED_STEPS * WAVES) {
-        const int values = 64 * (a.pairs * a.kt_f + (a.has_shared ? a.n_tokens * a.kt_fs : 0));
-        return launch_layer<true, true>(a, sums + values + rows * 4, s);
-    }
-    return launch_layer<true, false>(a, sums, s);
+    if (steps <= FUSED_STEPS * WAVES) return launch_layer<true, true>(a, s);
+    return launch_layer<true, false>(a, s);
 }
 
 }  // namespace lbh
