@@ -791,9 +791,12 @@ lbh_status lbh_router_route_rows(lbh_ctx *ctx, const lbh_router *router, int32_t
                                  size_t n_tokens, size_t top_k, int32_t mode, double weight_scale, uint32_t *ids_dev,
                                  float *coefs_dev, float *logits_dev, void *workspace_dev, size_t workspace_len,
                                  lbh_error *err);
-/* For calls of exactly n_tokens rows.  Up to 256 rows take four times as much a row, so one
- * workspace for any call of up to N rows is the larger of this for N and for min(N, 256). */
+/* For calls of exactly n_tokens rows.  Up to 256 rows take four times as much a row, so a
+ * call of fewer rows may need more. */
 size_t lbh_router_route_rows_workspace_bytes(const lbh_router *router, size_t n_tokens);
+/* For any call of up to n_tokens rows: what a program asks for that keeps one workspace for its
+ * largest batch. */
+size_t lbh_router_route_rows_workspace_bytes_up_to(const lbh_router *router, size_t n_tokens);
 
 /* The experts of a layer: for each a gated pair [ffn x n] and a down matrix [n x ffn], all
  * of one shape, and optionally a shared expert of its own ffn.  The matrices stay the

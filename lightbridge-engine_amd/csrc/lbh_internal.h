@@ -338,9 +338,9 @@ struct RouteRowsArgs {
     double weight_scale;
     int32_t n_tokens, n_experts, hidden, top_k, mode, x_type;
 };
-constexpr int ROUTE_SUMS = 4, ROUTE_PARTS = 8;
+constexpr int ROUTE_SUMS = 4, ROUTE_PARTS = 8, ROUTE_FEW = 256;
 // Sums of a logit that wait in the workspace.
-constexpr int route_parts(long long n_tokens) { return n_tokens <= 256 ? ROUTE_SUMS : 1; }
+constexpr int route_parts(long long n_tokens) { return n_tokens <= ROUTE_FEW ? ROUTE_SUMS : 1; }
 hipError_t launch_route_rows(const RouteRowsArgs &a, hipStream_t s);
 
 // Batch selection: top-k of each token's finished logits (select_route).

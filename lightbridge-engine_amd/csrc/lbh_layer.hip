@@ -164,6 +164,14 @@ size_t lbh_router_route_rows_workspace_bytes(const lbh_router *r, size_t n_token
     return (size_t)route_parts((long long)n_tokens) * n_tokens * r->n_experts * sizeof(double);
 }
 
+size_t lbh_router_route_rows_workspace_bytes_up_to(const lbh_router *r, size_t n_tokens) {
+    if (!r || n_tokens > MAX_ROUTE_TOKENS) return 0;
+    // Rows have as many parts up to ROUTE_FEW as they ever have, and fewer behind it: the most is at one of the two ends.
+    const size_t few = n_tokens < (size_t)ROUTE_FEW ? n_tokens : (size_t)ROUTE_FEW;
+    const size_t all = lbh_router_route_rows_workspace_bytes(r, n_tokens), most = lbh_router_route_rows_workspace_bytes(r, few);
+    return all > most ? all : most;
+}
+
 lbh_status lbh_router_route_rows(lbh_ctx *ctx, const lbh_router *r, int32_t type, const void *x, size_t x_stride,
                                  size_t n_tokens, size_t top_k, int32_t mode, double weight_scale, uint32_t *ids,
                                  float *coefs, float *logits, void *workspace, size_t workspace_len, lbh_error *err) {

@@ -174,6 +174,7 @@ def lib() -> C.CDLL:
                                      sz, sz, i32, p, sz, p, sz, p, p, E], i32),
             "lbh_router_route_rows": ([p, p, i32, p, sz, sz, sz, i32, C.c_double, p, p, p, p, sz, E], i32),
             "lbh_router_route_rows_workspace_bytes": ([p, sz], sz),
+            "lbh_router_route_rows_workspace_bytes_up_to": ([p, sz], sz),
             "lbh_moe_i8_create": ([p, p, p, sz, p, p, C.POINTER(p), E], i32),
             "lbh_moe_i8_destroy": ([p], i32),
             "lbh_moe_i8_workspace_bytes": ([p, sz, sz], sz),
@@ -532,8 +533,13 @@ class HipBackend:
 
     @staticmethod
     def route_rows_workspace_bytes(router: "Router", n_tokens: int) -> int:
-        """For calls of exactly n_tokens; of any number up to it, the larger of this and that of min(n_tokens, 256)."""
+        """For calls of exactly n_tokens rows; a call of fewer may need more."""
         return lib().lbh_router_route_rows_workspace_bytes(router.handle, n_tokens)
+
+    @staticmethod
+    def route_rows_workspace_bytes_up_to(router: "Router", n_tokens: int) -> int:
+        """For any call of up to n_tokens rows: one workspace for the largest batch."""
+        return lib().lbh_router_route_rows_workspace_bytes_up_to(router.handle, n_tokens)
 
     def route_rows(self, router: "Router", x, ids, coefs, workspace, mode: int = 0, weight_scale: float = 1.0,
                    logits=None) -> None:
