@@ -760,7 +760,7 @@ enum lbh_gate_act {
 /* [async] A block's output into the residual stream, and the norm in front of the next
  * block, of `rows` rows of n elements (n <= 16384):
  *   p = block * post_weight / sqrt(mean(block^2) + post_eps)   (post_weight NULL: block)
- *   h = hidden + scale * a(gate) * p            (gate NULL: 1; gate_stride 0: one row for all)
+ *   h = hidden + scale * a(gate) * p            (gate NULL: 1; gate_stride 0: one row for all; scale: a float's range)
  *   v = h * weight / sqrt(mean(h^2) + eps)
  * hidden_out receives h, rounded to float32 and to `type`; it may be hidden or block
  * themselves, in place.  v goes to any of y (in y_type), int8 rows with scales (q and

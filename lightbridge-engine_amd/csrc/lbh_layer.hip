@@ -6,6 +6,7 @@
 // nothing and leaves its outputs as they were.
 #include <hip/hip_runtime.h>
 
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -117,7 +118,8 @@ lbh_status lbh_block_norm_rows(lbh_ctx *ctx, int32_t type, const void *block, si
     if (n > (size_t)BLOCK_NORM_MAX) return fail(err, LBH_UNSUPPORTED_SHAPE, type, 0, BLOCK_NORM_MAX, n);
     if (rows > MAX_TOKENS) return fail(err, LBH_UNSUPPORTED_SHAPE, type, 0, MAX_TOKENS, rows);
     if (encoded && n % 256) return fail(err, LBH_LOGICAL_ELEMENTS_NOT_DIVISIBLE, LBH_Q8_K, 0, 256, n);
-    if (!std::isfinite(scale) || gate_act < GATE_AS_IS || gate_act > GATE_SILU || (!gate && gate_act) ||
+    // (a scale beyond the float range times 1 / sqrt(post_eps) could be infinite, and zeros NaN)
+    if (!(std::fabs(scale) <= FLT_MAX) || gate_act < GATE_AS_IS || gate_act > GATE_SILU || (!gate && gate_act) ||
         (post_weight && !(post_eps > 0.0 && post_eps < HUGE_VAL)) || (weight && !(eps > 0.0 && eps < HUGE_VAL)))
         return fail(err, LBH_INVALID_PARAMETER, type);
     const bool outputs = y || q || scales || encoded;
