@@ -783,7 +783,8 @@ lbh_status lbh_block_norm_rows(lbh_ctx *ctx, int32_t type, const void *block_dev
  *   mode 1: by sigmoid(logit) + bias, coefs = weight_scale * sigmoid / max(their sum, 2^-14)
  * in 64 bits (exponentials good to 2^-39), ties to the lower id, coefs and logits (optional, [n_tokens][n_experts])
  * rounded to float32.  A row with a logit (or score) that is not finite gets the ids
- * 0 .. top_k - 1 with NaN coefficients.  The same bits for any number of rows, at most
+ * 0 .. top_k - 1 with NaN coefficients (so an expert is masked by a bias of the lowest
+ * float, whose score is finite and below all others, not by -infinity).  The same bits for any number of rows, at most
  * 2^19.  Unlike lbh_router_route_into and lbh_route_experts_batch it does not reproduce
  * the reference's 32-bit sums.  Calls that may run at once need a workspace (8-byte
  * aligned) each. */
