@@ -733,10 +733,12 @@ enum lbh_activation {
  *   y = residual + scale * act(v + bias)                  v as in lbh_gemm_i8
  *   y = scale * act(gate + bias) * (up + up_bias)         a gated pair, without a residual
  * bias and up_bias (optional, up_bias a pair's only) are float32 [rows].  In float32
- * between the sum and y_type, to which it is rounded once; the activations are good to
- * 2^-20 of their value and 2^-22 of it for each unit of their exponent (with float32
- * outputs mostly to a few roundings), and 0 where they are below 2^-118 |v|.  y may be
- * the residual itself, in place.  The same bits for any number of tokens in the call.
+ * between the sum and y_type, to which it is rounded once.  The activations are good to
+ * 2^-20 of their value and, for each unit of their exponent, 2^-22 of it with float32
+ * outputs (mostly to a few roundings) and 2^-21 with 16-bit ones, whose exponentials and
+ * reciprocals skip a step (silu of a pair may differ from lbh_gemm_i8_swiglu by one step
+ * of those types, and is the same in float32); 0 where they are below 2^-118 |v|.  y may
+ * be the residual itself, in place.  The same bits for any number of tokens in the call.
  * Workspace as for lbh_gemm_i8. */
 lbh_status lbh_gemm_i8_act(lbh_ctx *ctx, const lbh_i8_matrix *m, const int8_t *x_dev, size_t x_stride,
                            const float *x_scales_dev, size_t n_tokens, int32_t activation, const float *bias_dev,

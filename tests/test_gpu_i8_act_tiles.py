@@ -148,3 +148,25 @@ def test_arguments_far_out_in_the_largest_tile(be, gated, act):
             assert not bool((bad & ~over).any()) and bool(torch.isinf(got[:-2][over]).all())
     finally:
         be.set_tuning(be.TUNE_I8_FORM, 0)
+
+
+@pytest.mark.parametrize("form", [0, *range(1, 12)])
+@pytest.mark.parametrize("ty", [torch.float16, torch.bfloat16])
+def test_silu_of_a_pair_and_swiglu_in_16_bits(be, cases, form, ty):
+    """One formula in two calls: both lie within 2^-16 of it (16 U and 8 U for each unit of an exponent |g| <= 30), far
+    less than a step of 16 bits, so their outputs are the same or neighbours."""
+    c = cases[True]
+    a, b = (torch.zeros(TOKENS, ROWS, dtype=ty, device="cuda") for _ in range(2))
+    g = c.arg(c.w, None)[0]
+    near = g.abs() <= 30
+    assert bool(near.float().mean() > 0.9)
+    try:
+        be.set_tuning(be.TUNE_I8_FORM, form)
+        be.gemm_i8_swiglu(c.m, c.q, c.s, a, c.space)
+        be.gemm_i8_act(c.m, c.q, c.s, b, "silu", c.space)
+    finally:
+        be.set_tuning(be.TUNE_I8_FORM, 0)
+    # neighbours of one sign are one apart as integers; what may go to 0 lies below the type's steps
+    small = (a.abs() < torch.finfo(ty).smallest_normal) & (b.abs() < torch.finfo(ty).smallest_normal)
+    apart = (a.view(torch.int16).int() - b.view(torch.int16).int()).abs()
+    assert bool((apart[near & ~small] <= 1).all())
