@@ -769,8 +769,8 @@ enum lbh_gate_act {
  * scales together) and Q8_K blocks (encoded; n % 256 == 0), each as in
  * lbh_rms_norm_rows and its siblings; without weight there is no v and no such
  * output.  Everything between the loads and the roundings is in 64 bits, the gates'
- * exponentials good to 2^-39.  A row gets the same bits among any number of rows, at any addresses and strides (Q8_K: as
- * lbh_rms_norm_q8_k_rows). */
+ * exponentials good to 2^-38.7.  A row gets the same bits among any number of rows, at
+ * any addresses and strides (Q8_K: as lbh_rms_norm_q8_k_rows). */
 lbh_status lbh_block_norm_rows(lbh_ctx *ctx, int32_t type, const void *block_dev, size_t block_stride,
                                const float *post_weight_dev, double post_eps, const void *gate_dev, size_t gate_stride,
                                int32_t gate_act, double scale, const void *hidden_dev, size_t hidden_stride,
@@ -783,8 +783,8 @@ lbh_status lbh_block_norm_rows(lbh_ctx *ctx, int32_t type, const void *block_dev
  * ids ascending, in device memory:
  *   mode 0: by logit, coefs = weight_scale * softmax over the chosen logits
  *   mode 1: by sigmoid(logit) + bias, coefs = weight_scale * sigmoid / max(their sum, 2^-14)
- * in 64 bits (exponentials good to 2^-39), ties to the lower id, coefs and logits (optional, [n_tokens][n_experts])
- * rounded to float32.  A row with a logit (or score) that is not finite gets the ids
+ * in 64 bits (exponentials good to 2^-38.7), ties to the lower id, coefs and logits
+ * (optional, [n_tokens][n_experts]) rounded to float32.  A row with a logit (or score) that is not finite gets the ids
  * 0 .. top_k - 1 with NaN coefficients (so an expert is masked by a bias of the lowest
  * float, whose score is finite and below all others, not by -infinity).  The same bits for any number of rows, at most
  * 2^19.  Unlike lbh_router_route_into and lbh_route_experts_batch it does not reproduce
@@ -813,7 +813,8 @@ lbh_status lbh_moe_i8_destroy(lbh_moe_i8 *moe);
 /* Workspace bytes of a call (16-byte aligned); calls that may run at once need one each. */
 size_t lbh_moe_i8_workspace_bytes(const lbh_moe_i8 *moe, size_t n_tokens, size_t top_k);
 /* [async] The layer's experts for int8 rows x [n_tokens][n] with a scale each:
- *   h = silu(gate) * up     of each slot's expert, in 64 bits (the exponential good to 2^-39), rounded to float32
+ *   h = silu(gate) * up     of each slot's expert, in 64 bits (the exponential good to
+ *                           2^-38.7), rounded to float32
  *   y[t] = residual[t] + sum over slots coefs[t][slot] * down(int8 row of h) + shared expert of x[t]
  * int8 rows as lbh_quantize_i8_rows makes them, the sums over an expert's products
  * exact, the sum over slots in 64 bits in their order, y rounded to float32 and to
@@ -822,7 +823,8 @@ size_t lbh_moe_i8_workspace_bytes(const lbh_moe_i8 *moe, size_t n_tokens, size_t
  * (as 0xffffffff) is an empty slot, whose coefficient is not used.  residual
  * (optional) may be y itself, in place.  The same bits for any number of tokens and
  * any order of the others.  n_tokens <= 256, n_tokens * top_k <= 2048, top_k <= 16;
- * made for few tokens: every used expert's weights are read once. */
+ * made for few tokens: every used expert's down matrix is read once, its gated pair (and
+ * the shared expert's) once for every 64 tokens that have it. */
 lbh_status lbh_moe_i8_forward(lbh_ctx *ctx, const lbh_moe_i8 *moe, const int8_t *x_dev, size_t x_stride,
                               const float *x_scales_dev, const uint32_t *ids_dev, const float *coefs_dev,
                               size_t n_tokens, size_t top_k, int32_t y_type, void *y_dev, size_t y_stride,

@@ -18,8 +18,9 @@
 // workgroup.  A matrix tile of 16 channels x 16 tokens costs the same for one
 // token as for sixteen, and up to 64 tokens of an expert (in k_experts_down all of
 // them) share one read of its weights.
-// 192 experts of 4096 x 1536, top 8, a shared one of 4096: 1 token 39.6 us (5.1 TB/s), 5 111
-// (6.1), 64 516 (6.6).
+// 192 experts of 4096 x 1536, top 8, a shared one of 4096: 1 token 39.6 us (5.1 TB/s of the used
+// experts' bytes), 5 111 (6.1), 64 516 (6.6); on another machine 64 535 (6.4), 128 601 (6.1), 256 721
+// (5.1: the shared expert's and the hot ones' gate and up are read up to four times).
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -613,7 +614,10 @@ hipError_t launch_down(const ExpertsArgs &a, hipStream_t s) {
 
 // Up to 2048 channels sixteen a workgroup leave half the CUs without one, eight (whole 128-byte lines of the
 // tiles) give each of them one: 64 experts of 2048 x 1024, 64 tokens 85.9 -> 80.2 us, 128 of 2048 x 1536 222.6 -> 204.8,
-// 4 tokens 63.0 -> 57.6; one token of the former 11.6 -> 11.8.  Four (half lines) for up to 1024 channels took
+// 4 tokens 63.0 -> 57.6; one token of the former 11.6 -> 11.8.  Beyond, eight make more workgroups than there are CUs, which
+// run them in turns (top 4 of 64 experts of n x 1024, 4 and 64 tokens, sixteen against eight: n = 2560 32.1 and 103.5
+// against 35.8 and 118.2, 4096 37.6 and 130.4 against 42.0 and 142.8, 5120 50.7 and 187 against 54.3 and 192, 7168 63.7
+// and 230 against 70.8 and 257; one token 13.6 to 23.9 against 16.5 to 29.8).  Four (half lines) for up to 1024 channels took
 // as long or longer than eight (64 experts of 1024 x 512, 64 tokens 48.8 against 46.2).
 template <int OUT, bool FEW, bool FUSED>
 hipError_t launch_down(const ExpertsArgs &a, hipStream_t s) {

@@ -122,8 +122,8 @@ __device__ __forceinline__ float sigmoid_of_16(float g) {
 
 // x times the normal distribution's function of x.  Its lower tail is exp(-a^2 / 2)
 // times a smooth function of a = |x|, here t P(t) with t = 1 / (1 + 0.35 a) and P of degree
-// eight, fitted for the least relative error over 0 <= a <= 14 (3.2e-8); a^2 goes into
-// the exponential in two parts (WIDE: an output of 32 bits).  Past a = 13.2 the tail is 0
+// eight, fitted for the least relative error over 0 <= a <= 14 (as written here, in floats,
+// 6.0e-8 or 2^-24); a^2 goes into the exponential in two parts (WIDE: an output of 32 bits).  Past a = 13.2 the tail is 0
 // (what is right is below 2^-126 there, and up to 2^-122 |x| is given up).
 template <bool WIDE>
 __device__ __forceinline__ float normal_gate(float x) {

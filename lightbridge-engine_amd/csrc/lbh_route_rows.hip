@@ -7,8 +7,8 @@
 //
 // Everything is in 64 bits (products of 32-bit values are exact there), ties go to the
 // lower id, so a choice between two experts does not hang on the order of a
-// sum unless their scores agree to some 1e-14; and that order is the same for any
-// number of rows.  (The router of lbh_router.hip reproduces a sequential 32-bit
+// sum unless their logits agree to some 1e-14 (nor, in mode 1, on the sigmoid's 2^-38.7
+// unless their scores agree to some 1e-12); and that order is the same for any number of rows.  (The router of lbh_router.hip reproduces a sequential 32-bit
 // sum instead, one token at a time, at 4096 dependent additions.)
 //
 // Products run on v_mfma_f64_16x16x4_f64, 16 experts x 16 rows.  The inner dimension

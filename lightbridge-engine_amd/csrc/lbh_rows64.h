@@ -100,12 +100,13 @@ __device__ __forceinline__ double wave_sum(double v) {
     return v;
 }
 
-// The exponential and the sigmoid to some 2^-39 of themselves.  exp(x) = 2^n 2^f with
-// |f| <= 1/2 (n by a 32-bit rounding; the product with log2(e) in 64 bits), 2^f by a
-// polynomial of degree eight through the Chebyshev nodes (off by 2^-38.8 at most), the
-// reciprocal by the hardware's estimate and one step of third order.  The library's
-// exp and division cost more than twice the instructions, and a kernel of gated
-// rows is bound by instructions.  Below g = -708 the sigmoid is 0, as its formula in
+// The exponential and the sigmoid to 2^-38.7 of themselves (measured against the
+// library's: 2^-38.75 and 2^-38.77 at most).  exp(x) = 2^n 2^f with |f| <= 1/2 (n by a
+// 32-bit rounding, which leaves f up to 2^-13 beyond; the product with log2(e) in 64
+// bits), 2^f by a polynomial of degree eight through the Chebyshev nodes (off by 2^-38.77
+// at most, 2^-38.75 with what f is beyond), the reciprocal by the hardware's estimate and
+// one step of third order.  The library's exp and division cost more than twice the
+// instructions, and a kernel of gated rows is bound by instructions.  Below g = -708 the sigmoid is 0, as its formula in
 // 64 bits is from -745.
 struct Exp64 {
     double c[8];
