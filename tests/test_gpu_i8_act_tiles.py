@@ -170,3 +170,22 @@ def test_silu_of_a_pair_and_swiglu_in_16_bits(be, cases, form, ty):
     small = (a.abs() < torch.finfo(ty).smallest_normal) & (b.abs() < torch.finfo(ty).smallest_normal)
     apart = (a.view(torch.int16).int() - b.view(torch.int16).int()).abs()
     assert bool((apart[near & ~small] <= 1).all())
+
+
+@pytest.mark.parametrize("ty", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("kind", ["plain", "residual", "gated"])
+def test_all_forms_give_the_same_bits(be, cases, kind, act, ty):
+    c = cases[kind == "gated"]
+    res = torch.randn(TOKENS, ROWS, device="cuda").to(ty) if kind == "residual" else None
+    outs = []
+    try:
+        for form in range(12):
+            be.set_tuning(be.TUNE_I8_FORM, form)
+            y = torch.zeros(TOKENS, ROWS, dtype=ty, device="cuda")
+            be.gemm_i8_act(c.m, c.q, c.s, y, act, c.space, bias=c.bias, up_bias=c.up_bias if kind == "gated" else None, residual=res,
+                           scale=0.7)
+            outs.append(y)
+    finally:
+        be.set_tuning(be.TUNE_I8_FORM, 0)
+    assert [form for form, y in enumerate(outs) if not torch.equal(y, outs[0])] == []
